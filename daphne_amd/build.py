@@ -71,6 +71,8 @@ def _compile(src: Path) -> Path:
 
 JIT_PRELUDE = """// generated: sources compiled at run time (hiprtc) for fused pipeline bodies
 typedef __SIZE_TYPE__ size_t;
+typedef __INT8_TYPE__ int8_t;
+typedef __UINT8_TYPE__ uint8_t;
 typedef __INT32_TYPE__ int32_t;
 typedef __UINT32_TYPE__ uint32_t;
 typedef __INT64_TYPE__ int64_t;

@@ -97,6 +97,10 @@ def _signatures(lib: C.CDLL) -> None:
             fn = getattr(lib, f"{name}_{suf}", None)
             if fn is not None:
                 fn.argtypes = [ct if a == "T" else a for a in at]
+        for name, n in (("dh_embedding_backward_workspace", 3), ("dh_rmsnorm_backward_workspace", 2),
+                        ("dh_gated_recurrence_workspace", 3)):
+            f(name).argtypes = [sz] * n
+            f(name).restype = sz
     # integer value types: elementwise for all four, aggregations and data reorganisation for 64-bit ones
     for suf, ct in (("si64", C.c_int64), ("ui64", C.c_uint64), ("si32", C.c_int32), ("ui32", C.c_uint32)):
         getattr(lib, f"dh_ew_binary_{suf}").argtypes = [ctxp, i32, vp, sz, vp, sz, sz, sz, vp, sz, sz, sz]
@@ -144,6 +148,17 @@ _LATE_SIGNATURES: dict[str, list] = {
     "dh_maxpool_backward": [vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, sz, sz],
     "dh_avgpool_backward": [vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, sz, sz],
     "dh_conv2d_backward_data": [vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, sz, sz, sz],
+    "dh_embedding_forward": [vp, vp, sz, vp, sz, sz, sz, vp, sz, sz, "T"],
+    "dh_embedding_backward": [vp, vp, sz, sz, sz, vp, sz, vp, sz, sz, "T", i32, vp, sz],
+    "dh_rmsnorm_forward": [vp, vp, sz, vp, sz, vp, vp, sz, sz, sz, vp, sz, vp, "T"],
+    "dh_rmsnorm_forward_q8": [vp, vp, sz, vp, vp, sz, vp, vp, sz, sz, sz, vp, sz, vp, "T"],
+    "dh_rmsnorm_backward": [vp, vp, sz, vp, vp, sz, sz, sz, vp, vp, vp, sz, vp, sz, vp, sz],
+    "dh_gated_recurrence_forward": [vp, vp, sz, vp, sz, vp, sz, sz, sz, vp, sz, vp, sz, vp, sz, sz, vp, sz],
+    "dh_gated_recurrence_backward": [vp, vp, sz, vp, sz, vp, sz, vp, sz, sz, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp, sz, vp, sz, sz,
+                                     vp, sz],
+    "dh_matvec_q4": [vp, vp, sz, vp, sz, sz, sz, vp, sz, sz, vp, sz, sz],
+    "dh_matvec_q4_q8": [vp, vp, sz, vp, sz, sz, sz, vp, vp, sz, sz, vp, sz, sz],
+    "dh_quantize_q4": [vp, vp, sz, vp, sz, vp, sz, sz, sz, sz],
     "dh_conv2d_backward_filter": [vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz, sz, sz, sz],
 }
 

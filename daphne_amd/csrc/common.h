@@ -60,6 +60,7 @@ struct dh_ctx {
     // dh_check_deferred reads that record. The record's host mirror is flag_host + DH_DEFERRED_AT.
     int deferred_depth = 0;
     size_t deferred_enqueued = 0; // checked calls since the last dh_check_deferred (none: nothing to wait for)
+    bool deferred_captured = false; // a checked call sits in a captured graph: its replays may raise at any time
 
     hipEvent_t ev_start = nullptr, ev_stop = nullptr;
     // dh_kernel_timing: pairs of events around the dominant kernel of each timed call since the last reading
@@ -112,18 +113,32 @@ dh_status dh_fail(dh_status st, const char *fmt, ...) __attribute__((format(prin
 // The deferred-verdict record, in ints from flag_dev / flag_host (both are 256 bytes; int 0 is the flag of a checked
 // call and the 8 bytes at byte 64 are the result slot of AggAll):
 //   [0] kind (0: nothing pending)  [1] operator code  [2..3] a 64-bit value  [4..5] a 64-bit bound
-constexpr int DH_DEFERRED_AT = 32, DH_DEFERRED_INTS = 6;
-enum { DH_DEFERRED_NONE = 0, DH_DEFERRED_INT_DIVMOD = 1, DH_DEFERRED_UNARY_DOMAIN = 2, DH_DEFERRED_EXTRACT_COL = 3, DH_DEFERRED_PIPELINE_DOMAIN = 4, DH_DEFERRED_SOLVE_SINGULAR = 5 };
+// DH_IMMEDIATE_AT: a second record of that form, for checked calls that raise from within their kernels (dh_raise) and
+// report at once. Nothing is pending in it between calls.
+constexpr int DH_DEFERRED_AT = 32, DH_DEFERRED_INTS = 6, DH_IMMEDIATE_AT = 48;
+enum { DH_DEFERRED_NONE = 0, DH_DEFERRED_INT_DIVMOD = 1, DH_DEFERRED_UNARY_DOMAIN = 2, DH_DEFERRED_EXTRACT_COL = 3, DH_DEFERRED_PIPELINE_DOMAIN = 4, DH_DEFERRED_SOLVE_SINGULAR = 5, DH_DEFERRED_TOKEN_ID = 6, DH_DEFERRED_OFFSETS = 7 };
 // The failures a checked call reports, immediately or from dh_check_deferred (context.hip).
 dh_status dh_fail_int_divmod(int op);
 dh_status dh_fail_unary_domain(int op);
 dh_status dh_fail_extract_col(long long position, size_t cols);
 dh_status dh_fail_pipeline_domain();
 dh_status dh_fail_solve_singular();
+dh_status dh_fail_token_id(long long id, size_t vocab);
+dh_status dh_fail_offsets(long long offset, size_t tokens);
 // After the kernels of a checked call on a context that defers its verdicts: enqueues the kernel that keeps the
 // call's flag (at ctx->flag_dev, raised if != ok_value) in the deferred record. sel != nullptr: the flag is the
 // index + 1 of the offending entry of sel (stride ld_sel), whose value is kept along with `bound`.
 dh_status dh_latch_deferred(dh_ctx *ctx, int ok_value, int kind, int op, const long long *sel, size_t ld_sel, long long bound);
+
+// Checked calls whose kernels raise by themselves (dh_raise): dh_checked_begin gives the record they raise in, or refuses
+// a call that would have to wait for its verdict inside a stream capture; dh_checked_end waits for the verdict and
+// reports it, or leaves it to dh_check_deferred while the context defers its verdicts.
+dh_status dh_checked_begin(dh_ctx *ctx, const char *what, int **rec);
+dh_status dh_checked_end(dh_ctx *ctx);
+
+// The workspace of a call that takes one from its caller: the caller's if given (refused if it is too small or not
+// aligned to 256 bytes), else the context's, which a captured graph must not hold (a later call may replace it).
+dh_status dh_call_workspace(dh_ctx *ctx, const char *what, void *given, size_t given_bytes, size_t need, void **out);
 
 // Returns a workspace of at least `bytes` bytes (256-byte aligned). Growing frees the old
 // buffer after a stream synchronise.

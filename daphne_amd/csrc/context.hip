@@ -182,6 +182,16 @@ dh_status dh_fail_solve_singular() {
     return dh_fail(DH_ERR_RUNTIME, "A factor Ui is exactly singular, so the solution could not be computed");
 }
 
+dh_status dh_fail_token_id(long long id, size_t vocab) {
+    return dh_fail(DH_ERR_OUT_OF_RANGE, "invalid token '%lld': out of bounds for an embedding table with row boundaries '[0, %zu)'", id,
+                   vocab);
+}
+
+dh_status dh_fail_offsets(long long offset, size_t tokens) {
+    return dh_fail(DH_ERR_OUT_OF_RANGE, "invalid sequence offset '%lld': offsets must not fall and must stay within '[0, %zu]'", offset,
+                   tokens);
+}
+
 // One thread: the record keeps the first failure of the stream's order.
 static __global__ void latch_deferred_kernel(const int *flag, int ok_value, int *rec, int kind, int op, const long long *sel,
                                              size_t ld_sel, long long bound) {
@@ -221,20 +231,8 @@ extern "C" dh_status dh_defer_checks(dh_ctx *ctx, int on) {
     return DH_OK;
 }
 
-extern "C" dh_status dh_check_deferred(dh_ctx *ctx) {
-    DH_REQUIRE_CTX(ctx);
-    if (ctx->deferred_enqueued == 0)
-        return DH_OK; // no checked call since the last verdict: nothing can be pending
-    ctx->deferred_enqueued = 0;
-    int *rec = ctx->flag_host + DH_DEFERRED_AT;
-    DH_CHECK_HIP(hipMemcpyAsync(rec, ctx->flag_dev + DH_DEFERRED_AT, DH_DEFERRED_INTS * sizeof(int), hipMemcpyDeviceToHost,
-                                ctx->stream));
-    DH_CHECK_HIP(hipStreamSynchronize(ctx->stream));
-    if (rec[0] == DH_DEFERRED_NONE)
-        return DH_OK;
-    // a small kernel, not a memset, so that a caller may capture this stream (memset nodes replay badly)
-    hipLaunchKernelGGL(clear_deferred_kernel, dim3(1), dim3(64), 0, ctx->stream, ctx->flag_dev + DH_DEFERRED_AT);
-    DH_CHECK_LAUNCH();
+// The failure a record holds, as the status and message of the call that raised it.
+static dh_status report_record(const int *rec) {
     const long long value = static_cast<long long>((static_cast<unsigned long long>(static_cast<unsigned>(rec[3])) << 32) |
                                                    static_cast<unsigned>(rec[2]));
     const unsigned long long bound = (static_cast<unsigned long long>(static_cast<unsigned>(rec[5])) << 32) | static_cast<unsigned>(rec[4]);
@@ -249,9 +247,82 @@ extern "C" dh_status dh_check_deferred(dh_ctx *ctx) {
         return dh_fail_pipeline_domain();
     case DH_DEFERRED_SOLVE_SINGULAR:
         return dh_fail_solve_singular();
+    case DH_DEFERRED_TOKEN_ID:
+        return dh_fail_token_id(value, static_cast<size_t>(bound));
+    case DH_DEFERRED_OFFSETS:
+        return dh_fail_offsets(value, static_cast<size_t>(bound));
     default:
-        return dh_fail(DH_ERR_RUNTIME, "dh_check_deferred: unknown record kind %d", rec[0]);
+        return dh_fail(DH_ERR_RUNTIME, "unknown record kind %d", rec[0]);
     }
+}
+
+extern "C" dh_status dh_check_deferred(dh_ctx *ctx) {
+    DH_REQUIRE_CTX(ctx);
+    if (ctx->deferred_enqueued == 0 && !ctx->deferred_captured)
+        return DH_OK; // no checked call since the last verdict: nothing can be pending
+    ctx->deferred_enqueued = 0;
+    int *rec = ctx->flag_host + DH_DEFERRED_AT;
+    DH_CHECK_HIP(hipMemcpyAsync(rec, ctx->flag_dev + DH_DEFERRED_AT, DH_DEFERRED_INTS * sizeof(int), hipMemcpyDeviceToHost,
+                                ctx->stream));
+    DH_CHECK_HIP(hipStreamSynchronize(ctx->stream));
+    if (rec[0] == DH_DEFERRED_NONE)
+        return DH_OK;
+    // a small kernel, not a memset, so that a caller may capture this stream (memset nodes replay badly)
+    hipLaunchKernelGGL(clear_deferred_kernel, dim3(1), dim3(64), 0, ctx->stream, ctx->flag_dev + DH_DEFERRED_AT);
+    DH_CHECK_LAUNCH();
+    return report_record(rec);
+}
+
+// Whether the context's stream is being captured into a graph.
+static bool capturing(dh_ctx *ctx) {
+    if (ctx->stream == nullptr)
+        return false;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(ctx->stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+}
+
+dh_status dh_checked_begin(dh_ctx *ctx, const char *what, int **rec) {
+    const bool deferred = ctx->deferred_depth > 0;
+    if (!deferred && capturing(ctx))
+        return dh_fail(DH_ERR_RUNTIME, "%s: the call waits for its check, which a stream capture does not allow; defer it (dh_defer_checks)",
+                       what);
+    *rec = ctx->flag_dev + (deferred ? DH_DEFERRED_AT : DH_IMMEDIATE_AT);
+    return DH_OK;
+}
+
+dh_status dh_checked_end(dh_ctx *ctx) {
+    if (ctx->deferred_depth > 0) {
+        ctx->deferred_enqueued++;
+        if (!ctx->deferred_captured && capturing(ctx))
+            ctx->deferred_captured = true;
+        return DH_OK;
+    }
+    int *rec = ctx->flag_host + DH_IMMEDIATE_AT;
+    DH_CHECK_HIP(hipMemcpyAsync(rec, ctx->flag_dev + DH_IMMEDIATE_AT, DH_DEFERRED_INTS * sizeof(int), hipMemcpyDeviceToHost, ctx->stream));
+    DH_CHECK_HIP(hipStreamSynchronize(ctx->stream));
+    if (rec[0] == DH_DEFERRED_NONE)
+        return DH_OK;
+    hipLaunchKernelGGL(clear_deferred_kernel, dim3(1), dim3(64), 0, ctx->stream, ctx->flag_dev + DH_IMMEDIATE_AT);
+    DH_CHECK_LAUNCH();
+    return report_record(rec);
+}
+
+dh_status dh_call_workspace(dh_ctx *ctx, const char *what, void *given, size_t given_bytes, size_t need, void **out) {
+    *out = nullptr;
+    if (need == 0)
+        return DH_OK;
+    if (given != nullptr) {
+        if (given_bytes < need)
+            return dh_fail(DH_ERR_INVALID_ARG, "%s: the workspace has %zu bytes, %zu are needed", what, given_bytes, need);
+        if (!dh_aligned(given, 256))
+            return dh_fail(DH_ERR_INVALID_ARG, "%s: the workspace is not aligned to 256 bytes", what);
+        *out = given;
+        return DH_OK;
+    }
+    if (capturing(ctx))
+        return dh_fail(DH_ERR_RUNTIME, "%s: inside a stream capture the caller passes the workspace (the context's may be replaced while the "
+                       "graph lives)", what);
+    return dh_workspace(ctx, need, out);
 }
 
 // Capacity class of a request: multiples of 512 B below 64 KiB, above that 1/16 of the largest

@@ -192,3 +192,15 @@ template <typename T, int VEC> __device__ __forceinline__ void dh_store_vec_stre
 }
 // Streaming store of one value that this kernel does not read again (results of a pass over a large input).
 template <typename T> __device__ __forceinline__ void dh_store_stream(T *p, T v) { __builtin_nontemporal_store(v, p); }
+
+// Keeps the first failure that a kernel raises in a six-int record (kind, operator code, value, bound): the thread that
+// turns the kind from 0 writes the rest. The record is read after the stream has drained, or by later work on it.
+__device__ __forceinline__ void dh_raise(int *rec, int kind, int op, long long value, long long bound) {
+    if (atomicCAS(rec, 0, kind) != 0)
+        return;
+    rec[1] = op;
+    rec[2] = static_cast<int>(static_cast<unsigned long long>(value) & 0xffffffffull);
+    rec[3] = static_cast<int>(static_cast<unsigned long long>(value) >> 32);
+    rec[4] = static_cast<int>(static_cast<unsigned long long>(bound) & 0xffffffffull);
+    rec[5] = static_cast<int>(static_cast<unsigned long long>(bound) >> 32);
+}

@@ -1,0 +1,327 @@
+// Root-mean-square norm on a residual stream for DenseMatrix<float|double>: forward (values or 8-bit rows) and backward.
+//
+//   h = x + residual                    (rounded to T: h is the stream's stored value and everything below goes by it)
+//   inv = 1 / sqrt(mean(h^2) + eps)     y = h inv gamma
+//   8 bits: u = h gamma in 64 bits, m = max |u| of the row, code = rint(u (127 / m)), scale = m inv / 127: inv cancels
+//           out of the codes, which therefore do not depend on how the mean was summed
+//   backward: d_h = inv (gamma d_y - h inv^2 mean(gamma d_y h)) + d_sum,   d_gamma = sum over rows of d_y h inv
+//
+// All of it moves whole rows once and is bound by memory. A row is held in the registers of TPR threads (64, 256 or
+// 1024) between its reduction and its result; rows too wide for that are read a second time. Sums over a row are kept in
+// 64 bits: the conversions hide behind the loads, and a row of any length keeps T's precision.
+#pragma once
+
+#include "common.h"
+
+namespace dh_rms {
+
+constexpr int THREADS = 256;
+
+// Sum (or maximum) of a double over the TPR threads of a row, the same value in all of them. `slots`: TPR / 64 doubles of
+// LDS for this row; the barrier before their next use is the caller's second one.
+struct Add {
+    __device__ __forceinline__ double operator()(double a, double b) const { return a + b; }
+};
+struct Max { // a NaN wins, so that it reaches the row's scale
+    __device__ __forceinline__ double operator()(double a, double b) const { return a != a ? a : b != b ? b : (a > b ? a : b); }
+};
+template <int TPR, class Op> __device__ __forceinline__ double over_row(double v, double *slots, Op op) {
+    dh_butterfly(DH_WAVE, [&](auto peer) { v = op(v, peer(v)); });
+    if constexpr (TPR > DH_WAVE) {
+        __syncthreads(); // the slots' last readers
+        if (threadIdx.x % DH_WAVE == 0)
+            slots[threadIdx.x / DH_WAVE] = v;
+        __syncthreads();
+        v = slots[0];
+#pragma unroll
+        for (int w = 1; w < TPR / DH_WAVE; w++)
+            v = op(v, slots[w]);
+    }
+    return v;
+}
+
+template <typename T> struct ForwardArgs {
+    T *res;
+    signed char *codes; // the 8-bit result instead of res
+    T *scale;
+    size_t ld_res;
+    T *sum;
+    size_t ld_sum;
+    T *inv_rms;
+    const T *x;
+    size_t ld_x;
+    const T *residual;
+    size_t ld_r;
+    const T *gamma;
+    size_t rows, cols;
+    double eps;
+};
+
+// What follows the reductions, for one vector of a row.
+template <typename T, int VEC, bool Q8>
+__device__ __forceinline__ void write_vec(const ForwardArgs<T> &a, size_t row, size_t at, const T (&h)[VEC], const T (&g)[VEC], T inv,
+                                          double to_code) {
+    if constexpr (Q8) {
+        signed char q[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            q[e] = static_cast<signed char>(static_cast<int>(rint(static_cast<double>(h[e]) * static_cast<double>(g[e]) * to_code)));
+        if constexpr (VEC == 4) {
+            *reinterpret_cast<unsigned *>(a.codes + row * a.ld_res + at) =
+                (static_cast<unsigned char>(q[0])) | (static_cast<unsigned>(static_cast<unsigned char>(q[1])) << 8) |
+                (static_cast<unsigned>(static_cast<unsigned char>(q[2])) << 16) | (static_cast<unsigned>(static_cast<unsigned char>(q[3])) << 24);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                a.codes[row * a.ld_res + at + e] = q[e];
+        }
+    } else {
+        T y[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            y[e] = h[e] * inv * g[e];
+        dh_store_vec<T, VEC>(a.res + row * a.ld_res + at, y);
+    }
+}
+
+// KV vectors of VEC values a thread, TPR threads a row, max(TPR, THREADS) threads a workgroup. KV = 0: rows of any
+// length, read a second time for the result (from `sum` where there is one, since x may have been replaced by it).
+template <typename T, int VEC, int TPR, int KV, bool Q8>
+__global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void forward_kernel(ForwardArgs<T> a) {
+    constexpr int WG = TPR > THREADS ? TPR : THREADS, RPW = WG / TPR, K = KV ? KV : 1;
+    __shared__ double slots[WG / DH_WAVE];
+    const unsigned lane = threadIdx.x % TPR;
+    const size_t row = static_cast<size_t>(blockIdx.x) * RPW + threadIdx.x / TPR;
+    if (RPW > 1 && row >= a.rows) // whole wavefronts: a row of TPR = 64 meets no barrier
+        return;
+    const size_t vecs = a.cols / VEC;
+    const T *x = a.x + row * a.ld_x, *r = a.residual ? a.residual + row * a.ld_r : nullptr;
+    T *sum = a.sum ? a.sum + row * a.ld_sum : nullptr;
+    double sq = 0.0, most = 0.0;
+    T h[K][VEC], g[K][VEC];
+    if constexpr (KV != 0) {
+        T b[K][VEC];
+#pragma unroll
+        for (int k = 0; k < KV; k++) { // beyond the row: its last vector again, which counts for nothing
+            const size_t j = lane + static_cast<size_t>(k) * TPR, at = (j < vecs ? j : vecs - 1) * VEC;
+            dh_load_vec<T, VEC>(x + at, h[k]);
+            if (r)
+                dh_load_vec<T, VEC>(r + at, b[k]);
+            if (a.gamma)
+                dh_load_vec<T, VEC>(a.gamma + at, g[k]);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    g[k][e] = T(1);
+        }
+#pragma unroll
+        for (int k = 0; k < KV; k++) {
+            const size_t j = lane + static_cast<size_t>(k) * TPR;
+            const bool live = j < vecs;
+            if (r)
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    h[k][e] += b[k][e];
+            if (live && sum)
+                dh_store_vec<T, VEC>(sum + j * VEC, h[k]);
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const double v = live ? static_cast<double>(h[k][e]) : 0.0;
+                sq += v * v;
+                if constexpr (Q8)
+                    most = Max()(most, live ? fabs(v * static_cast<double>(g[k][e])) : 0.0);
+            }
+        }
+    } else {
+        for (size_t j = lane; j < vecs; j += TPR) {
+            dh_load_vec<T, VEC>(x + j * VEC, h[0]);
+            if (r) {
+                T b[VEC];
+                dh_load_vec<T, VEC>(r + j * VEC, b);
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    h[0][e] += b[e];
+            }
+            if (sum)
+                dh_store_vec<T, VEC>(sum + j * VEC, h[0]);
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const double v = static_cast<double>(h[0][e]);
+                sq += v * v;
+                if constexpr (Q8)
+                    most = Max()(most, fabs(v * (a.gamma ? static_cast<double>(a.gamma[j * VEC + e]) : 1.0)));
+            }
+        }
+    }
+    sq = over_row<TPR>(sq, slots, Add());
+    const double inv = 1.0 / sqrt(sq / static_cast<double>(a.cols) + a.eps);
+    if (a.inv_rms && lane == 0)
+        a.inv_rms[row] = static_cast<T>(inv);
+    double to_code = 0.0;
+    if constexpr (Q8) {
+        most = over_row<TPR>(most, slots, Max());
+        // a row of zeros has scale 0; one that holds an infinity or a NaN has no scale: codes 0 and the scale NaN
+        const bool finite = most <= 1.7976931348623157e308;
+        const double unit = static_cast<double>(static_cast<T>(inv));
+        to_code = finite && most > 0.0 ? 127.0 / most : 0.0;
+        if (lane == 0)
+            a.scale[row] = !finite ? static_cast<T>(dh_nan<double>()) : most > 0.0 ? static_cast<T>(most * unit / 127.0) : T(0);
+        if (!finite) {
+            for (size_t c = lane; c < a.cols; c += TPR)
+                a.codes[row * a.ld_res + c] = 0;
+            return; // the whole row's threads
+        }
+    }
+    if constexpr (KV != 0) {
+#pragma unroll
+        for (int k = 0; k < KV; k++) {
+            const size_t j = lane + static_cast<size_t>(k) * TPR;
+            if (j < vecs)
+                write_vec<T, VEC, Q8>(a, row, j * VEC, h[k], g[k], static_cast<T>(inv), to_code);
+        }
+    } else {
+        for (size_t j = lane; j < vecs; j += TPR) {
+            dh_load_vec<T, VEC>((sum ? sum : x) + j * VEC, h[0]);
+            if (r && !sum)
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    h[0][e] += r[j * VEC + e];
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                g[0][e] = a.gamma ? a.gamma[j * VEC + e] : T(1);
+            write_vec<T, VEC, Q8>(a, row, j * VEC, h[0], g[0], static_cast<T>(inv), to_code);
+        }
+    }
+}
+
+template <typename T, int VEC, int TPR, int KV, bool Q8> static inline void launch_forward(dh_ctx *ctx, const ForwardArgs<T> &a) {
+    constexpr int WG = TPR > THREADS ? TPR : THREADS;
+    hipLaunchKernelGGL((forward_kernel<T, VEC, TPR, KV, Q8>), dim3(static_cast<unsigned>(dh_ceil_div(a.rows, WG / TPR))), dim3(WG), 0,
+                       ctx->stream, a);
+}
+
+// The fewest threads a row whose registers hold it with up to four vectors each.
+template <typename T, int VEC, bool Q8> static inline void forward_by_width(dh_ctx *ctx, const ForwardArgs<T> &a) {
+    const size_t vecs = a.cols / VEC;
+    if (vecs <= 64)
+        launch_forward<T, VEC, 64, 1, Q8>(ctx, a);
+    else if (vecs <= 128)
+        launch_forward<T, VEC, 64, 2, Q8>(ctx, a);
+    else if (vecs <= 256)
+        launch_forward<T, VEC, 64, 4, Q8>(ctx, a);
+    else if (vecs <= 512)
+        launch_forward<T, VEC, 256, 2, Q8>(ctx, a);
+    else if (vecs <= 1024)
+        launch_forward<T, VEC, 256, 4, Q8>(ctx, a);
+    else if (vecs <= 4096)
+        launch_forward<T, VEC, 1024, 4, Q8>(ctx, a);
+    else
+        launch_forward<T, VEC, 1024, 0, Q8>(ctx, a);
+}
+
+template <typename T, bool Q8> dh_status forward(dh_ctx *ctx, const ForwardArgs<T> &a) {
+    constexpr const char *what = Q8 ? "rmsNormForwardQ8" : "rmsNormForward";
+    if (a.ld_res < a.cols || a.ld_x < a.cols || (a.sum && a.ld_sum < a.cols) || (a.residual && a.ld_r < a.cols))
+        return dh_fail(DH_ERR_RUNTIME, "%s - a leading dimension is smaller than its column count", what);
+    if (!(a.eps >= 0.0))
+        return dh_fail(DH_ERR_INVALID_ARG, "%s - eps must not be negative", what);
+    if (a.rows > 0 && a.cols > 0 && (a.x == nullptr || (Q8 ? a.codes == nullptr || a.scale == nullptr : a.res == nullptr)))
+        return dh_fail(DH_ERR_RUNTIME, "%s - a matrix is null", what);
+    if (!Q8 && a.res != nullptr && a.res == a.sum)
+        return dh_fail(DH_ERR_INVALID_ARG, "%s - the result and the sum are the same matrix", what);
+    if (a.rows >= (size_t(1) << 31))
+        return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
+    DH_REQUIRE_CTX(ctx);
+    if (a.rows == 0 || a.cols == 0)
+        return DH_OK;
+    constexpr int V = dh_vec<T>::N;
+    const bool vec = a.cols % V == 0 && a.ld_x % V == 0 && dh_aligned(a.x, 16) && (!a.sum || (a.ld_sum % V == 0 && dh_aligned(a.sum, 16))) &&
+                     (!a.residual || (a.ld_r % V == 0 && dh_aligned(a.residual, 16))) && (!a.gamma || dh_aligned(a.gamma, 16)) &&
+                     (Q8 ? a.ld_res % 4 == 0 && dh_aligned(a.codes, 4) : a.ld_res % V == 0 && dh_aligned(a.res, 16));
+    if (vec)
+        forward_by_width<T, V, Q8>(ctx, a);
+    else
+        forward_by_width<T, 1, Q8>(ctx, a);
+    DH_CHECK_LAUNCH();
+    return DH_OK;
+}
+
+// ---------------------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------------------
+template <typename T> struct BackwardArgs {
+    T *dx;
+    size_t ld_dx;
+    T *d_gamma;
+    const T *h;
+    size_t ld_h;
+    const T *inv_rms;
+    const T *gamma;
+    const T *dy;
+    size_t ld_dy;
+    const T *dsum;
+    size_t ld_ds;
+    size_t rows, cols;
+};
+
+// d_h, one row to a workgroup.
+template <typename T> __global__ __launch_bounds__(THREADS) void backward_rows_kernel(BackwardArgs<T> a) {
+    __shared__ double slots[THREADS / DH_WAVE];
+    const size_t row = blockIdx.x;
+    const T *h = a.h + row * a.ld_h, *dy = a.dy + row * a.ld_dy, *ds = a.dsum ? a.dsum + row * a.ld_ds : nullptr;
+    T *dx = a.dx + row * a.ld_dx;
+    const T inv = a.inv_rms[row];
+    double dot = 0.0;
+    for (size_t c = threadIdx.x; c < a.cols; c += THREADS)
+        dot += static_cast<double>(dy[c]) * static_cast<double>(a.gamma ? a.gamma[c] : T(1)) * static_cast<double>(h[c]);
+    dot = over_row<THREADS>(dot, slots, Add());
+    const T k = static_cast<T>(dot / static_cast<double>(a.cols) * static_cast<double>(inv) * static_cast<double>(inv));
+    for (size_t c = threadIdx.x; c < a.cols; c += THREADS) {
+        const T u = dy[c] * (a.gamma ? a.gamma[c] : T(1));
+        dx[c] = inv * (u - h[c] * k) + (ds ? ds[c] : T(0));
+    }
+}
+
+// d_gamma, one thread a column and share of the rows; the shares are added in order.
+template <typename T> __global__ __launch_bounds__(THREADS) void gamma_kernel(BackwardArgs<T> a) {
+    __shared__ double part[THREADS / 32][32];
+    const size_t c = static_cast<size_t>(blockIdx.x) * 32 + threadIdx.x % 32;
+    const unsigned share = threadIdx.x / 32;
+    double s = 0.0;
+    if (c < a.cols)
+        for (size_t r = share; r < a.rows; r += THREADS / 32)
+            s += static_cast<double>(a.dy[r * a.ld_dy + c]) * static_cast<double>(a.h[r * a.ld_h + c]) * static_cast<double>(a.inv_rms[r]);
+    part[share][threadIdx.x % 32] = s;
+    __syncthreads();
+    if (share == 0 && c < a.cols) {
+        for (int k = 1; k < THREADS / 32; k++)
+            s += part[k][threadIdx.x];
+        a.d_gamma[c] = static_cast<T>(s);
+    }
+}
+
+template <typename T> size_t backward_workspace(size_t, size_t) { return 0; }
+
+template <typename T> dh_status backward(dh_ctx *ctx, const BackwardArgs<T> &a, void *ws, size_t ws_bytes) {
+    constexpr const char *what = "rmsNormBackward";
+    if (a.ld_dx < a.cols || a.ld_h < a.cols || a.ld_dy < a.cols || (a.dsum && a.ld_ds < a.cols))
+        return dh_fail(DH_ERR_RUNTIME, "%s - a leading dimension is smaller than its column count", what);
+    if (a.cols > 0 && a.rows > 0 && (a.dx == nullptr || a.h == nullptr || a.inv_rms == nullptr || a.dy == nullptr))
+        return dh_fail(DH_ERR_RUNTIME, "%s - a matrix is null", what);
+    if (a.rows >= (size_t(1) << 31) || a.cols >= (size_t(1) << 31))
+        return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
+    DH_REQUIRE_CTX(ctx);
+    if (a.cols == 0)
+        return DH_OK;
+    void *work = nullptr;
+    if (dh_status st = dh_call_workspace(ctx, what, ws, ws_bytes, backward_workspace<T>(a.rows, a.cols), &work); st != DH_OK)
+        return st;
+    if (a.d_gamma) // before d_x, which may take the place of d_y
+        hipLaunchKernelGGL((gamma_kernel<T>), dim3(static_cast<unsigned>(dh_ceil_div(a.cols, 32))), dim3(THREADS), 0, ctx->stream, a);
+    if (a.rows)
+        hipLaunchKernelGGL((backward_rows_kernel<T>), dim3(static_cast<unsigned>(a.rows)), dim3(THREADS), 0, ctx->stream, a);
+    DH_CHECK_LAUNCH();
+    return DH_OK;
+}
+
+} // namespace dh_rms

@@ -1,0 +1,60 @@
+// Sequence-model kernels, float instantiation. See embed_impl.h, rmsnorm_impl.h and recurrence_impl.h for the mathematics.
+#include "embed_impl.h"
+#include "recurrence_impl.h"
+#include "rmsnorm_impl.h"
+
+static inline const long long *as_ll(const int64_t *p) { return reinterpret_cast<const long long *>(p); }
+
+extern "C" dh_status dh_embedding_forward_f32(dh_ctx *ctx, float *res, size_t ld_res, const float *table, size_t vocab, size_t width,
+                                              size_t ld_table, const int64_t *ids, size_t n, size_t ld_ids, float scale) {
+    return dh_embed::forward<float>(ctx, res, ld_res, table, vocab, width, ld_table, as_ll(ids), n, ld_ids, scale);
+}
+extern "C" size_t dh_embedding_backward_workspace_f32(size_t n, size_t vocab, size_t width) {
+    return dh_embed::backward_workspace<float>(n, vocab, width);
+}
+extern "C" dh_status dh_embedding_backward_f32(dh_ctx *ctx, float *d_table, size_t vocab, size_t width, size_t ld_table, const float *d_out,
+                                               size_t ld_out, const int64_t *ids, size_t n, size_t ld_ids, float scale, int accumulate,
+                                               void *workspace, size_t workspace_bytes) {
+    return dh_embed::backward<float>(ctx, d_table, vocab, width, ld_table, d_out, ld_out, as_ll(ids), n, ld_ids, scale, accumulate, workspace,
+                                   workspace_bytes);
+}
+
+extern "C" dh_status dh_rmsnorm_forward_f32(dh_ctx *ctx, float *res, size_t ld_res, float *sum, size_t ld_sum, float *inv_rms, const float *x,
+                                            size_t rows, size_t cols, size_t ld_x, const float *residual, size_t ld_residual,
+                                            const float *gamma, float eps) {
+    return dh_rms::forward<float, false>(ctx, {res, nullptr, nullptr, ld_res, sum, ld_sum, inv_rms, x, ld_x, residual, ld_residual, gamma, rows,
+                                             cols, static_cast<double>(eps)});
+}
+extern "C" dh_status dh_rmsnorm_forward_q8_f32(dh_ctx *ctx, int8_t *res, size_t ld_res, float *scale, float *sum, size_t ld_sum, float *inv_rms,
+                                               const float *x, size_t rows, size_t cols, size_t ld_x, const float *residual,
+                                               size_t ld_residual, const float *gamma, float eps) {
+    return dh_rms::forward<float, true>(ctx, {nullptr, reinterpret_cast<signed char *>(res), scale, ld_res, sum, ld_sum, inv_rms, x, ld_x,
+                                              residual, ld_residual, gamma, rows, cols, static_cast<double>(eps)});
+}
+extern "C" size_t dh_rmsnorm_backward_workspace_f32(size_t rows, size_t cols) { return dh_rms::backward_workspace<float>(rows, cols); }
+extern "C" dh_status dh_rmsnorm_backward_f32(dh_ctx *ctx, float *dx, size_t ld_dx, float *d_gamma, const float *h, size_t rows, size_t cols,
+                                             size_t ld_h, const float *inv_rms, const float *gamma, const float *d_res, size_t ld_dres,
+                                             const float *d_sum, size_t ld_dsum, void *workspace, size_t workspace_bytes) {
+    return dh_rms::backward<float>(ctx, {dx, ld_dx, d_gamma, h, ld_h, inv_rms, gamma, d_res, ld_dres, d_sum, ld_dsum, rows, cols}, workspace,
+                                 workspace_bytes);
+}
+
+extern "C" size_t dh_gated_recurrence_workspace_f32(size_t tokens, size_t num_seq, size_t channels) {
+    return dh_rec::workspace<float>(tokens, num_seq, channels);
+}
+extern "C" dh_status dh_gated_recurrence_forward_f32(dh_ctx *ctx, float *res, size_t ld_res, float *last, size_t ld_last, const float *x,
+                                                     size_t tokens, size_t channels, size_t ld_x, const float *z, size_t ld_z,
+                                                     const float *h0, size_t ld_h0, const int64_t *offsets, size_t ld_offsets,
+                                                     size_t num_seq, void *workspace, size_t workspace_bytes) {
+    return dh_rec::forward<float>(ctx, res, ld_res, last, ld_last, x, tokens, channels, ld_x, z, ld_z, h0, ld_h0, as_ll(offsets), ld_offsets,
+                                num_seq, workspace, workspace_bytes);
+}
+extern "C" dh_status dh_gated_recurrence_backward_f32(dh_ctx *ctx, float *d_x, size_t ld_dx, float *d_z, size_t ld_dz, float *d_h0,
+                                                      size_t ld_dh0, const float *x, size_t tokens, size_t channels, size_t ld_x,
+                                                      const float *z, size_t ld_z, const float *h, size_t ld_h, const float *h0, size_t ld_h0,
+                                                      const float *d_res, size_t ld_dres, const float *d_last, size_t ld_dlast,
+                                                      const int64_t *offsets, size_t ld_offsets, size_t num_seq, void *workspace,
+                                                      size_t workspace_bytes) {
+    return dh_rec::backward<float>(ctx, d_x, ld_dx, d_z, ld_dz, d_h0, ld_dh0, x, tokens, channels, ld_x, z, ld_z, h, ld_h, h0, ld_h0, d_res,
+                                 ld_dres, d_last, ld_dlast, as_ll(offsets), ld_offsets, num_seq, workspace, workspace_bytes);
+}

@@ -176,7 +176,8 @@ class DenseMatrix:
 
         assert t.is_cuda and t.dim() == 2 and t.stride(1) == 1
         dt = {torch.float32: np.float32, torch.float64: np.float64, torch.int64: np.int64,
-              torch.uint64: np.uint64, torch.int32: np.int32, torch.uint32: np.uint32}[t.dtype]
+              torch.uint64: np.uint64, torch.int32: np.int32, torch.uint32: np.uint32, torch.int8: np.int8,
+              torch.uint8: np.uint8}[t.dtype]
         return DenseMatrix(ctx, t.shape[0], t.shape[1], dt, ptr=t.data_ptr(), row_skip=t.stride(0) if t.shape[0] > 1 else t.shape[1],
                            keepalive=t)
 
@@ -690,3 +691,221 @@ def conv2DBackwardFilter(dFilter, input_: DenseMatrix, output: DenseMatrix, stri
                                                     input_num_channels, input_h, input_w, filter_num_filters, filter_h, filter_w,
                                                     stride_h, stride_w, pad_h, pad_w))
     return dFilter
+
+
+# ------------------------------------------------------------------------------------------
+# sequence models
+# ------------------------------------------------------------------------------------------
+# Rows are tokens, the sequences of a batch one behind the other. `None` as a result makes the kernel allocate it, `None` as
+# an argument that may be missing (residual, gamma, h0, ...) leaves it out. `workspace`: device memory of the caller's for
+# this call (any DenseMatrix of at least ...WorkspaceBytes(...) bytes), needed inside a stream capture.
+def _opt(m: Optional[DenseMatrix]):
+    return (m.ptr, m.row_skip) if m is not None else (None, 0)
+
+
+def _ws(m: Optional[DenseMatrix]):
+    return (m.ptr, ((m.rows - 1) * m.row_skip + m.cols) * m.dtype.itemsize if m.rows else 0) if m is not None else (None, 0)
+
+
+def _shape(name: str, what: str, m: Optional[DenseMatrix], rows: int, cols: int) -> None:
+    if m is not None and (m.rows != rows or m.cols != cols):
+        raise capi.DaphneHipError(capi.DH_ERR_RUNTIME, f"{name}: {what} is {m.rows} x {m.cols}, {rows} x {cols} is needed")
+
+
+def _vector(name: str, what: str, m: Optional[DenseMatrix], n: int):
+    """The values of a row or a column without gaps."""
+    if m is None:
+        return None
+    if m.rows * m.cols != n or min(m.rows, m.cols) != min(1, n) or (m.rows > 1 and m.row_skip != m.cols):
+        raise capi.DaphneHipError(capi.DH_ERR_RUNTIME, f"{name}: {what} is not a vector of {n} values without gaps")
+    return m.ptr
+
+
+def _int64_column(name: str, what: str, m: DenseMatrix, rows: Optional[int] = None) -> None:
+    if m.dtype != np.dtype(np.int64):
+        raise TypeError(f"{name}: {what} must be int64")
+    if m.cols != 1 or (rows is not None and m.rows != rows):
+        raise capi.DaphneHipError(capi.DH_ERR_RUNTIME, f"{name}: {what} must be a column" + (f" of {rows}" if rows is not None else ""))
+
+
+def embeddingForward(res, table: DenseMatrix, ids: DenseMatrix, scale: float, ctx: HIPContext) -> DenseMatrix:
+    """res[i] = scale * table[ids[i]]; `ids` an int64 column of token numbers, each below the table's rows."""
+    dt = _same_dtype(table, res)
+    _int64_column("embeddingForward", "ids", ids)
+    if res is None:
+        res = DenseMatrix(ctx, ids.rows, table.cols, dt)
+    _shape("embeddingForward", "the result", res, ids.rows, table.cols)
+    capi.check(_fn("dh_embedding_forward", dt)(ctx._h, res.ptr, res.row_skip, table.ptr, table.rows, table.cols, table.row_skip,
+                                               ids.ptr, ids.rows, ids.row_skip, scale))
+    return res
+
+
+def embeddingBackwardWorkspaceBytes(n: int, vocab: int, width: int, dtype) -> int:
+    return _fn("dh_embedding_backward_workspace", dtype)(n, vocab, width)
+
+
+def embeddingBackward(dTable, dOut: DenseMatrix, ids: DenseMatrix, vocab: int, scale: float, ctx: HIPContext, accumulate: bool = False,
+                      workspace: Optional[DenseMatrix] = None) -> DenseMatrix:
+    """dTable[v] = scale * the sum of dOut's rows whose token is v (accumulate: added to dTable, which must be given)."""
+    dt = _same_dtype(dOut, dTable)
+    _int64_column("embeddingBackward", "ids", ids, dOut.rows)
+    if dTable is None:
+        if accumulate:
+            raise capi.DaphneHipInvalidArgument(capi.DH_ERR_INVALID_ARG, "embeddingBackward: nothing is given to accumulate into")
+        dTable = DenseMatrix(ctx, vocab, dOut.cols, dt)
+    _shape("embeddingBackward", "the result", dTable, vocab, dOut.cols)
+    capi.check(_fn("dh_embedding_backward", dt)(ctx._h, dTable.ptr, vocab, dOut.cols, dTable.row_skip, dOut.ptr, dOut.row_skip, ids.ptr,
+                                                ids.rows, ids.row_skip, scale, int(accumulate), *_ws(workspace)))
+    return dTable
+
+
+def rmsNormForward(res, resSum, invRms, x: DenseMatrix, residual: Optional[DenseMatrix], gamma: Optional[DenseMatrix], eps: float,
+                   ctx: HIPContext):
+    """h = x + residual, invRms = 1 / sqrt(mean(h^2) + eps) per row, res = h * invRms * gamma. Returns (res, resSum, invRms);
+    resSum is h, which is x itself (and nothing is written) without a residual."""
+    dt = _same_dtype(x, residual, gamma, res, resSum, invRms)
+    if res is None:
+        res = DenseMatrix(ctx, x.rows, x.cols, dt)
+    if resSum is None:
+        resSum = DenseMatrix(ctx, x.rows, x.cols, dt) if residual is not None else x
+    if invRms is None:
+        invRms = DenseMatrix(ctx, x.rows, 1, dt)
+    for what, m in (("residual", residual), ("the result", res), ("the sum", resSum)):
+        _shape("rmsNormForward", what, m, x.rows, x.cols)
+    capi.check(_fn("dh_rmsnorm_forward", dt)(ctx._h, res.ptr, res.row_skip, *(_opt(None) if resSum is x and residual is None else _opt(resSum)),
+                                             _vector("rmsNormForward", "invRms", invRms, x.rows), x.ptr, x.rows, x.cols, x.row_skip,
+                                             *_opt(residual), _vector("rmsNormForward", "gamma", gamma, x.cols), eps))
+    return res, resSum, invRms
+
+
+def rmsNormForwardQ8(res, resScale, resSum, invRms, x: DenseMatrix, residual: Optional[DenseMatrix], gamma: Optional[DenseMatrix],
+                     eps: float, ctx: HIPContext):
+    """rmsNormForward with 8-bit rows: the norm is res (int8) * resScale (one value a row). Returns (res, resScale, resSum, invRms)."""
+    dt = _same_dtype(x, residual, gamma, resScale, resSum, invRms)
+    if res is None:
+        res = DenseMatrix(ctx, x.rows, x.cols, np.int8)
+    if res.dtype != np.dtype(np.int8):
+        raise TypeError("rmsNormForwardQ8: the result must be int8")
+    if resScale is None:
+        resScale = DenseMatrix(ctx, x.rows, 1, dt)
+    if resSum is None:
+        resSum = DenseMatrix(ctx, x.rows, x.cols, dt) if residual is not None else x
+    if invRms is None:
+        invRms = DenseMatrix(ctx, x.rows, 1, dt)
+    for what, m in (("residual", residual), ("the result", res), ("the sum", resSum)):
+        _shape("rmsNormForwardQ8", what, m, x.rows, x.cols)
+    capi.check(_fn("dh_rmsnorm_forward_q8", dt)(ctx._h, res.ptr, res.row_skip, _vector("rmsNormForwardQ8", "resScale", resScale, x.rows),
+                                                *(_opt(None) if resSum is x and residual is None else _opt(resSum)),
+                                                _vector("rmsNormForwardQ8", "invRms", invRms, x.rows), x.ptr, x.rows, x.cols, x.row_skip,
+                                                *_opt(residual), _vector("rmsNormForwardQ8", "gamma", gamma, x.cols), eps))
+    return res, resScale, resSum, invRms
+
+
+def rmsNormBackwardWorkspaceBytes(rows: int, cols: int, dtype) -> int:
+    return _fn("dh_rmsnorm_backward_workspace", dtype)(rows, cols)
+
+
+def rmsNormBackward(dX, dGamma, h: DenseMatrix, invRms: DenseMatrix, gamma: Optional[DenseMatrix], dRes: DenseMatrix,
+                    dSum: Optional[DenseMatrix], ctx: HIPContext, workspace: Optional[DenseMatrix] = None):
+    """Gradients of rmsNormForward, h and invRms being its resSum and invRms: dX is that of x and of residual alike, dSum
+    what comes down the residual stream. Returns (dX, dGamma)."""
+    dt = _same_dtype(h, invRms, gamma, dRes, dSum, dX, dGamma)
+    if dX is None:
+        dX = DenseMatrix(ctx, h.rows, h.cols, dt)
+    if dGamma is None:
+        dGamma = DenseMatrix(ctx, 1, h.cols, dt)
+    for what, m in (("dRes", dRes), ("dSum", dSum), ("the result", dX)):
+        _shape("rmsNormBackward", what, m, h.rows, h.cols)
+    capi.check(_fn("dh_rmsnorm_backward", dt)(ctx._h, dX.ptr, dX.row_skip, _vector("rmsNormBackward", "dGamma", dGamma, h.cols), h.ptr, h.rows,
+                                              h.cols, h.row_skip, _vector("rmsNormBackward", "invRms", invRms, h.rows),
+                                              _vector("rmsNormBackward", "gamma", gamma, h.cols), dRes.ptr, dRes.row_skip, *_opt(dSum),
+                                              *_ws(workspace)))
+    return dX, dGamma
+
+
+def gatedRecurrenceWorkspaceBytes(tokens: int, numSeqs: int, channels: int, dtype) -> int:
+    return _fn("dh_gated_recurrence_workspace", dtype)(tokens, numSeqs, channels)
+
+
+def gatedRecurrenceForward(res, resLast, x: DenseMatrix, z: DenseMatrix, h0: Optional[DenseMatrix], offsets: Optional[DenseMatrix],
+                           numSeqs: int, ctx: HIPContext, workspace: Optional[DenseMatrix] = None):
+    """res_t = f_t * res_{t-1} + (1 - f_t) * x_t with f = sigmoid(z), from h0 (numSeqs x channels). Sequence s has the rows
+    [offsets[s], offsets[s + 1]) (an int64 column of numSeqs + 1), without offsets all have equally many: x.rows = numSeqs is
+    one decoding step. Returns (res, resLast), resLast each sequence's last state; it may be h0 itself."""
+    dt = _same_dtype(x, z, h0, res, resLast)
+    if offsets is not None:
+        _int64_column("gatedRecurrenceForward", "offsets", offsets, numSeqs + 1)
+    if res is None:
+        res = DenseMatrix(ctx, x.rows, x.cols, dt)
+    if resLast is None:
+        resLast = DenseMatrix(ctx, numSeqs, x.cols, dt)
+    for what, m, n in (("z", z, x.rows), ("the result", res, x.rows), ("h0", h0, numSeqs), ("the last state", resLast, numSeqs)):
+        _shape("gatedRecurrenceForward", what, m, n, x.cols)
+    capi.check(_fn("dh_gated_recurrence_forward", dt)(ctx._h, res.ptr, res.row_skip, resLast.ptr, resLast.row_skip, x.ptr, x.rows, x.cols,
+                                                      x.row_skip, z.ptr, z.row_skip, *_opt(h0), *_opt(offsets), numSeqs, *_ws(workspace)))
+    return res, resLast
+
+
+def gatedRecurrenceBackward(dX, dZ, dH0, x: DenseMatrix, z: DenseMatrix, h: DenseMatrix, h0: Optional[DenseMatrix], dRes: DenseMatrix,
+                            dLast: Optional[DenseMatrix], offsets: Optional[DenseMatrix], numSeqs: int, ctx: HIPContext,
+                            workspace: Optional[DenseMatrix] = None):
+    """Gradients of gatedRecurrenceForward, h being its res: returns (dX, dZ, dH0)."""
+    dt = _same_dtype(x, z, h, h0, dRes, dLast, dX, dZ, dH0)
+    if offsets is not None:
+        _int64_column("gatedRecurrenceBackward", "offsets", offsets, numSeqs + 1)
+    if dX is None:
+        dX = DenseMatrix(ctx, x.rows, x.cols, dt)
+    if dZ is None:
+        dZ = DenseMatrix(ctx, x.rows, x.cols, dt)
+    if dH0 is None:
+        dH0 = DenseMatrix(ctx, numSeqs, x.cols, dt)
+    for what, m, n in (("z", z, x.rows), ("h", h, x.rows), ("dRes", dRes, x.rows), ("dX", dX, x.rows), ("dZ", dZ, x.rows),
+                       ("h0", h0, numSeqs), ("dLast", dLast, numSeqs), ("dH0", dH0, numSeqs)):
+        _shape("gatedRecurrenceBackward", what, m, n, x.cols)
+    capi.check(_fn("dh_gated_recurrence_backward", dt)(ctx._h, dX.ptr, dX.row_skip, dZ.ptr, dZ.row_skip, dH0.ptr, dH0.row_skip, x.ptr, x.rows,
+                                                       x.cols, x.row_skip, z.ptr, z.row_skip, h.ptr, h.row_skip, *_opt(h0), dRes.ptr,
+                                                       dRes.row_skip, *_opt(dLast), *_opt(offsets), numSeqs, *_ws(workspace)))
+    return dX, dZ, dH0
+
+
+def _q4_weights(name: str, codes: DenseMatrix, scales: DenseMatrix, rows: int, cols: int, group: int) -> None:
+    if codes.dtype != np.dtype(np.uint8) or scales.dtype != np.dtype(np.float32):
+        raise TypeError(f"{name}: codes must be uint8 and scales float32")
+    if group <= 0:
+        raise capi.DaphneHipInvalidArgument(capi.DH_ERR_INVALID_ARG, f"{name}: the group of {group} columns is not a multiple of 32")
+    _shape(name, "codes", codes, rows, -(-cols // 2))
+    _shape(name, "scales", scales, rows, -(-cols // group))
+
+
+def quantizeQ4(codes, scales, weights: DenseMatrix, group: int, ctx: HIPContext):
+    """Weights (one row per output) as 4-bit codes, two to a byte, and one scale per `group` columns. Returns (codes, scales)."""
+    if group <= 0:
+        raise capi.DaphneHipInvalidArgument(capi.DH_ERR_INVALID_ARG, f"quantizeQ4: the group of {group} columns is not a multiple of 32")
+    if codes is None:
+        codes = DenseMatrix(ctx, weights.rows, -(-weights.cols // 2), np.uint8)
+    if scales is None:
+        scales = DenseMatrix(ctx, weights.rows, -(-weights.cols // group), np.float32)
+    _q4_weights("quantizeQ4", codes, scales, weights.rows, weights.cols, group)
+    capi.check(_fn("dh_quantize_q4", weights.dtype)(ctx._h, codes.ptr, codes.row_skip, scales.ptr, scales.row_skip, weights.ptr, weights.rows,
+                                                    weights.cols, weights.row_skip, group))
+    return codes, scales
+
+
+def matVecQ4(res, x: DenseMatrix, xScale: Optional[DenseMatrix], codes: DenseMatrix, scales: DenseMatrix, group: int,
+             ctx: HIPContext) -> DenseMatrix:
+    """res = x @ t(W) with W as quantizeQ4 gives it; x float32, or int8 with xScale (one value a row) as rmsNormForwardQ8
+    gives it."""
+    if (x.dtype == np.dtype(np.int8)) != (xScale is not None):
+        raise TypeError("matVecQ4: int8 rows need a scale, others have none")
+    _same_dtype(scales, res, xScale, x if xScale is None else None)
+    _q4_weights("matVecQ4", codes, scales, codes.rows, x.cols, group)
+    if res is None:
+        res = DenseMatrix(ctx, x.rows, codes.rows, np.float32)
+    _shape("matVecQ4", "the result", res, x.rows, codes.rows)
+    w = (codes.ptr, codes.rows, codes.row_skip, scales.ptr, scales.row_skip, group)
+    if xScale is None:
+        capi.check(_fn("dh_matvec_q4", x.dtype)(ctx._h, res.ptr, res.row_skip, x.ptr, x.rows, x.cols, x.row_skip, *w))
+    else:
+        capi.check(_fn("dh_matvec_q4_q8", np.float32)(ctx._h, res.ptr, res.row_skip, x.ptr, x.rows, x.cols, x.row_skip,
+                                                      _vector("matVecQ4", "xScale", xScale, x.rows), *w))
+    return res

@@ -663,6 +663,120 @@ dh_status dh_normal_equations_f64(dh_ctx *ctx, double *A, size_t lda, double *b,
                                   size_t cols, size_t ldx, const double *y, size_t ldy, double lambda);
 
 /* ------------------------------------------------------------------------------------ */
+/* sequence models                                                                       */
+/* ------------------------------------------------------------------------------------ */
+/* What a model of token sequences needs around its products: rows by token number and their gradient, the norm on the
+ * residual stream, a recurrence over time, and products with 4-bit weights. They have no counterpart in the reference's
+ * device library. Rows are tokens; the sequences of a batch lie one behind the other without padding.
+ *
+ * Workspaces: entry points that end in (workspace, workspace_bytes) use the caller's device memory if one is given (at
+ * least what the _workspace_ function says for these sizes, aligned to 256 bytes), else the context's own. Inside a
+ * stream capture a workspace has to be given where its size is not 0 (DH_ERR_RUNTIME otherwise): the context's may be
+ * replaced by a later call while the graph lives. Calls that overlap need workspaces of their own.
+ *
+ * Checked calls (token numbers, offsets) wait for their verdict; between dh_defer_checks(ctx, 1) and (ctx, 0) they do
+ * not, and dh_check_deferred reports it. Inside a stream capture the check has to be deferred.
+ *
+ * Results must not overlap inputs except where an entry point says so. */
+
+/* res[i] = scale * table[ids[i]]: res n x width, table vocab x width, ids n x 1 (row stride ld_ids). A token outside
+ * [0, vocab): DH_ERR_OUT_OF_RANGE, its row of res is left as it was, the others are written. (ExtractRow,
+ * kernels/ExtractRow.h, with a factor.) */
+dh_status dh_embedding_forward_f32(dh_ctx *ctx, float *res, size_t ld_res, const float *table, size_t vocab, size_t width,
+                                   size_t ld_table, const int64_t *ids, size_t n, size_t ld_ids, float scale);
+dh_status dh_embedding_forward_f64(dh_ctx *ctx, double *res, size_t ld_res, const double *table, size_t vocab, size_t width,
+                                   size_t ld_table, const int64_t *ids, size_t n, size_t ld_ids, double scale);
+
+/* The table's gradient: d_table[v] = scale * sum of d_out[i] over all i with ids[i] = v, 0 for tokens that do not occur;
+ * accumulate != 0: added to d_table instead (rows of tokens that do not occur are left as they were). A token outside
+ * [0, vocab): DH_ERR_OUT_OF_RANGE, its row of d_out is left out. Sums are taken in 64 bits and in an order that depends on
+ * the sizes and tokens alone. */
+size_t dh_embedding_backward_workspace_f32(size_t n, size_t vocab, size_t width);
+size_t dh_embedding_backward_workspace_f64(size_t n, size_t vocab, size_t width);
+dh_status dh_embedding_backward_f32(dh_ctx *ctx, float *d_table, size_t vocab, size_t width, size_t ld_table, const float *d_out,
+                                    size_t ld_out, const int64_t *ids, size_t n, size_t ld_ids, float scale, int accumulate,
+                                    void *workspace, size_t workspace_bytes);
+dh_status dh_embedding_backward_f64(dh_ctx *ctx, double *d_table, size_t vocab, size_t width, size_t ld_table, const double *d_out,
+                                    size_t ld_out, const int64_t *ids, size_t n, size_t ld_ids, double scale, int accumulate,
+                                    void *workspace, size_t workspace_bytes);
+
+/* Root-mean-square norm: h = x + residual (NULL: h = x), inv_rms = 1 / sqrt(mean(h^2) + eps) per row,
+ * res = h * inv_rms * gamma (gamma: cols values, NULL: ones). `sum` receives h and inv_rms one value a row; each may be
+ * NULL. res or sum may be x or residual itself (same pointer and leading dimension), not both the same matrix.
+ * DH_ERR_INVALID_ARG for a negative eps. */
+dh_status dh_rmsnorm_forward_f32(dh_ctx *ctx, float *res, size_t ld_res, float *sum, size_t ld_sum, float *inv_rms,
+                                 const float *x, size_t rows, size_t cols, size_t ld_x, const float *residual,
+                                 size_t ld_residual, const float *gamma, float eps);
+dh_status dh_rmsnorm_forward_f64(dh_ctx *ctx, double *res, size_t ld_res, double *sum, size_t ld_sum, double *inv_rms,
+                                 const double *x, size_t rows, size_t cols, size_t ld_x, const double *residual,
+                                 size_t ld_residual, const double *gamma, double eps);
+/* The same with 8-bit rows as the result: res[i][j] = rint(127 u / m) with u = h * gamma in 64 bits and m the row's largest
+ * |u|, scale[i] = m * inv_rms / 127, so that res * scale stands for the norm. A row of zeros has scale 0; a row with an
+ * infinity or a NaN has codes 0 and the scale NaN. */
+dh_status dh_rmsnorm_forward_q8_f32(dh_ctx *ctx, int8_t *res, size_t ld_res, float *scale, float *sum, size_t ld_sum,
+                                    float *inv_rms, const float *x, size_t rows, size_t cols, size_t ld_x, const float *residual,
+                                    size_t ld_residual, const float *gamma, float eps);
+/* Gradients of the norm, with h and inv_rms as the forward pass gave them: dx = inv_rms * (gamma * d_res -
+ * h * inv_rms^2 * mean(gamma * d_res * h)) + d_sum, the gradient of x and of residual alike; d_sum (NULL: 0) is what comes
+ * down the residual stream itself. d_gamma (NULL: not computed) = sum over rows of d_res * h * inv_rms. dx may be h, d_res or
+ * d_sum itself (same pointer and leading dimension). */
+size_t dh_rmsnorm_backward_workspace_f32(size_t rows, size_t cols);
+size_t dh_rmsnorm_backward_workspace_f64(size_t rows, size_t cols);
+dh_status dh_rmsnorm_backward_f32(dh_ctx *ctx, float *dx, size_t ld_dx, float *d_gamma, const float *h, size_t rows, size_t cols,
+                                  size_t ld_h, const float *inv_rms, const float *gamma, const float *d_res, size_t ld_dres,
+                                  const float *d_sum, size_t ld_dsum, void *workspace, size_t workspace_bytes);
+dh_status dh_rmsnorm_backward_f64(dh_ctx *ctx, double *dx, size_t ld_dx, double *d_gamma, const double *h, size_t rows, size_t cols,
+                                  size_t ld_h, const double *inv_rms, const double *gamma, const double *d_res, size_t ld_dres,
+                                  const double *d_sum, size_t ld_dsum, void *workspace, size_t workspace_bytes);
+
+/* Gated linear recurrence along the rows of each sequence, every channel by itself:
+ *   f_t = sigmoid(z_t), res_t = f_t * res_{t-1} + (1 - f_t) * x_t, starting from h0 (num_seq x channels, NULL: zeros).
+ * Sequence s has rows [offsets[s], offsets[s + 1]) (offsets: num_seq + 1 values in device memory, row stride ld_offsets);
+ * offsets NULL: tokens / num_seq rows each (DH_ERR_RUNTIME if they do not divide), so that tokens = num_seq is one decoding
+ * step. `last` (num_seq x channels, NULL: not written) receives each sequence's last state, h0's row if it is empty; it may
+ * be h0 itself. Rows outside all sequences are left as they were. Offsets that fall or leave [0, tokens]:
+ * DH_ERR_OUT_OF_RANGE, and the results are undefined (nothing outside them is written).
+ * Backward: d_res and d_last (NULL: 0) are the gradients of res and last, h the forward pass's res; d_x, d_z, and
+ * d_h0 (NULL: not computed). */
+size_t dh_gated_recurrence_workspace_f32(size_t tokens, size_t num_seq, size_t channels);
+size_t dh_gated_recurrence_workspace_f64(size_t tokens, size_t num_seq, size_t channels);
+dh_status dh_gated_recurrence_forward_f32(dh_ctx *ctx, float *res, size_t ld_res, float *last, size_t ld_last, const float *x,
+                                          size_t tokens, size_t channels, size_t ld_x, const float *z, size_t ld_z,
+                                          const float *h0, size_t ld_h0, const int64_t *offsets, size_t ld_offsets,
+                                          size_t num_seq, void *workspace, size_t workspace_bytes);
+dh_status dh_gated_recurrence_forward_f64(dh_ctx *ctx, double *res, size_t ld_res, double *last, size_t ld_last, const double *x,
+                                          size_t tokens, size_t channels, size_t ld_x, const double *z, size_t ld_z,
+                                          const double *h0, size_t ld_h0, const int64_t *offsets, size_t ld_offsets,
+                                          size_t num_seq, void *workspace, size_t workspace_bytes);
+dh_status dh_gated_recurrence_backward_f32(dh_ctx *ctx, float *d_x, size_t ld_dx, float *d_z, size_t ld_dz, float *d_h0,
+                                           size_t ld_dh0, const float *x, size_t tokens, size_t channels, size_t ld_x,
+                                           const float *z, size_t ld_z, const float *h, size_t ld_h, const float *h0, size_t ld_h0,
+                                           const float *d_res, size_t ld_dres, const float *d_last, size_t ld_dlast,
+                                           const int64_t *offsets, size_t ld_offsets, size_t num_seq, void *workspace,
+                                           size_t workspace_bytes);
+dh_status dh_gated_recurrence_backward_f64(dh_ctx *ctx, double *d_x, size_t ld_dx, double *d_z, size_t ld_dz, double *d_h0,
+                                           size_t ld_dh0, const double *x, size_t tokens, size_t channels, size_t ld_x,
+                                           const double *z, size_t ld_z, const double *h, size_t ld_h, const double *h0,
+                                           size_t ld_h0, const double *d_res, size_t ld_dres, const double *d_last,
+                                           size_t ld_dlast, const int64_t *offsets, size_t ld_offsets, size_t num_seq,
+                                           void *workspace, size_t workspace_bytes);
+
+/* res (rows x outs) = x (rows x cols) t(W) with 4-bit weights: W[o][k] = scales[o][k / group] * code, codes in [-8, 7] as
+ * two's complement halves of bytes, row by row (codes: outs rows of ld_codes bytes), the even column in the low half;
+ * scales outs x ceil(cols / group). group is a multiple of 32 (DH_ERR_INVALID_ARG). Made for few rows of x (a decoding
+ * step). _q8_: x as 8-bit rows with one scale each (dh_rmsnorm_forward_q8_f32). */
+dh_status dh_matvec_q4_f32(dh_ctx *ctx, float *res, size_t ld_res, const float *x, size_t rows, size_t cols, size_t ld_x,
+                           const uint8_t *codes, size_t outs, size_t ld_codes, const float *scales, size_t ld_scales,
+                           size_t group);
+dh_status dh_matvec_q4_q8_f32(dh_ctx *ctx, float *res, size_t ld_res, const int8_t *x, size_t rows, size_t cols, size_t ld_x,
+                              const float *x_scale, const uint8_t *codes, size_t outs, size_t ld_codes, const float *scales,
+                              size_t ld_scales, size_t group);
+/* Weights (rows x cols, one row per output) to that form: per group scale = largest |w| / 7, code = rint(w * 7 / largest).
+ * A group of zeros has scale 0; one with an infinity or a NaN has codes 0 and the scale NaN. */
+dh_status dh_quantize_q4_f32(dh_ctx *ctx, uint8_t *codes, size_t ld_codes, float *scales, size_t ld_scales, const float *w,
+                             size_t rows, size_t cols, size_t ld, size_t group);
+
+/* ------------------------------------------------------------------------------------ */
 /* fused vectorized pipeline                                                             */
 /* ------------------------------------------------------------------------------------ */
 /* Device side of VectorizedPipeline<DenseMatrix<VT>>::apply

@@ -1,0 +1,880 @@
+"""GPU: embeddings, the residual RMS norm, the gated recurrence and products with 4-bit weights against plain numpy in 64
+bits (extended precision where the kernels compute in 64 bits themselves). u below is half a step of the value type
+(2^-24 for float, 2^-53 for double); every tolerance counts roundings in it."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+from daphne_amd import capi
+from daphne_amd.kernels import (DenseMatrix, HIPContext, embeddingBackward, embeddingBackwardWorkspaceBytes, embeddingForward,
+                                gatedRecurrenceBackward, gatedRecurrenceForward, gatedRecurrenceWorkspaceBytes, matMul, matVecQ4,
+                                quantizeQ4, rmsNormBackward, rmsNormBackwardWorkspaceBytes, rmsNormForward, rmsNormForwardQ8)
+
+F32, F64 = np.float32, np.float64
+DTYPES = [F32, F64]
+L = np.longdouble
+
+
+def U(dt):
+    return float(np.finfo(dt).eps) / 2
+
+
+def wide(dt):
+    return F64 if dt == F32 else L
+
+
+def D(ctx, a):
+    return DenseMatrix.from_numpy(ctx, a)
+
+
+def view(ctx, a, left=0, right=0, fill=7.0):
+    """`a` as columns [left, left + cols) of a wider matrix: (the view, the whole matrix)."""
+    whole = np.full((a.shape[0], left + a.shape[1] + right), fill, a.dtype)
+    whole[:, left:left + a.shape[1]] = a
+    m = D(ctx, whole)
+    return m.slice(0, a.shape[0], left, left + a.shape[1]), m
+
+
+def near(got, want, tol, what=""):
+    got, want = np.asarray(got, L), np.asarray(want, L)
+    assert got.shape == want.shape, what
+    off = np.abs(got - want) - np.asarray(tol, L)
+    assert np.all(off <= 0), f"{what}: {np.sum(~(off <= 0))} of {off.size} off, worst {np.max(np.abs(got - want))} at {np.unravel_index(np.argmax(off), off.shape)}"
+
+
+# ------------------------------------------------------------------------------------------
+# embeddings
+# ------------------------------------------------------------------------------------------
+def token_ids(rng, n, vocab):
+    """Frequencies fall off as one over the rank."""
+    return np.minimum(((vocab + 1.0) ** rng.random(n) - 1).astype(np.int64), vocab - 1).reshape(-1, 1)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n,vocab,width", [(1, 1, 1), (1, 300, 64), (5, 17, 3), (64, 1000, 512), (100, 50, 129), (1000, 4000, 1000), (33, 9, 4099),
+                                           (70000, 11, 20), (20, 5, 70001)])
+def test_embedding_forward(ctx, dt, n, vocab, width):
+    rng = np.random.default_rng(n + vocab + width)
+    table, ids = rng.standard_normal((vocab, width)).astype(dt), token_ids(rng, n, vocab)
+    ids[-1], ids[0] = vocab - 1, 0
+    for scale in (1.0, -0.37):
+        got = embeddingForward(None, D(ctx, table), D(ctx, ids), scale, ctx).to_numpy()
+        np.testing.assert_array_equal(got, table[ids[:, 0]] * dt(scale))  # one product
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_embedding_forward_views(ctx, dt):
+    rng = np.random.default_rng(5)
+    table, ids = rng.standard_normal((40, 37)).astype(dt), token_ids(rng, 90, 40)
+    for left, right in ((0, 3), (1, 0), (4, 7)):
+        tv, _ = view(ctx, table, left, right)
+        iv, _ = view(ctx, ids, left, right, fill=-5)
+        rv, whole = view(ctx, np.zeros((90, 37), dt), right, left)
+        embeddingForward(rv, tv, iv, 2.5, ctx)
+        np.testing.assert_array_equal(rv.to_numpy()[:, :37], table[ids[:, 0]] * dt(2.5))
+        w = whole.to_numpy()
+        assert np.all(w[:, :right] == 7) and np.all(w[:, right + 37:] == 7)
+
+
+@pytest.mark.parametrize("bad", [-1, 40, 2**40, -2**63, 2**63 - 1])
+def test_tokens_outside_the_table(ctx, bad):
+    rng = np.random.default_rng(6)
+    table, ids = rng.standard_normal((40, 64)).astype(F32), token_ids(rng, 500, 40)
+    ids[123] = bad
+    res = D(ctx, np.full((500, 64), 3, F32))
+    with pytest.raises(IndexError, match=f"'{bad}'.*0, 40"):
+        embeddingForward(res, D(ctx, table), D(ctx, ids), 1.0, ctx)
+    want = table[np.clip(ids[:, 0], 0, 39)]
+    want[123] = 3
+    np.testing.assert_array_equal(res.to_numpy(), want)
+    d_out = rng.standard_normal((500, 64)).astype(F32)
+    with pytest.raises(IndexError, match=f"'{bad}'"):
+        embeddingBackward(None, D(ctx, d_out), D(ctx, ids), 40, 1.0, ctx)
+    # the same calls with their verdicts deferred, and a good call after it is not blamed
+    with pytest.raises(IndexError, match=f"'{bad}'"):
+        with ctx.deferred_checks():
+            embeddingForward(res, D(ctx, table), D(ctx, ids), 1.0, ctx)
+            ids[123] = 7
+            embeddingForward(res, D(ctx, table), D(ctx, ids), 1.0, ctx)
+    embeddingForward(res, D(ctx, table), D(ctx, ids), 1.0, ctx)
+    np.testing.assert_array_equal(res.to_numpy(), table[ids[:, 0]])
+
+
+def embedding_gradient(ids, d_out, vocab, scale, before=None):
+    """The sums in extended precision, and the sum of the magnitudes."""
+    acc, mag = np.zeros((vocab, d_out.shape[1]), L), np.zeros((vocab, d_out.shape[1]), L)
+    np.add.at(acc, ids[:, 0], d_out.astype(L))
+    np.add.at(mag, ids[:, 0], np.abs(d_out.astype(L)))
+    acc, mag = acc * L(scale), mag * abs(L(scale))
+    if before is not None:
+        acc, mag = acc + before, mag + np.abs(before)
+    return acc, mag
+
+
+EMBED_BWD = [(1, 1, 1), (1, 300, 64), (5, 17, 3), (64, 1000, 512), (300, 50, 129), (4096, 70, 33), (4097, 70, 33), (4099, 6000, 260),
+             (9000, 1, 8), (20000, 513, 36), (30000, 40000, 12), (12345, 300000, 5), (50, 3, 5000)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n,vocab,width", EMBED_BWD)
+def test_embedding_backward(ctx, dt, n, vocab, width):
+    rng = np.random.default_rng(n + vocab + width)
+    ids, d_out = token_ids(rng, n, vocab), rng.standard_normal((n, width)).astype(dt)
+    ids[-1], ids[0] = vocab - 1, 0
+    scale = dt(1.7)
+    want, mag = embedding_gradient(ids, d_out, vocab, scale)
+    # additions in 64 bits, each off by 2^-53 of the magnitudes that are in it, n of them at most; then the product and the
+    # rounding to the value type
+    tol = (n + 2) * 2.0**-53 * mag + U(dt) * np.abs(want) * 1.001
+    got = embeddingBackward(None, D(ctx, d_out), D(ctx, ids), vocab, scale, ctx).to_numpy()
+    near(got, want, tol, "gradient")
+    absent = np.setdiff1d(np.arange(vocab), ids)
+    assert not got[absent].any()
+    again = embeddingBackward(None, D(ctx, d_out), D(ctx, ids), vocab, scale, ctx).to_numpy()
+    np.testing.assert_array_equal(got, again)
+    before = rng.standard_normal((vocab, width)).astype(dt)
+    want, mag = embedding_gradient(ids, d_out, vocab, scale, before)
+    tol = (n + 3) * 2.0**-53 * mag + U(dt) * np.abs(want) * 1.001
+    dv, whole = view(ctx, before, 3, 2)
+    embeddingBackward(dv, D(ctx, d_out), D(ctx, ids), vocab, scale, ctx, accumulate=True)
+    got = whole.to_numpy()
+    near(got[:, 3:3 + width], want, tol, "accumulated")
+    np.testing.assert_array_equal(got[absent, 3:3 + width], before[absent])
+    assert np.all(got[:, :3] == 7) and np.all(got[:, 3 + width:] == 7)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_embedding_backward_views_and_no_tokens(ctx, dt):
+    rng = np.random.default_rng(8)
+    for n in (200, 5000):
+        ids, d_out = token_ids(rng, n, 90), rng.standard_normal((n, 21)).astype(dt)
+        iv, _ = view(ctx, ids, 1, 2, fill=-9)
+        dv, _ = view(ctx, d_out, 2, 1)
+        want, mag = embedding_gradient(ids, d_out, 90, 1.0)
+        near(embeddingBackward(None, dv, iv, 90, 1.0, ctx).to_numpy(), want, (n + 2) * 2.0**-53 * mag + U(dt) * np.abs(want) * 1.001)
+    none = embeddingBackward(D(ctx, np.ones((9, 21), dt)), DenseMatrix(ctx, 0, 21, dt), DenseMatrix(ctx, 0, 1, np.int64), 9, 1.0, ctx)
+    assert not none.to_numpy().any()
+    assert embeddingForward(None, D(ctx, np.ones((9, 21), dt)), DenseMatrix(ctx, 0, 1, np.int64), 1.0, ctx).rows == 0
+
+
+# ------------------------------------------------------------------------------------------
+# RMS norm
+# ------------------------------------------------------------------------------------------
+def norm_forward(x, r, g, eps, dt):
+    h = x + r if r is not None else x  # one addition in the value type: what the stream keeps
+    w = h.astype(wide(dt))
+    inv = 1 / np.sqrt((w * w).mean(axis=1, keepdims=True) + wide(dt)(eps))
+    return h, inv, w * inv * (g.astype(wide(dt)) if g is not None else 1)
+
+
+NORM = [(1, 1), (3, 5), (7, 64), (130, 256), (5, 512), (9, 1000), (33, 1023), (4, 2052), (6, 4096), (3, 6001), (2, 16384), (2, 16390), (3, 20004),
+        (2, 70001), (1000, 12)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,cols", NORM)
+def test_rms_norm_forward(ctx, dt, rows, cols):
+    rng = np.random.default_rng(rows * 31 + cols)
+    x, r = (rng.standard_normal((rows, cols)) * 3).astype(dt), rng.standard_normal((rows, cols)).astype(dt)
+    g = (1 + 0.1 * rng.standard_normal((1, cols))).astype(dt)
+    eps = dt(1e-5)
+    for res_, g_ in ((r, g), (None, g), (r, None), (None, None)):
+        h, inv, y = norm_forward(x, res_, g_, eps, dt)
+        got, gsum, ginv = rmsNormForward(None, None, None, D(ctx, x), None if res_ is None else D(ctx, res_), None if g_ is None else D(ctx, g_),
+                                         eps, ctx)
+        np.testing.assert_array_equal(gsum.to_numpy(), h)
+        # the mean in 64 bits: half of its relative error (cols additions, 2^-53 each) in inv; then inv's rounding, and two products
+        rel = cols / 2 * 2.0**-53 + 3 * 2.0**-53
+        near(ginv.to_numpy(), inv, (rel + U(dt)) * np.abs(inv) * 1.001, "inv")
+        near(got.to_numpy(), y, (rel + 3 * U(dt)) * np.abs(y) * 1.001, "norm")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(5, 64), (70, 516), (3, 4100), (2, 20000)])
+def test_rms_norm_forward_views_and_in_place(ctx, dt, rows, cols):
+    rng = np.random.default_rng(cols)
+    x, r = rng.standard_normal((rows, cols)).astype(dt), rng.standard_normal((rows, cols)).astype(dt)
+    g = rng.standard_normal((cols, 1)).astype(dt)
+    h, inv, y = norm_forward(x, r, g.T, 1e-6, dt)
+    tol = ((cols / 2 + 3) * 2.0**-53 + 3 * U(dt)) * np.abs(y) * 1.001
+    for left, right in ((0, 4), (3, 1), (8, 0)):
+        xv, _ = view(ctx, x, left, right)
+        rv, _ = view(ctx, r, right, left)
+        yv, ywhole = view(ctx, np.zeros_like(x), left, right)
+        hv, hwhole = view(ctx, np.zeros_like(x), right, left)
+        rmsNormForward(yv, hv, None, xv, rv, D(ctx, g), 1e-6, ctx)
+        a, b = ywhole.to_numpy(), hwhole.to_numpy()
+        near(a[:, left:left + cols], y, tol)
+        np.testing.assert_array_equal(b[:, right:right + cols], h)
+        for w, l in ((a, left), (b, right)):
+            assert np.all(w[:, :l] == 7) and np.all(w[:, l + cols:] == 7)
+    # the stream is updated in place; the result takes an input's place
+    X, R = D(ctx, x), D(ctx, r)
+    got, _, _ = rmsNormForward(None, R, None, X, R, D(ctx, g), 1e-6, ctx)
+    near(got.to_numpy(), y, tol)
+    np.testing.assert_array_equal(R.to_numpy(), h)
+    X, R = D(ctx, x), D(ctx, r)
+    rmsNormForward(X, R, None, X, R, D(ctx, g), 1e-6, ctx)
+    near(X.to_numpy(), y, tol)
+    np.testing.assert_array_equal(R.to_numpy(), h)
+    X, R = D(ctx, x), D(ctx, r)
+    rmsNormForward(R, X, None, X, R, D(ctx, g), 1e-6, ctx)
+    near(R.to_numpy(), y, tol)
+    np.testing.assert_array_equal(X.to_numpy(), h)
+
+
+@pytest.mark.parametrize("rows,cols", NORM)
+def test_rms_norm_forward_q8(ctx, rows, cols):
+    rng = np.random.default_rng(rows * 31 + cols)
+    x, r = (rng.standard_normal((rows, cols)) * 3).astype(F32), rng.standard_normal((rows, cols)).astype(F32)
+    g = (1 + 0.1 * rng.standard_normal((1, cols))).astype(F32)
+    if rows > 2:
+        x[1], r[1] = 0, 0                                  # a row of zeros
+        x[2] = np.round(x[2])                              # small whole numbers: values on a border between two codes
+        r[2] = 0
+        x[2, 0] = 127
+    for g_ in (g, np.ones_like(g)):
+        h, inv, _ = norm_forward(x, r, g_, F32(1e-5), F32)
+        u = h.astype(F64) * g_.astype(F64)
+        most = np.abs(u).max(axis=1, keepdims=True)
+        want = np.rint(u * np.divide(127.0, most, out=np.zeros_like(most), where=most > 0))
+        res, scale, hs, iv = rmsNormForwardQ8(None, None, None, None, D(ctx, x), D(ctx, r), D(ctx, g_), 1e-5, ctx)
+        np.testing.assert_array_equal(res.to_numpy(), want.astype(np.int8))
+        np.testing.assert_array_equal(hs.to_numpy(), h)
+        # inv rounded to 32 bits, the product rounded once more; cols additions in 64 bits below it
+        near(scale.to_numpy(), most * inv / 127, (2 * U(F32) + (cols / 2 + 6) * 2.0**-53) * (most * inv / 127) * 1.001, "scale")
+        near(iv.to_numpy(), inv, (U(F32) + (cols / 2 + 3) * 2.0**-53) * inv * 1.001, "inv")
+
+
+@pytest.mark.parametrize("cols", [60, 700, 5000, 20001])
+def test_rms_norm_of_rows_that_are_not_finite(ctx, cols):
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((5, cols)).astype(F32)
+    x[1, 3], x[2, cols - 1], x[3, cols // 2] = np.nan, np.inf, -np.inf
+    res, scale, _, inv = rmsNormForwardQ8(None, None, None, None, D(ctx, x), None, None, 1e-5, ctx)
+    s = scale.to_numpy()[:, 0]
+    assert np.array_equal(np.isnan(s), [False, True, True, True, False])
+    assert not res.to_numpy()[1:4].any() and res.to_numpy()[0].any()
+    got, _, inv = rmsNormForward(None, None, None, D(ctx, x), None, None, 1e-5, ctx)
+    got, inv = got.to_numpy(), inv.to_numpy()[:, 0]
+    assert np.isnan(inv[1]) and inv[2] == 0 and inv[3] == 0 and np.isnan(got[1]).all()
+    assert np.isnan(got[2, cols - 1]) and not got[2, :cols - 1].any()  # inf * 0
+    np.testing.assert_array_equal(np.isfinite(got[[0, 4]]), True)
+    # magnitudes whose squares do not fit a float
+    big = np.full((1, cols), 1e30, F32)
+    near(rmsNormForward(None, None, None, D(ctx, big), None, None, 0.0, ctx)[0].to_numpy(), np.ones((1, cols)), 4 * U(F32))
+
+
+def norm_backward(h, inv, g, dy, ds, dt):
+    w = wide(dt)
+    h, inv, dy = h.astype(w), inv.astype(w), dy.astype(w)
+    u = dy * (g.astype(w) if g is not None else 1)
+    k = inv * inv * (u * h).mean(axis=1, keepdims=True)
+    dx = inv * (u - h * k) + (ds.astype(w) if ds is not None else 0)
+    # roundings: u, k, h k, the difference, the product with inv, the sum: at most 6 of these magnitudes; the mean's
+    # cols additions in 64 bits
+    mag = inv * (np.abs(u) + np.abs(h * k)) + (np.abs(ds.astype(w)) if ds is not None else 0)
+    mean = np.abs(inv * h * inv * inv) * (np.abs(u * h).mean(axis=1, keepdims=True))
+    tol = 6 * U(dt) * mag * 1.001 + (h.shape[1] + 4) * 2.0**-53 * mean
+    dg = (dy * h * inv).sum(axis=0, keepdims=True)
+    mg = np.abs(dy * h * inv).sum(axis=0, keepdims=True)
+    return dx, tol, dg, mg
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,cols", NORM + [(5000, 36), (700, 2560)])
+def test_rms_norm_backward(ctx, dt, rows, cols):
+    rng = np.random.default_rng(rows + cols)
+    h, dy = rng.standard_normal((rows, cols)).astype(dt), rng.standard_normal((rows, cols)).astype(dt)
+    g, ds = (1 + 0.1 * rng.standard_normal((1, cols))).astype(dt), rng.standard_normal((rows, cols)).astype(dt)
+    inv = (1 / np.sqrt((h.astype(F64) ** 2).mean(axis=1, keepdims=True) + 1e-5)).astype(dt)
+    for g_, ds_ in ((g, ds), (None, None)):
+        dx, tol, dg, mg = norm_backward(h, inv, g_, dy, ds_, dt)
+        opt = lambda m: None if m is None else D(ctx, m)  # noqa: E731
+        got, gg = rmsNormBackward(None, None, D(ctx, h), D(ctx, inv), opt(g_), D(ctx, dy), opt(ds_), ctx)
+        near(got.to_numpy(), dx, tol, "dx")
+        # shares of the rows are rounded to the value type once, and their sum once; in double every addition counts
+        dtol = 2 * U(dt) * mg * 1.001 + (rows + 4) * 2.0**-53 * mg
+        near(gg.to_numpy(), dg, dtol, "dgamma")
+        again, gg2 = rmsNormBackward(None, None, D(ctx, h), D(ctx, inv), opt(g_), D(ctx, dy), opt(ds_), ctx)
+        np.testing.assert_array_equal(got.to_numpy(), again.to_numpy())
+        np.testing.assert_array_equal(gg.to_numpy(), gg2.to_numpy())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(40, 68), (11, 1027), (5, 20000)])
+def test_rms_norm_backward_views_and_in_place(ctx, dt, rows, cols):
+    rng = np.random.default_rng(cols)
+    h, dy, ds = (rng.standard_normal((rows, cols)).astype(dt) for _ in range(3))
+    g, inv = rng.standard_normal((1, cols)).astype(dt), (rng.random((rows, 1)) + 0.5).astype(dt)
+    dx, tol, dg, mg = norm_backward(h, inv, g, dy, ds, dt)
+    dtol = 2 * U(dt) * mg * 1.001 + (rows + 4) * 2.0**-53 * mg
+    hv, yv, sv = view(ctx, h, 1, 2)[0], view(ctx, dy, 4, 0)[0], view(ctx, ds, 0, 3)[0]
+    xv, whole = view(ctx, np.zeros_like(h), 2, 1)
+    _, gg = rmsNormBackward(xv, None, hv, D(ctx, inv), D(ctx, g), yv, sv, ctx)
+    w = whole.to_numpy()
+    near(w[:, 2:2 + cols], dx, tol)
+    near(gg.to_numpy(), dg, dtol)
+    assert np.all(w[:, :2] == 7) and np.all(w[:, 2 + cols:] == 7)
+    for place in range(3):
+        m = [D(ctx, h), D(ctx, dy), D(ctx, ds)]
+        _, gg = rmsNormBackward(m[place], None, m[0], D(ctx, inv), D(ctx, g), m[1], m[2], ctx)
+        near(m[place].to_numpy(), dx, tol)
+        near(gg.to_numpy(), dg, dtol)
+
+
+def test_rms_norm_gradient_against_differences(ctx):
+    rng = np.random.default_rng(3)
+    x, r, g, c = (rng.standard_normal(s) for s in ((3, 40), (3, 40), (1, 40), (3, 40)))
+    def loss(x_, g_):
+        return float((rmsNormForward(None, None, None, D(ctx, x_), D(ctx, r), D(ctx, g_), 1e-3, ctx)[0].to_numpy() * c).sum())
+    _, h, inv = rmsNormForward(None, None, None, D(ctx, x), D(ctx, r), D(ctx, g), 1e-3, ctx)
+    dx, dg = (m.to_numpy() for m in rmsNormBackward(None, None, h, inv, D(ctx, g), D(ctx, c), None, ctx))
+    step = 1e-5  # central differences: step^2 of the third derivative (of order 1 to 100), and 2^-53 |loss| / step
+    for i, j in ((0, 0), (1, 7), (2, 39)):
+        e = np.zeros_like(x)
+        e[i, j] = step
+        assert abs((loss(x + e, g) - loss(x - e, g)) / (2 * step) - dx[i, j]) < 1e-7
+        e = np.zeros_like(g)
+        e[0, j] = step
+        assert abs((loss(x, g + e) - loss(x, g - e)) / (2 * step) - dg[0, j]) < 1e-7
+
+
+# ------------------------------------------------------------------------------------------
+# gated recurrence
+# ------------------------------------------------------------------------------------------
+def rec_forward(x, z, h0, starts, dt):
+    """h, the last states, and tolerances. Every term of h_t is a product of one (1 - f) x (or h0) with the f behind it;
+    `count` is the sum of the terms' magnitudes times their number of factors."""
+    w = wide(dt)
+    x, z, h0 = x.astype(w), z.astype(w), h0.astype(w)
+    f, om = 1 / (1 + np.exp(-z)), 1 / (1 + np.exp(z))
+    n, c = x.shape
+    h, mag, count = np.full((n, c), np.nan, w), np.zeros((n, c), w), np.zeros((n, c), w)
+    last, ltol = h0.copy(), np.zeros_like(h0)
+    tol = rec_delta(z, dt)
+    for s, (a, e) in enumerate(zip(starts[:-1], starts[1:])):
+        hp, m, k = h0[s], np.abs(h0[s]), np.zeros(c, w)
+        for t in range(a, e):
+            hp = f[t] * hp + om[t] * x[t]
+            k = f[t] * (k + m) + om[t] * np.abs(x[t])
+            m = f[t] * m + om[t] * np.abs(x[t])
+            h[t], mag[t], count[t] = hp, m, k
+        if e > a:
+            last[s], ltol[s] = hp, tol * count[e - 1] + 16 * U(dt) * mag[e - 1]
+    return h, last, tol * count + 16 * U(dt) * mag, ltol
+
+
+def rec_delta(z, dt):
+    """Relative error of a factor and its product: exp of -|z| is off by the argument's rounding, |z| half steps, and 3 of its
+    own; the sum, the quotient and the product of a gate add 3, the factor's product and sum in the recurrence 2."""
+    return (float(np.max(np.abs(z), initial=0)) + 8) * U(dt)
+
+
+def rec_backward(x, z, h, h0, d_out, d_last, starts, dt):
+    w = wide(dt)
+    x, z, h, h0, d_out, d_last = (m.astype(w) for m in (x, z, h, h0, d_out, d_last))
+    f, om = 1 / (1 + np.exp(-z)), 1 / (1 + np.exp(z))
+    n, c = x.shape
+    delta = rec_delta(z, dt)
+    dx, dz = np.full((n, c), np.nan, w), np.full((n, c), np.nan, w)
+    xt, zt = np.zeros((n, c), w), np.zeros((n, c), w)
+    d0, t0 = d_last.copy(), np.zeros_like(d_last)
+    for s, (a, e) in enumerate(zip(starts[:-1], starts[1:])):
+        carry, m, k = d_last[s], np.abs(d_last[s]), np.zeros(c, w)
+        for t in range(e - 1, a - 1, -1):
+            g = d_out[t] + carry
+            gm = m + np.abs(d_out[t])
+            gk = k + np.abs(d_out[t])
+            gt = delta * gk + 16 * U(dt) * gm
+            before = h[t - 1] if t > a else h0[s]
+            dx[t], xt[t] = om[t] * g, om[t] * (gt + (delta + U(dt)) * np.abs(g))
+            p = (before - x[t]) * f[t] * om[t]
+            dz[t], zt[t] = g * p, np.abs(p) * (gt + (2 * delta + 4 * U(dt)) * np.abs(g))
+            carry, m, k = f[t] * g, f[t] * gm, f[t] * (gk + gm)
+        if e > a:
+            d0[s], t0[s] = carry, delta * k + 16 * U(dt) * m
+    return dx, dz, d0, xt, zt, t0
+
+
+def lengths_to_starts(lengths, first=0):
+    return np.concatenate(([first], first + np.cumsum(lengths))).astype(np.int64)
+
+
+EVEN = [(1, 1, 1), (1, 5, 3), (7, 1, 64), (64, 1, 300), (3, 40, 128), (2, 257, 33), (1, 1000, 5), (5, 129, 260), (1, 4097, 96), (2, 2500, 64), (300, 2, 20),
+        (1, 20000, 3), (1, 700, 1025)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("seqs,length,channels", EVEN)
+def test_gated_recurrence_even(ctx, dt, seqs, length, channels):
+    check_recurrence(ctx, dt, [length] * seqs, channels, even=True)
+
+
+RAGGED = [[0], [3, 0, 0, 5], [0, 0, 70, 1, 0], [1] * 40, [1000, 1, 300, 0, 64, 65, 63], [5000], [17, 4000, 16, 15], [0, 2049], [33] * 70]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("channels", [1, 37, 64, 260])
+@pytest.mark.parametrize("lengths", RAGGED, ids=lambda v: f"{len(v)}seqs{sum(v)}")
+def test_gated_recurrence_ragged(ctx, dt, lengths, channels):
+    check_recurrence(ctx, dt, lengths, channels, even=False)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_gated_recurrence_rows_outside_all_sequences(ctx, dt):
+    for lengths in ([30, 0, 200], [0, 0], [1], [300, 300]):
+        for before, behind in ((0, 100), (5, 0), (70, 1)):
+            check_recurrence(ctx, dt, lengths, 70, even=False, before=before, behind=behind)
+
+
+def check_recurrence(ctx, dt, lengths, channels, even, before=0, behind=0):
+    seqs = len(lengths)
+    starts = lengths_to_starts(lengths, before)
+    n = int(starts[-1]) + behind
+    rng = np.random.default_rng(n + channels + seqs)
+    x, z = rng.standard_normal((n, channels)).astype(dt), (rng.standard_normal((n, channels)) * 2 + 2).astype(dt)
+    h0 = rng.standard_normal((seqs, channels)).astype(dt)
+    offsets = None if even else D(ctx, starts.reshape(-1, 1))
+    inside = np.zeros(n, bool)
+    inside[int(starts[0]):int(starts[-1])] = True
+    for h0_ in (h0, None):
+        zero = h0 if h0_ is not None else np.zeros_like(h0)
+        want, last, tol, ltol = rec_forward(x, z, zero, starts, dt)
+        res = D(ctx, np.full((n, channels), 7, dt)) if n else DenseMatrix(ctx, 0, channels, dt)
+        X = D(ctx, x) if n else DenseMatrix(ctx, 0, channels, dt)
+        Z = D(ctx, z) if n else DenseMatrix(ctx, 0, channels, dt)
+        H0 = None if h0_ is None else D(ctx, h0_)
+        _, gl = gatedRecurrenceForward(res, None, X, Z, H0, offsets, seqs, ctx)
+        got = res.to_numpy()
+        assert np.all(got[~inside] == 7)
+        near(got[inside], want[inside], tol[inside], "h")
+        near(gl.to_numpy(), last, ltol, "last")
+        h = want.astype(dt)
+        h[~inside] = np.nan  # rows that no sequence has are never read
+        d_out, d_last = rng.standard_normal((n, channels)).astype(dt), rng.standard_normal((seqs, channels)).astype(dt)
+        for dl in (d_last, None):
+            dx, dz, d0, xt, zt, t0 = rec_backward(x, z, h, zero, d_out, dl if dl is not None else np.zeros_like(d_last), starts, dt)
+            mk = lambda a: D(ctx, a) if a.shape[0] else DenseMatrix(ctx, 0, channels, dt)  # noqa: E731
+            gx, gz = mk(np.full((n, channels), 7, dt)), mk(np.full((n, channels), 7, dt))
+            _, _, g0 = gatedRecurrenceBackward(gx, gz, None, X, Z, mk(h), H0, mk(d_out), None if dl is None else D(ctx, dl), offsets, seqs, ctx)
+            a, b = gx.to_numpy(), gz.to_numpy()
+            assert np.all(a[~inside] == 7) and np.all(b[~inside] == 7)
+            near(a[inside], dx[inside], xt[inside], "dx")
+            near(b[inside], dz[inside], zt[inside], "dz")
+            near(g0.to_numpy(), d0, t0, "dh0")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_gated_recurrence_views_and_state_in_place(ctx, dt):
+    rng = np.random.default_rng(2)
+    for lengths, c in (([300, 20, 0, 80], 66), ([1] * 9, 68), ([1500], 20)):
+        starts, n, b = lengths_to_starts(lengths), sum(lengths), len(lengths)
+        x, z, h0 = rng.standard_normal((n, c)).astype(dt), rng.standard_normal((n, c)).astype(dt) + 1, rng.standard_normal((b, c)).astype(dt)
+        want, last, tol, ltol = rec_forward(x, z, h0, starts, dt)
+        xv, zv = view(ctx, x, 1, 2)[0], view(ctx, z, 4, 0)[0]
+        rv, rwhole = view(ctx, np.zeros_like(x), 2, 3)
+        sv, swhole = view(ctx, h0, 3, 2)
+        ov = view(ctx, starts.reshape(-1, 1), 1, 1, fill=-3)[0]
+        gatedRecurrenceForward(rv, sv, xv, zv, sv, ov, b, ctx)  # the state is updated in place
+        for w, l, v, t in ((rwhole.to_numpy(), 2, want, tol), (swhole.to_numpy(), 3, last, ltol)):
+            near(w[:, l:l + c], v, t)
+            assert np.all(w[:, :l] == 7) and np.all(w[:, l + c:] == 7)
+        d_out, d_last = rng.standard_normal((n, c)).astype(dt), rng.standard_normal((b, c)).astype(dt)
+        h = want.astype(dt)
+        dx, dz, d0, xt, zt, t0 = rec_backward(x, z, h, h0, d_out, d_last, starts, dt)
+        outs = [view(ctx, np.zeros_like(x), 1, 3), view(ctx, np.zeros_like(x), 0, 1), view(ctx, np.zeros_like(h0), 2, 2)]
+        gatedRecurrenceBackward(outs[0][0], outs[1][0], outs[2][0], xv, zv, view(ctx, h, 3, 1)[0], view(ctx, h0, 1, 0)[0], view(ctx, d_out, 0, 2)[0],
+                                view(ctx, d_last, 1, 1)[0], ov, b, ctx)
+        for (_, whole), l, v, t in zip(outs, (1, 0, 2), (dx, dz, d0), (xt, zt, t0)):
+            w = whole.to_numpy()
+            near(w[:, l:l + c], v, t)
+            assert np.all(w[:, :l] == 7) and np.all(w[:, l + c:] == 7)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_gated_recurrence_extreme_gates(ctx, dt):
+    """Gates that are shut or wide open to the last bit: a state that lives on unchanged, or is replaced at once."""
+    n, c = 700, 65
+    rng = np.random.default_rng(4)
+    x, h0 = rng.standard_normal((n, c)).astype(dt), rng.standard_normal((1, c)).astype(dt)
+    z = np.where(np.arange(c) % 3 == 0, np.inf, np.where(np.arange(c) % 3 == 1, -np.inf, 1e4)) * np.ones((n, 1))
+    got, last = gatedRecurrenceForward(None, None, D(ctx, x), D(ctx, z.astype(dt)), D(ctx, h0), None, 1, ctx)
+    want = np.where(np.arange(c) % 3 == 1, x, h0)
+    np.testing.assert_array_equal(got.to_numpy(), want)
+    np.testing.assert_array_equal(last.to_numpy(), want[-1:])
+    d = rng.standard_normal((n, c)).astype(dt)
+    dx, dz, d0 = gatedRecurrenceBackward(None, None, None, D(ctx, x), D(ctx, z.astype(dt)), got, D(ctx, h0), D(ctx, d), None, None, 1, ctx)
+    assert not dz.to_numpy().any()
+    np.testing.assert_array_equal(dx.to_numpy(), np.where(np.arange(c) % 3 == 1, d, 0))
+    # a NaN stays in its sequence and channel, from its row on
+    x[:, :] = 1
+    z = np.full((n, c), 0.5, dt)
+    z[300, 5] = np.nan
+    got = gatedRecurrenceForward(None, None, D(ctx, x), D(ctx, z), None, D(ctx, np.array([[0], [250], [500], [n]])), 3, ctx)[0].to_numpy()
+    bad = np.zeros((n, c), bool)
+    bad[300:500, 5] = True
+    np.testing.assert_array_equal(np.isnan(got), bad)
+
+
+@pytest.mark.parametrize("starts", [[0, 50, 40, 100], [-1, 50, 60, 100], [0, 50, 60, 101], [0, 2**62, 2**62, 100], [5, 3, 2, 1]])
+def test_gated_recurrence_bad_offsets(ctx, starts):
+    rng = np.random.default_rng(1)
+    x, z = rng.standard_normal((100, 70)).astype(F32), rng.standard_normal((100, 70)).astype(F32)
+    off = D(ctx, np.array(starts, np.int64).reshape(-1, 1))
+    with pytest.raises(IndexError, match="offset"):
+        gatedRecurrenceForward(None, None, D(ctx, x), D(ctx, z), None, off, 3, ctx)
+    with pytest.raises(IndexError, match="offset"):
+        gatedRecurrenceBackward(None, None, None, D(ctx, x), D(ctx, z), D(ctx, x), None, D(ctx, x), None, off, 3, ctx)
+    with pytest.raises(IndexError, match="offset"):
+        with ctx.deferred_checks():
+            gatedRecurrenceForward(None, None, D(ctx, x), D(ctx, z), None, off, 3, ctx)
+    good = D(ctx, np.array([[0], [50], [50], [100]]))
+    gatedRecurrenceForward(None, None, D(ctx, x), D(ctx, z), None, good, 3, ctx)
+
+
+def test_gated_recurrence_gradient_against_differences(ctx):
+    rng = np.random.default_rng(9)
+    starts = lengths_to_starts([30, 0, 25])
+    x, z, c = (rng.standard_normal((55, 6)) for _ in range(3))
+    h0, cl = rng.standard_normal((3, 6)), rng.standard_normal((3, 6))
+    off = D(ctx, starts.reshape(-1, 1))
+    def loss(x_, z_, h_):
+        r, l = gatedRecurrenceForward(None, None, D(ctx, x_), D(ctx, z_), D(ctx, h_), off, 3, ctx)
+        return float((r.to_numpy() * c).sum() + (l.to_numpy() * cl).sum())
+    h, _ = gatedRecurrenceForward(None, None, D(ctx, x), D(ctx, z), D(ctx, h0), off, 3, ctx)
+    grads = gatedRecurrenceBackward(None, None, None, D(ctx, x), D(ctx, z), h, D(ctx, h0), D(ctx, c), D(ctx, cl), off, 3, ctx)
+    step = 1e-5  # as for the norm
+    for k, (i, j) in ((0, (0, 0)), (0, (29, 5)), (0, (30, 2)), (1, (0, 1)), (1, (17, 3)), (1, (54, 0)), (2, (0, 4)), (2, (1, 1)), (2, (2, 2))):
+        a = [x, z, h0]
+        e = np.zeros_like(a[k])
+        e[i, j] = step
+        up, down = [m + e if q == k else m for q, m in enumerate(a)], [m - e if q == k else m for q, m in enumerate(a)]
+        assert abs((loss(*up) - loss(*down)) / (2 * step) - grads[k].to_numpy()[i, j]) < 1e-7
+
+
+def test_decoding_steps_equal_the_whole_sequence(ctx):
+    """One call over 40 tokens, and 40 calls of one token each that carry the state: the same recurrence."""
+    rng = np.random.default_rng(12)
+    b, n, c = 3, 40, 200
+    x, z = rng.standard_normal((b, n, c)).astype(F32), rng.standard_normal((b, n, c)).astype(F32)
+    h0 = rng.standard_normal((b, c)).astype(F32)
+    whole, last = gatedRecurrenceForward(None, None, D(ctx, x.reshape(-1, c)), D(ctx, z.reshape(-1, c)), D(ctx, h0), None, b, ctx)
+    _, _, tol, ltol = rec_forward(x.reshape(-1, c), z.reshape(-1, c), h0, lengths_to_starts([n] * b), F32)
+    state = D(ctx, h0)
+    for t in range(n):
+        step, _ = gatedRecurrenceForward(None, state, D(ctx, x[:, t]), D(ctx, z[:, t]), state, None, b, ctx)
+        near(step.to_numpy(), whole.to_numpy().reshape(b, n, c)[:, t], 2 * tol.reshape(b, n, c)[:, t])
+    near(state.to_numpy(), last.to_numpy(), 2 * ltol)
+
+
+# ------------------------------------------------------------------------------------------
+# 4-bit weights
+# ------------------------------------------------------------------------------------------
+def q4_dense(codes, scales, cols, group):
+    lo, hi = (codes & 15).astype(np.int64), (codes >> 4).astype(np.int64)
+    c = np.stack((lo, hi), -1).reshape(codes.shape[0], -1)[:, :cols]
+    return ((c ^ 8) - 8), np.repeat(scales.astype(F64), group, axis=1)[:, :cols]
+
+
+Q4 = [(1, 1, 1, 32), (1, 64, 5, 32), (1, 100, 33, 32), (2, 256, 17, 64), (1, 4096, 40, 128), (3, 1000, 70, 96), (4, 512, 64, 256), (5, 2048, 31, 64),
+      (8, 128, 300, 32), (9, 544, 20, 32), (16, 4096, 64, 64), (17, 640, 48, 128), (33, 320, 36, 32), (64, 1024, 130, 128), (1, 20000, 12, 128),
+      (16, 33, 16, 32), (1, 31, 3, 64), (2, 2049, 16, 128), (7, 96, 16, 1024), (1, 8, 4000, 32), (40, 4100, 257, 64)]
+
+
+@pytest.mark.parametrize("rows,cols,outs,group", Q4)
+def test_q4_products(ctx, rows, cols, outs, group):
+    rng = np.random.default_rng(rows + cols + outs)
+    codes = rng.integers(0, 256, (outs, -(-cols // 2)), dtype=np.uint8)
+    scales = ((rng.random((outs, -(-cols // group))) + 0.5) / 8).astype(F32)
+    c, s = q4_dense(codes, scales, cols, group)
+    x = rng.standard_normal((rows, cols)).astype(F32)
+    C_, S_ = D(ctx, codes), D(ctx, scales)
+    want, mag = x.astype(F64) @ (c * s).T, np.abs(x.astype(F64)) @ np.abs(c * s).T
+    # a product with a code, additions in chains of at most an eighth of the columns and 16 more, a product with a scale
+    near(matVecQ4(None, D(ctx, x), None, C_, S_, group, ctx).to_numpy(), want, (cols / 8 + 20) * U(F32) * mag, "floats")
+    q, qs = rng.integers(-127, 128, (rows, cols), dtype=np.int8), (rng.random((rows, 1)) / 50).astype(F32)
+    xq = q.astype(F64) * qs.astype(F64)
+    want, mag = xq @ (c * s).T, np.abs(xq) @ np.abs(c * s).T
+    # whole numbers are exact (a float holds the sums of 32 products); then as above
+    near(matVecQ4(None, D(ctx, q), D(ctx, qs), C_, S_, group, ctx).to_numpy(), want, (cols / 8 + 20) * U(F32) * mag, "8 bits")
+
+
+@pytest.mark.parametrize("rows,cols,outs,group", [(1, 256, 20, 64), (5, 384, 33, 128), (20, 130, 17, 32)])
+def test_q4_views(ctx, rows, cols, outs, group):
+    rng = np.random.default_rng(cols)
+    codes = rng.integers(0, 256, (outs, -(-cols // 2)), dtype=np.uint8)
+    scales = (rng.random((outs, -(-cols // group))) + 0.5).astype(F32)
+    c, s = q4_dense(codes, scales, cols, group)
+    x, q = rng.standard_normal((rows, cols)).astype(F32), rng.integers(-128, 128, (rows, cols), dtype=np.int8)
+    qs = rng.random((rows, 1)).astype(F32)
+    for left, right in ((0, 16), (3, 2), (16, 16), (1, 0)):
+        cv, sv = view(ctx, codes, left, right, fill=255)[0], view(ctx, scales, right, left, fill=np.nan)[0]
+        for xm, f in ((x, 1.0), (q, qs.astype(F64))):
+            xv = view(ctx, xm, left, right, fill=99)[0]
+            rv, whole = view(ctx, np.zeros((rows, outs), F32), right, left)
+            matVecQ4(rv, xv, None if xm is x else D(ctx, qs), cv, sv, group, ctx)
+            w, xw = whole.to_numpy(), xm.astype(F64) * f
+            near(w[:, right:right + outs], xw @ (c * s).T, (cols / 8 + 20) * U(F32) * (np.abs(xw) @ np.abs(c * s).T))
+            assert np.all(w[:, :right] == 7) and np.all(w[:, right + outs:] == 7)
+
+
+def test_q4_values_that_are_not_finite_stay_in_their_rows(ctx):
+    rng = np.random.default_rng(7)
+    codes, scales = rng.integers(0, 256, (40, 128), dtype=np.uint8), rng.random((40, 4)).astype(F32)
+    codes[:] |= 0x11  # no code is 0
+    for rows in (1, 5, 20):
+        x = rng.standard_normal((rows, 256)).astype(F32)
+        x[0, 17] = np.inf
+        scales[3, 1] = np.nan
+        got = matVecQ4(None, D(ctx, x), None, D(ctx, codes), D(ctx, scales), 64, ctx).to_numpy()
+        assert not np.isfinite(got[0]).any() and np.isnan(got[:, 3]).all()
+        assert np.isfinite(np.delete(got[1:], 3, axis=1)).all()
+
+
+@pytest.mark.parametrize("rows,cols,group", [(1, 1, 32), (5, 64, 32), (7, 1000, 128), (33, 257, 64), (3, 96, 96), (2, 5000, 1024), (4, 31, 32)])
+def test_quantize_q4(ctx, rows, cols, group):
+    rng = np.random.default_rng(rows + cols)
+    w = rng.standard_normal((rows, cols)).astype(F32)
+    w[0, :] = np.round(w[0] * 3) / 2  # halves: values on a border between two codes
+    w[0, 0] = 3.5
+    if rows > 1:
+        w[1, :min(cols, group)] = 0
+    codes, scales = quantizeQ4(None, None, D(ctx, w), group, ctx)
+    groups = -(-cols // group)
+    pad = np.zeros((rows, groups * group), F64)
+    pad[:, :cols] = w
+    most = np.abs(pad.reshape(rows, groups, group)).max(axis=2)
+    np.testing.assert_array_equal(scales.to_numpy(), most.astype(F32) / F32(7))
+    want = np.rint(pad * np.repeat(np.divide(7.0, most, out=np.zeros_like(most), where=most > 0), group, axis=1))[:, :cols]
+    c, _ = q4_dense(codes.to_numpy(), scales.to_numpy(), cols, group)
+    np.testing.assert_array_equal(c, want)
+    if cols % 2:
+        assert not (codes.to_numpy()[:, -1] >> 4).any()
+    w[rows - 1, cols - 1] = np.nan
+    codes, scales = quantizeQ4(None, None, D(ctx, w), group, ctx)
+    s = scales.to_numpy()
+    assert np.isnan(s[-1, -1]) and np.isfinite(np.delete(s.reshape(-1), -1)).all()
+
+
+# ------------------------------------------------------------------------------------------
+# as they are used together
+# ------------------------------------------------------------------------------------------
+def test_training_step_of_a_small_model(ctx):
+    """Embedding, norm on the stream, gate and value products, recurrence, and all of their gradients down to the table,
+    against the same model in numpy whose gradients are taken by differences."""
+    rng = np.random.default_rng(20)
+    lengths, vocab, w = [9, 0, 14], 11, 16
+    starts, n = lengths_to_starts(lengths), sum(lengths)
+    ids = token_ids(rng, n, vocab)
+    par = {"E": rng.standard_normal((vocab, w)), "g": 1 + 0.1 * rng.standard_normal((1, w)), "Wx": rng.standard_normal((w, w)) / 4,
+           "Wz": rng.standard_normal((w, w)) / 4, "h0": rng.standard_normal((3, w))}
+    target = rng.standard_normal((n, w))
+
+    def loss(p):
+        e = p["E"][ids[:, 0]] * 4.0
+        inv = 1 / np.sqrt((e * e).mean(axis=1, keepdims=True) + 1e-5)
+        y = e * inv * p["g"]
+        h, _, _, _ = rec_forward(y @ p["Wx"], y @ p["Wz"], p["h0"], starts, F32)
+        return float(((h + e) * target).sum())
+
+    m = {k: D(ctx, v) for k, v in par.items()}
+    I, off, T = D(ctx, ids), D(ctx, starts.reshape(-1, 1)), D(ctx, target)
+    e = embeddingForward(None, m["E"], I, 4.0, ctx)
+    y, stream, inv = rmsNormForward(None, None, None, e, None, m["g"], 1e-5, ctx)
+    x, z = matMul(None, y, m["Wx"], False, False, ctx), matMul(None, y, m["Wz"], False, False, ctx)
+    h, _ = gatedRecurrenceForward(None, None, x, z, m["h0"], off, 3, ctx)
+    assert abs(float(((h.to_numpy() + e.to_numpy()) * target).sum()) - loss(par)) < 1e-10
+    dx, dz, dh0 = gatedRecurrenceBackward(None, None, None, x, z, h, m["h0"], T, None, off, 3, ctx)
+    dy = D(ctx, matMul(None, dx, m["Wx"], False, True, ctx).to_numpy() + matMul(None, dz, m["Wz"], False, True, ctx).to_numpy())
+    de, dg = rmsNormBackward(None, None, stream, inv, m["g"], dy, T, ctx)
+    got = {"E": embeddingBackward(None, de, I, vocab, 4.0, ctx), "g": dg, "h0": dh0, "Wx": matMul(None, y, dx, True, False, ctx),
+           "Wz": matMul(None, y, dz, True, False, ctx)}
+    step = 1e-5
+    for k, v in par.items():
+        for _ in range(6):
+            at = tuple(rng.integers(0, s) for s in v.shape)
+            up, down = dict(par), dict(par)
+            up[k], down[k] = v.copy(), v.copy()
+            up[k][at] += step
+            down[k][at] -= step
+            assert abs((loss(up) - loss(down)) / (2 * step) - got[k].to_numpy()[at]) < 1e-6, (k, at)
+
+
+def decode_step(ctx, ids, table, gamma, weights, state, stream, out, ws=None):
+    """One token per sequence: embedding, residual norm to 8 bits, two 4-bit products, one step of the recurrence."""
+    embeddingForward(out["e"], table, ids, 1.0, ctx)
+    rmsNormForwardQ8(out["q"], out["qs"], stream, out["inv"], out["e"], stream, gamma, 1e-5, ctx)
+    for k in ("x", "z"):
+        matVecQ4(out[k], out["q"], out["qs"], *weights[k], 64, ctx)
+    gatedRecurrenceForward(out["h"], state, out["x"], out["z"], state, None, state.rows, ctx, workspace=ws)
+    return out["h"]
+
+
+def decode_setup(ctx, b=5, w=256, vocab=50):
+    rng = np.random.default_rng(33)
+    mk = lambda *s: rng.standard_normal(s).astype(F32)  # noqa: E731
+    host = {"table": mk(vocab, w), "gamma": mk(1, w), "state": mk(b, w), "stream": mk(b, w)}
+    dev = {k: D(ctx, v) for k, v in host.items()}
+    weights = {k: quantizeQ4(None, None, D(ctx, mk(w, w) / 16), 64, ctx) for k in ("x", "z")}
+    out = {k: DenseMatrix(ctx, b, w, F32) for k in ("e", "x", "z", "h")} | {"q": DenseMatrix(ctx, b, w, np.int8), "qs": DenseMatrix(ctx, b, 1, F32),
+                                                                             "inv": DenseMatrix(ctx, b, 1, F32)}
+    return rng, host, dev, weights, out
+
+
+def test_decoding_a_few_tokens(ctx):
+    rng, host, dev, weights, out = decode_setup(ctx)
+    b, w = host["state"].shape
+    dense = {k: np.multiply(*q4_dense(v[0].to_numpy(), v[1].to_numpy(), w, 64)) for k, v in weights.items()}
+    stream, state = host["stream"], host["state"].astype(F64)
+    for _ in range(6):
+        ids = token_ids(rng, b, 50)
+        got = decode_step(ctx, D(ctx, ids), dev["table"], dev["gamma"], weights, dev["state"], dev["stream"], out).to_numpy()
+        stream = host["table"][ids[:, 0]] + stream
+        u = stream.astype(F64) * host["gamma"]
+        most = np.abs(u).max(axis=1, keepdims=True)
+        inv = 1 / np.sqrt((stream.astype(F64) ** 2).mean(axis=1, keepdims=True) + 1e-5)
+        a = np.rint(u * (127 / most)) * (most * inv / 127)
+        x, z = a @ dense["x"].T, a @ dense["z"].T
+        state = state / (1 + np.exp(-z)) + x / (1 + np.exp(z))
+        np.testing.assert_array_equal(dev["stream"].to_numpy(), stream)
+        # x and z are off by 52 half steps of their terms' magnitudes (q4's tolerance), which are below 64; the state adds the
+        # gates' 16 and keeps what it had
+        near(got, state, (6 * 52 * 64 + 100) * U(F32))
+
+
+def test_decoding_in_a_captured_graph(ctx):
+    """The whole step captured once, replayed with other tokens between eager work; every replay equals an eager step."""
+    torch = pytest.importorskip("torch")
+    c = HIPContext(0)
+    try:
+        rng, host, dev, weights, out = decode_setup(c)
+        b, w = host["state"].shape
+        stream = torch.cuda.Stream()
+        c.set_stream(stream.cuda_stream)
+        ids = D(c, token_ids(rng, b, 50))
+        eager = {k: D(c, v) for k, v in host.items()}
+        eout = {k: DenseMatrix(c, m.rows, m.cols, m.dtype) for k, m in out.items()}
+        g = torch.cuda.CUDAGraph()
+        c.sync()
+        with pytest.raises(capi.DaphneHipError, match="defer"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream, capture_error_mode="thread_local"):
+                embeddingForward(out["e"], dev["table"], ids, 1.0, c)
+        with c.deferred_checks():
+            with torch.cuda.graph(g, stream=stream, capture_error_mode="thread_local"):
+                decode_step(c, ids, dev["table"], dev["gamma"], weights, dev["state"], dev["stream"], out)
+        for k in range(4):
+            new = token_ids(rng, b, 50)
+            capi.check(capi.lib().dh_h2d(c._h, ids.ptr, new.ctypes.data, new.nbytes))
+            with torch.cuda.stream(stream):
+                g.replay()
+            c.sync()
+            want = decode_step(c, D(c, new), eager["table"], eager["gamma"], weights, eager["state"], eager["stream"], eout).to_numpy()
+            np.testing.assert_array_equal(out["h"].to_numpy(), want)
+            np.testing.assert_array_equal(dev["state"].to_numpy(), eager["state"].to_numpy())
+        c.check_deferred()
+        new[2] = 50  # a token that does not exist: the replay's verdict waits for the next check
+        capi.check(capi.lib().dh_h2d(c._h, ids.ptr, new.ctypes.data, new.nbytes))
+        with torch.cuda.stream(stream):
+            g.replay()
+        with pytest.raises(IndexError, match="'50'"):
+            c.check_deferred()
+        c.check_deferred()
+        del g
+    finally:
+        c.sync()
+        c.destroy()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_gradients_in_two_captured_graphs(ctx, dt):
+    """Two graphs of the gradient calls, each with a workspace of its own, replayed in turn with eager calls between."""
+    torch = pytest.importorskip("torch")
+    c = HIPContext(0)
+    tdt = torch.float32 if dt == F32 else torch.float64
+    try:
+        stream = torch.cuda.Stream()
+        rng = np.random.default_rng(44)
+        n, w, vocab = 6000, 40, 70
+        starts = D(c, lengths_to_starts([2500, 0, 3400]).reshape(-1, 1))
+        sets = []
+        c.set_stream(stream.cuda_stream)
+        need = max(embeddingBackwardWorkspaceBytes(n, vocab, w, dt), rmsNormBackwardWorkspaceBytes(n, w, dt), gatedRecurrenceWorkspaceBytes(n, 3, w, dt))
+
+        def run(s, ws):
+            a, o = s["in"], s["out"]
+            gatedRecurrenceForward(o["h"], o["last"], a["x"], a["z"], None, starts, 3, c, workspace=ws)
+            gatedRecurrenceBackward(o["dx"], o["dz"], o["dh0"], a["x"], a["z"], o["h"], None, a["d"], None, starts, 3, c, workspace=ws)
+            rmsNormBackward(o["dn"], o["dg"], a["x"], a["inv"], None, o["dx"], o["dz"], c, workspace=ws)
+            embeddingBackward(o["dE"], o["dn"], a["ids"], vocab, 1.5, c, workspace=ws)
+
+        def outputs():
+            return {k: DenseMatrix(c, *s, dt) for k, s in {"h": (n, w), "last": (3, w), "dx": (n, w), "dz": (n, w), "dh0": (3, w), "dn": (n, w),
+                                                           "dg": (1, w), "dE": (vocab, w)}.items()}
+
+        for _ in range(2):
+            a = {k: D(c, rng.standard_normal((n, w)).astype(dt)) for k in ("x", "z", "d")}
+            a["inv"], a["ids"] = D(c, rng.random((n, 1)).astype(dt)), D(c, token_ids(rng, n, vocab))
+            sets.append({"in": a, "out": outputs(), "ws": DenseMatrix(c, 1, need + 8, np.uint8), "graph": torch.cuda.CUDAGraph()})
+        zeros = {k: np.zeros((m.rows, m.cols), dt) for k, m in sets[0]["out"].items()}
+        c.sync()
+        with c.deferred_checks():
+            if need:
+                with pytest.raises(capi.DaphneHipError, match="workspace"):
+                    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream, capture_error_mode="thread_local"):
+                        run(sets[0], None)
+                with pytest.raises(ValueError, match="workspace"):
+                    run(sets[0], DenseMatrix(c, 1, 1, np.uint8))
+            for s in sets:
+                with torch.cuda.graph(s["graph"], stream=stream, capture_error_mode="thread_local"):
+                    run(s, s["ws"])
+        for k in range(3):
+            for s in sets:
+                for key, z in zeros.items():
+                    capi.check(capi.lib().dh_h2d(c._h, s["out"][key].ptr, z.ctypes.data, z.nbytes))
+            for s in sets:
+                with torch.cuda.stream(stream):
+                    s["graph"].replay()
+            for s in sets:
+                plain = {"in": s["in"], "out": outputs()}
+                run(plain, None)
+                for key, m in plain["out"].items():
+                    np.testing.assert_array_equal(s["out"][key].to_numpy(), m.to_numpy(), err_msg=key)
+        c.check_deferred()
+        for s in sets:
+            del s["graph"]
+        assert tdt.itemsize == np.dtype(dt).itemsize
+    finally:
+        c.sync()
+        c.destroy()
+
+
+def test_two_contexts_on_streams_of_their_own(ctx):
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(50)
+    cs = [HIPContext(0), HIPContext(0)]
+    try:
+        n, w, vocab = 20000, 64, 700
+        ids, d = token_ids(rng, n, vocab), rng.standard_normal((n, w)).astype(F32)
+        want = embeddingBackward(None, D(ctx, d), D(ctx, ids), vocab, 1.0, ctx).to_numpy()
+        rec = gatedRecurrenceForward(None, None, D(ctx, d), D(ctx, d), None, None, 4, ctx)[0].to_numpy()
+        for c in cs:
+            c.stream = torch.cuda.Stream()
+            c.set_stream(c.stream.cuda_stream)
+            capi.check(capi.lib().dh_defer_checks(c._h, 1))
+        args = [(D(c, d), D(c, ids)) for c in cs]
+        outs = []
+        for _ in range(3):  # queued on both streams before either is waited for
+            for c, (dm, im) in zip(cs, args):
+                outs.append((embeddingBackward(None, dm, im, vocab, 1.0, c), gatedRecurrenceForward(None, None, dm, dm, None, None, 4, c)[0]))
+        for a, b in outs:
+            np.testing.assert_array_equal(a.to_numpy(), want)
+            np.testing.assert_array_equal(b.to_numpy(), rec)
+        outs.clear()
+        args.clear()
+    finally:
+        for c in cs:
+            c.sync()
+            c.destroy()
+

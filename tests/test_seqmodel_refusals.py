@@ -1,0 +1,125 @@
+"""CPU: what the sequence-model entry points refuse, before they need a device. The C functions check their arguments
+first and their context then, so that a null context shows how far a call gets."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from daphne_amd import capi
+from daphne_amd.kernels import (DenseMatrix, embeddingBackward, embeddingForward, gatedRecurrenceBackward, gatedRecurrenceForward, matVecQ4,
+                                quantizeQ4, rmsNormBackward, rmsNormForward, rmsNormForwardQ8)
+
+P = 0x1000  # a pointer no call gets to use
+
+
+class NoContext:
+    _h = None
+
+
+CTX = NoContext()
+
+
+def M(rows, cols, dt=np.float32, skip=None, at=iter(range(2 * P, 1000 * P, P))):
+    return DenseMatrix(CTX, rows, cols, dt, ptr=next(at), row_skip=skip)
+
+
+def refused(call, *args, kind=RuntimeError, match=None):
+    with pytest.raises(kind, match=match) as e:
+        call(*args)
+    assert "context is null" not in str(e.value)
+
+
+def gets_through(call, *args):
+    with pytest.raises(capi.DaphneHipError, match="context is null"):
+        call(*args)
+
+
+I64 = np.int64
+
+
+def test_embedding_refusals():
+    gets_through(embeddingForward, M(3, 8), M(10, 8), M(3, 1, I64), 1.0, CTX)
+    gets_through(embeddingBackward, M(10, 8), M(3, 8), M(3, 1, I64), 10, 1.0, CTX)
+    refused(embeddingForward, M(3, 8), M(10, 8), M(3, 1, np.int32), 1.0, CTX, kind=TypeError)
+    refused(embeddingForward, M(3, 8), M(10, 8), M(3, 2, I64), 1.0, CTX, match="column")
+    refused(embeddingForward, M(3, 7), M(10, 8), M(3, 1, I64), 1.0, CTX, match="3 x 8 is needed")
+    refused(embeddingForward, M(3, 8, np.float64), M(10, 8), M(3, 1, I64), 1.0, CTX, match="mixed value types")
+    refused(embeddingForward, M(3, 8, I64), M(10, 8, I64), M(3, 1, I64), 1.0, CTX, match="not instantiated")
+    refused(embeddingForward, M(3, 8, skip=7), M(10, 8), M(3, 1, I64), 1.0, CTX, match="leading dimension")
+    refused(embeddingBackward, M(10, 8), M(3, 8), M(4, 1, I64), 10, 1.0, CTX, match="column of 3")
+    refused(embeddingBackward, M(9, 8), M(3, 8), M(3, 1, I64), 10, 1.0, CTX, match="10 x 8 is needed")
+    refused(embeddingBackward, None, M(3, 8), M(3, 1, I64), 10, 1.0, CTX, True, kind=ValueError, match="accumulate")
+    lib = capi.lib()
+    assert lib.dh_embedding_forward_f32(None, None, 8, P, 10, 8, 8, P, 3, 1, 1.0) == capi.DH_ERR_RUNTIME
+    assert b"null" in lib.dh_last_error()
+    assert lib.dh_embedding_backward_f64(None, P, 10, 8, 8, None, 8, P, 3, 1, 1.0, 0, None, 0) == capi.DH_ERR_RUNTIME
+    assert b"a matrix is null" in lib.dh_last_error()
+
+
+def test_rms_norm_refusals():
+    x, g, inv = M(3, 8), M(1, 8), M(3, 1)
+    gets_through(rmsNormForward, M(3, 8), M(3, 8), inv, x, M(3, 8), g, 1e-5, CTX)
+    gets_through(rmsNormForward, M(3, 8), None, inv, x, None, None, 0.0, CTX)
+    same = M(3, 8)
+    refused(rmsNormForward, same, same, inv, x, M(3, 8), g, 1e-5, CTX, kind=ValueError, match="same matrix")
+    refused(rmsNormForward, M(3, 8), M(3, 8), inv, x, M(3, 8), g, -1e-5, CTX, kind=ValueError, match="eps")
+    refused(rmsNormForward, M(3, 8), M(3, 8), inv, x, M(3, 8), g, float("nan"), CTX, kind=ValueError)
+    refused(rmsNormForward, M(3, 8), M(3, 8), inv, x, M(2, 8), g, 1e-5, CTX, match="residual is 2 x 8")
+    refused(rmsNormForward, M(3, 8), M(3, 8), inv, x, M(3, 8), M(1, 7), 1e-5, CTX, match="gamma")
+    refused(rmsNormForward, M(3, 8), M(3, 8), M(3, 1, skip=2), x, M(3, 8), g, 1e-5, CTX, match="invRms")
+    refused(rmsNormForwardQ8, M(3, 8), M(3, 1), M(3, 8), inv, x, M(3, 8), g, 1e-5, CTX, kind=TypeError)
+    d = lambda r, c: M(r, c, np.float64)  # noqa: E731
+    refused(rmsNormForwardQ8, M(3, 8, np.int8), d(3, 1), d(3, 8), d(3, 1), d(3, 8), d(3, 8), d(1, 8), 1e-5, CTX, match="not instantiated")
+    gets_through(rmsNormBackward, M(3, 8), M(1, 8), x, inv, g, M(3, 8), None, CTX)
+    refused(rmsNormBackward, M(3, 8), M(1, 8), x, inv, g, M(3, 7), None, CTX, match="dRes is 3 x 7")
+    refused(rmsNormBackward, M(3, 8), M(1, 8), x, M(2, 1), g, M(3, 8), None, CTX, match="invRms")
+    refused(rmsNormBackward, M(3, 8, skip=4), M(1, 8), x, inv, g, M(3, 8), None, CTX, match="leading dimension")
+
+
+def test_gated_recurrence_refusals():
+    x, h0 = M(6, 5), M(3, 5)
+    gets_through(gatedRecurrenceForward, M(6, 5), h0, x, M(6, 5), h0, None, 3, CTX)
+    gets_through(gatedRecurrenceForward, M(6, 5), M(4, 5), x, M(6, 5), None, M(5, 1, I64), 4, CTX)
+    refused(gatedRecurrenceForward, M(6, 5), M(4, 5), x, M(6, 5), None, None, 4, CTX, match="do not divide")
+    refused(gatedRecurrenceForward, M(6, 5), M(0, 5), x, M(6, 5), None, None, 0, CTX, match="do not divide")
+    refused(gatedRecurrenceForward, M(6, 5), M(4, 5), x, M(6, 5), None, M(4, 1, I64), 4, CTX, match="column of 5")
+    refused(gatedRecurrenceForward, M(6, 5), M(4, 5), x, M(6, 5), None, M(5, 1, np.uint64), 4, CTX, kind=TypeError)
+    refused(gatedRecurrenceForward, M(6, 5), h0, x, M(6, 4), h0, None, 3, CTX, match="z is 6 x 4")
+    refused(gatedRecurrenceForward, M(6, 5), h0, x, M(6, 5), M(2, 5), None, 3, CTX, match="h0 is 2 x 5")
+    refused(gatedRecurrenceForward, M(6, 5), h0, x, M(6, 5, skip=3), h0, None, 3, CTX, match="leading dimension")
+    a = [M(6, 5), M(6, 5), h0, x, M(6, 5), M(6, 5), h0, M(6, 5), h0, None, 3, CTX]
+    gets_through(gatedRecurrenceBackward, *a)
+    refused(gatedRecurrenceBackward, *(a[:5] + [M(5, 5)] + a[6:]), match="h is 5 x 5")
+    refused(gatedRecurrenceBackward, *(a[:8] + [M(3, 5, np.float64)] + a[9:]), match="mixed value types")
+    refused(gatedRecurrenceBackward, *(a[:10] + [4, CTX]), match="h0 is 3 x 5")
+
+
+def test_q4_refusals():
+    U8 = np.uint8
+    x, c, s = M(2, 100), M(7, 50, U8), M(7, 4)
+    gets_through(matVecQ4, M(2, 7), x, None, c, s, 32, CTX)
+    gets_through(matVecQ4, M(2, 7), M(2, 100, np.int8), M(2, 1), c, s, 32, CTX)
+    refused(matVecQ4, M(2, 7), x, None, c, M(7, 3), 32, CTX, match="scales is 7 x 3")
+    refused(matVecQ4, M(2, 7), x, None, c, M(7, 5), 20, CTX, kind=ValueError, match="multiple of 32")
+    refused(matVecQ4, M(2, 7), x, None, c, s, 0, CTX, kind=ValueError)
+    refused(matVecQ4, M(2, 7), x, None, M(7, 51, U8), s, 32, CTX, match="codes is 7 x 51")
+    refused(matVecQ4, M(2, 7), x, None, M(7, 50, np.int8), s, 32, CTX, kind=TypeError)
+    refused(matVecQ4, M(2, 7), M(2, 100, np.int8), None, c, s, 32, CTX, kind=TypeError)
+    refused(matVecQ4, M(2, 7), x, M(2, 1), c, s, 32, CTX, kind=TypeError)
+    refused(matVecQ4, M(2, 7), M(2, 100, np.float64), None, c, s, 32, CTX, match="mixed value types")
+    refused(matVecQ4, M(2, 8), x, None, c, s, 32, CTX, match="2 x 7 is needed")
+    refused(matVecQ4, M(2, 7), x, None, M(7, 50, U8, skip=49), s, 32, CTX, match="leading dimension")
+    gets_through(quantizeQ4, c, s, M(7, 100), 32, CTX)
+    refused(quantizeQ4, c, s, M(7, 100), -32, CTX, kind=ValueError)
+    refused(quantizeQ4, c, s, M(7, 99), 31, CTX, kind=ValueError, match="multiple of 32")
+    refused(quantizeQ4, c, s, M(7, 100, np.float64), 32, CTX, match="not instantiated")
+
+
+def test_workspace_sizes_are_whole_numbers_of_bytes():
+    lib = capi.lib()
+    for suf in ("f32", "f64"):
+        for n in (0, 1, 4096, 4097, 300000):
+            assert getattr(lib, f"dh_embedding_backward_workspace_{suf}")(n, 1000, 64) >= 0
+            assert getattr(lib, f"dh_rmsnorm_backward_workspace_{suf}")(n, 640) >= 0
+            assert getattr(lib, f"dh_gated_recurrence_workspace_{suf}")(n, 3, 640) >= 0
+    assert C.sizeof(C.c_size_t) == 8
