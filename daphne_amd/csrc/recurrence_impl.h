@@ -1,24 +1,42 @@
 // Gated linear recurrence over packed sequences for DenseMatrix<float|double>, forward and backward.
 //
 //   f_t = sigmoid(z_t)      h_t = f_t h_{t-1} + (1 - f_t) x_t                 for every channel of every sequence,
-//   G_t = d_out_t + f_{t+1} G_{t+1}  (the last row adds d_last),
-//   d_x_t = (1 - f_t) G_t   d_z_t = G_t (h_{t-1} - x_t) f_t (1 - f_t)         d_h0 = f_0 G_0.
+//   G_t = d_out_t + c_t     c_{t-1} = f_t G_t                                 (c = d_last behind the last row),
+//   d_x_t = (1 - f_t) G_t   d_z_t = G_t (h_{t-1} - x_t) f_t (1 - f_t)         d_h0 = f_0 G_0 = c in front of the first row.
 //
 // Rows are tokens: the sequences lie one behind the other, sequence s in rows [offsets[s], offsets[s + 1]).
+//
+// Both directions carry one value per channel through maps v -> A v + B of one row each, and such maps compose:
+// (A2, B2) after (A1, B1) is (A2 A1, A2 B1 + B2). That lets the token axis be cut anywhere. All rows of the batch are cut
+// into chunks, whatever the sequences' lengths; a row that begins a sequence (backward: ends one) takes the value it is
+// given instead of the carried one, so a carry never crosses from one sequence into another, not even a NaN.
+//
+// scan_kernel does it in one pass over the data (a chunk's inputs stay in registers from its composition to its
+// result), which makes it bound by memory: a workgroup composes its chunk, publishes the composition, looks back over its
+// predecessors' until it meets a carry that is already whole, publishes its own, and writes its rows.
 #pragma once
 
 #include "common.h"
+
+#include <type_traits>
 
 namespace dh_rec {
 
 constexpr int THREADS = 256;
 
 // f = 1 / (1 + exp(-z)) and 1 - f, each to full relative precision: both from e = exp(-|z|), which never overflows.
-template <typename T> __device__ __forceinline__ void gates(T z, T &f, T &w) {
-    const T e = sizeof(T) == 4 ? static_cast<T>(__expf(-fabsf(static_cast<float>(z)))) : static_cast<T>(exp(-fabs(static_cast<double>(z))));
-    const T r = T(1) / (T(1) + e), er = e * r;
-    f = z >= T(0) ? r : er;
-    w = z >= T(0) ? er : r;
+__device__ __forceinline__ void gates(float z, float &f, float &w) {
+    const float e = __expf(-fabsf(z)), d = 1.0f + e;
+    float r = __builtin_amdgcn_rcpf(d); // d in [1, 2]: one Newton step takes the approximation to the division's half step
+    r = fmaf(fmaf(-d, r, 1.0f), r, r);
+    const float er = e * r;
+    f = z >= 0.0f ? r : er;
+    w = z >= 0.0f ? er : r;
+}
+__device__ __forceinline__ void gates(double z, double &f, double &w) {
+    const double e = exp(-fabs(z)), r = 1.0 / (1.0 + e), er = e * r;
+    f = z >= 0.0 ? r : er;
+    w = z >= 0.0 ? er : r;
 }
 
 // Rows of sequence s, clamped to the tokens that exist; equal lengths without offsets.
@@ -50,21 +68,23 @@ template <typename T>
 __global__ __launch_bounds__(THREADS) void forward_serial_kernel(T *res, size_t ld_res, T *last, size_t ld_last, const T *x, size_t ld_x,
                                                                  const T *z, size_t ld_z, const T *h0, size_t ld_h0, Spans sp,
                                                                  size_t num_seq, size_t channels, int *rec) {
-    const size_t c = static_cast<size_t>(blockIdx.x) * THREADS + threadIdx.x, s = blockIdx.y;
-    if (s == 0)
+    const size_t c = static_cast<size_t>(blockIdx.x) * THREADS + threadIdx.x;
+    if (blockIdx.y == 0)
         check_offsets(sp, num_seq, c, static_cast<size_t>(gridDim.x) * THREADS, rec);
     if (c >= channels)
         return;
-    T h = h0 ? h0[s * ld_h0 + c] : T(0);
-    const size_t end = sp.at(s + 1);
-    for (size_t t = sp.at(s); t < end; t++) {
-        T f, w;
-        gates(z[t * ld_z + c], f, w);
-        h = f * h + w * x[t * ld_x + c];
-        res[t * ld_res + c] = h;
+    for (size_t s = blockIdx.y; s < num_seq; s += gridDim.y) {
+        T h = h0 ? h0[s * ld_h0 + c] : T(0);
+        const size_t end = sp.at(s + 1);
+        for (size_t t = sp.at(s); t < end; t++) {
+            T f, w;
+            gates(z[t * ld_z + c], f, w);
+            h = f * h + w * x[t * ld_x + c];
+            res[t * ld_res + c] = h;
+        }
+        if (last)
+            last[s * ld_last + c] = h;
     }
-    if (last)
-        last[s * ld_last + c] = h;
 }
 
 template <typename T>
@@ -72,27 +92,450 @@ __global__ __launch_bounds__(THREADS) void backward_serial_kernel(T *d_x, size_t
                                                                   const T *x, size_t ld_x, const T *z, size_t ld_z, const T *h, size_t ld_h,
                                                                   const T *h0, size_t ld_h0, const T *d_out, size_t ld_do, const T *d_last,
                                                                   size_t ld_dl, Spans sp, size_t num_seq, size_t channels, int *rec) {
-    const size_t c = static_cast<size_t>(blockIdx.x) * THREADS + threadIdx.x, s = blockIdx.y;
-    if (s == 0)
+    const size_t c = static_cast<size_t>(blockIdx.x) * THREADS + threadIdx.x;
+    if (blockIdx.y == 0)
         check_offsets(sp, num_seq, c, static_cast<size_t>(gridDim.x) * THREADS, rec);
     if (c >= channels)
         return;
-    T carry = d_last ? d_last[s * ld_dl + c] : T(0); // f_{t+1} G_{t+1}
-    const size_t begin = sp.at(s);
-    for (size_t t = sp.at(s + 1); t > begin;) {
-        t--;
-        T f, w;
-        gates(z[t * ld_z + c], f, w);
-        const T g = d_out[t * ld_do + c] + carry;
-        const T before = t > begin ? h[(t - 1) * ld_h + c] : h0 ? h0[s * ld_h0 + c] : T(0);
-        const T xv = x[t * ld_x + c];
-        d_x[t * ld_dx + c] = w * g;
-        d_z[t * ld_dz + c] = g * (before - xv) * f * w;
-        carry = f * g;
+    for (size_t s = blockIdx.y; s < num_seq; s += gridDim.y) {
+        T carry = d_last ? d_last[s * ld_dl + c] : T(0); // f_{t+1} G_{t+1}
+        const size_t begin = sp.at(s);
+        for (size_t t = sp.at(s + 1); t > begin;) {
+            t--;
+            T f, w;
+            gates(z[t * ld_z + c], f, w);
+            const T g = d_out[t * ld_do + c] + carry;
+            const T before = t > begin ? h[(t - 1) * ld_h + c] : h0 ? h0[s * ld_h0 + c] : T(0);
+            const T xv = x[t * ld_x + c];
+            d_x[t * ld_dx + c] = w * g;
+            d_z[t * ld_dz + c] = g * (before - xv) * f * w;
+            carry = f * g;
+        }
+        if (d_h0)
+            d_h0[s * ld_dh0 + c] = carry;
     }
-    if (d_h0)
-        d_h0[s * ld_dh0 + c] = carry;
 }
+
+// ---------------------------------------------------------------------------------------
+// one pass over chunks of rows
+// ---------------------------------------------------------------------------------------
+// A published value: each 32 bits of it in a word of their own beside the mark that they are there, so that a reader needs
+// no fence between a flag and the value. Zero: not there yet.
+template <typename T> struct Words {
+    static constexpr int N = sizeof(T) / 4;
+};
+template <typename T> __device__ __forceinline__ void publish(unsigned long long *p, size_t stride, T v) {
+    if constexpr (sizeof(T) == 4) {
+        __hip_atomic_store(p, (static_cast<unsigned long long>(__builtin_bit_cast(unsigned, v)) << 32) | 1ull, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+        const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+        __hip_atomic_store(p, (b << 32) | 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(p + stride, (b & 0xffffffff00000000ull) | 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+template <typename T> __device__ __forceinline__ bool published(const unsigned long long *p, size_t stride, T &v) {
+    const unsigned long long a = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if constexpr (sizeof(T) == 4) {
+        v = __builtin_bit_cast(T, static_cast<unsigned>(a >> 32));
+        return a != 0;
+    } else {
+        const unsigned long long b = __hip_atomic_load(p + stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        v = __builtin_bit_cast(T, (a >> 32) | (b & 0xffffffff00000000ull));
+        return a != 0 && b != 0;
+    }
+}
+
+// The workspace: a ticket counter (256 bytes), then for every chunk the three published values A, B and the whole carry,
+// each a row of `padded` channels (times the words of a value). Cleared by clear_kernel before each pass.
+static __global__ __launch_bounds__(THREADS) void clear_kernel(ulonglong2 *p, size_t n) {
+    for (size_t i = static_cast<size_t>(blockIdx.x) * THREADS + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * THREADS)
+        p[i] = ulonglong2{0, 0};
+}
+
+template <typename T> struct ScanArgs {
+    const T *x, *z, *h0; // h0 backward: as forward
+    size_t ld_x, ld_z, ld_h0;
+    T *res, *last; // forward: h, last states
+    size_t ld_res, ld_last;
+    const T *h, *d_out, *d_last; // backward
+    size_t ld_h, ld_do, ld_dl;
+    T *d_x, *d_z, *d_h0;
+    size_t ld_dx, ld_dz, ld_dh0;
+    Spans sp;
+    size_t num_seq, channels, tokens;
+    size_t blocks, chunks, padded; // channel blocks, row chunks, channels as the workspace counts them
+    unsigned long long *ws;        // nullptr: there is one chunk
+    int *rec;
+};
+
+constexpr int ROW_LIVE = 1, ROW_FIRST = 2, ROW_LAST = 4;
+
+// A workgroup takes LC lanes x VEC channels and LC lanes share a row; its THREADS / LC row groups take R rows each. BACK: rows in
+// reverse; the number i of a row counts in scanning order.
+template <typename T, int VEC, int LC, int R, bool BACK>
+__global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
+    constexpr int RG = THREADS / LC, ROWS = RG * R, CW = LC * VEC, NW = Words<T>::N, WAVES = THREADS / DH_WAVE;
+    constexpr int LB = RG < 16 ? RG : 16; // predecessors looked at in one round
+    // ROW_*: which rows open the chain (take a given carry) and which close it (give their carry away), in scanning order
+    constexpr int OPENS = BACK ? ROW_LAST : ROW_FIRST, CLOSES = BACK ? ROW_FIRST : ROW_LAST;
+    __shared__ unsigned long long ticket_lds;
+    __shared__ int flags[ROWS];
+    __shared__ unsigned seq_of[ROWS];
+    constexpr int SLOTS = LB > WAVES ? LB : WAVES;
+    __shared__ T sA[SLOTS][CW], sB[SLOTS][CW]; // compositions of the wavefronts, then of the predecessors
+    __shared__ int sOpen[SLOTS][LC];
+    const unsigned tid = threadIdx.x, lc = tid % LC, g = tid / LC, wave = tid / DH_WAVE;
+    unsigned long long ticket = blockIdx.x;
+    if (a.ws) { // workgroups take chunks in the order in which they start, so that whoever is waited for is running
+        if (tid == 0)
+            ticket_lds = atomicAdd(a.ws, 1ull);
+        __syncthreads();
+        ticket = ticket_lds;
+    }
+    const size_t chunk = ticket / a.blocks, block = ticket % a.blocks;
+    const size_t c0 = block * CW + lc * VEC;
+    const bool on = c0 < a.channels; // vectors are whole: channels is a multiple of VEC
+    const size_t cc = on ? c0 : 0;
+    const size_t first_i = chunk * ROWS, my_i = first_i + static_cast<size_t>(g) * R;
+    // scanning order number -> row; numbers past the last one read the last one and count for nothing
+    auto row_of = [&](size_t i) -> size_t {
+        i = i < a.tokens ? i : a.tokens - 1;
+        return BACK ? a.tokens - 1 - i : i;
+    };
+
+    T va[R][VEC], vb[R][VEC];                               // forward: z, x. backward: z, d_out
+    T xv[BACK ? R : 1][VEC], hv[BACK ? R : 1][VEC];         // backward: x, h one row earlier
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        const size_t row = row_of(my_i + k);
+        dh_load_vec_stream<T, VEC>(a.z + row * a.ld_z + cc, va[k]);
+        dh_load_vec_stream<T, VEC>(BACK ? a.d_out + row * a.ld_do + cc : a.x + row * a.ld_x + cc, vb[k]);
+    }
+    if constexpr (BACK)
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            const size_t row = row_of(my_i + k);
+            dh_load_vec_stream<T, VEC>(a.x + row * a.ld_x + cc, xv[k]);
+            dh_load_vec_stream<T, VEC>(a.h + (row ? row - 1 : 0) * a.ld_h + cc, hv[k]);
+        }
+    // which sequence each row belongs to
+    bool plain = true; // rows that are all live and neither first nor last: most chunks of long sequences
+    for (int q = tid; q < ROWS; q += THREADS) {
+        const size_t i = first_i + q;
+        int fl = 0;
+        size_t s = 0;
+        if (i < a.tokens) {
+            const size_t row = row_of(i);
+            size_t begin, end;
+            if (a.sp.offsets == nullptr) {
+                s = row / a.sp.even;
+                begin = s * a.sp.even;
+                end = begin + a.sp.even;
+            } else { // the last sequence that begins at this row or before it
+                size_t lo = 0, hi = a.num_seq;
+                while (hi - lo > 1) {
+                    const size_t mid = lo + (hi - lo) / 2;
+                    if (a.sp.at(mid) <= row)
+                        lo = mid;
+                    else
+                        hi = mid;
+                }
+                s = lo;
+                begin = a.sp.at(s);
+                end = a.sp.at(s + 1);
+            }
+            if (row >= begin && row < end)
+                fl = ROW_LIVE | (row == begin ? ROW_FIRST : 0) | (row + 1 == end ? ROW_LAST : 0);
+        }
+        flags[q] = fl;
+        seq_of[q] = static_cast<unsigned>(s);
+        plain &= fl == ROW_LIVE;
+    }
+    if (a.sp.offsets) {
+        check_offsets(a.sp, a.num_seq, ticket * THREADS + tid, static_cast<size_t>(a.blocks * a.chunks) * THREADS, a.rec);
+        if (on) // sequences without rows hand their state on
+            for (size_t s = chunk * RG + g; s < a.num_seq; s += a.chunks * RG)
+                if (a.sp.at(s) >= a.sp.at(s + 1)) {
+                    T v[VEC] = {};
+                    const T *src = BACK ? a.d_last : a.h0;
+                    T *dst = BACK ? a.d_h0 : a.last;
+                    if (src)
+                        dh_load_vec<T, VEC>(src + s * (BACK ? a.ld_dl : a.ld_h0) + c0, v);
+                    if (dst)
+                        dh_store_vec<T, VEC>(dst + s * (BACK ? a.ld_dh0 : a.ld_last) + c0, v);
+                }
+    }
+    plain = __syncthreads_and(plain);
+
+    // The rows' maps: va = A, vb = B (a row that opens the chain: B whole, from its given carry). Backward keeps 1 - f, d_out
+    // and h_{t-1} - x_t beside them, in xv, its own registers and hv.
+    T d[BACK ? R : 1][VEC];
+    T A[VEC], B[VEC];
+    bool open = false;
+#pragma unroll
+    for (int e = 0; e < VEC; e++)
+        A[e] = T(1), B[e] = T(0);
+    auto maps = [&](auto simple) {
+        constexpr bool SIMPLE = decltype(simple)::value;
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            const int fl = SIMPLE ? ROW_LIVE : flags[g * R + k];
+            T given[VEC] = {};
+            if constexpr (!SIMPLE) {
+                const size_t s = seq_of[g * R + k];
+                const T *src = BACK ? a.d_last : a.h0;
+                if ((fl & OPENS) && src)
+                    dh_load_vec<T, VEC>(src + s * (BACK ? a.ld_dl : a.ld_h0) + cc, given);
+                if constexpr (BACK)
+                    if (fl & ROW_FIRST) {
+                        if (a.h0)
+                            dh_load_vec<T, VEC>(a.h0 + s * a.ld_h0 + cc, hv[k]);
+                        else
+#pragma unroll
+                            for (int e = 0; e < VEC; e++)
+                                hv[k][e] = T(0);
+                    }
+                if (fl & OPENS)
+                    open = true;
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                T f, om;
+                gates(va[k][e], f, om);
+                if constexpr (BACK) {
+                    hv[k][e] -= xv[k][e];
+                    xv[k][e] = om;
+                    d[k][e] = vb[k][e];
+                    vb[k][e] *= f;
+                } else {
+                    vb[k][e] *= om;
+                }
+                if constexpr (!SIMPLE) {
+                    if (!(fl & ROW_LIVE)) {
+                        f = T(1);
+                        vb[k][e] = T(0);
+                    }
+                    if (fl & OPENS) {
+                        if constexpr (BACK)
+                            d[k][e] += given[e]; // the carry is inside d_out's row from here on
+                        vb[k][e] += f * given[e];
+                    }
+                }
+                va[k][e] = f;
+                const bool opens = !SIMPLE && (fl & OPENS);
+                A[e] = opens ? T(0) : A[e] * f;
+                B[e] = opens ? vb[k][e] : f * B[e] + vb[k][e];
+            }
+        }
+    };
+    if (plain)
+        maps(std::true_type{});
+    else
+        maps(std::false_type{});
+    // Inclusive composition over the row groups of the wavefront, then what comes in front of it within the chunk.
+    T pA[VEC], pB[VEC]; // in front of this row group
+    bool popen = false;
+    {
+        T iA[VEC], iB[VEC];
+        int io = open;
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            iA[e] = A[e], iB[e] = B[e];
+#pragma unroll
+        for (int step = LC; step < DH_WAVE; step <<= 1) {
+            const bool take = tid % DH_WAVE >= static_cast<unsigned>(step);
+            const int qo = __shfl_up(io, step, DH_WAVE);
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const T qa = __shfl_up(iA[e], step, DH_WAVE), qb = __shfl_up(iB[e], step, DH_WAVE);
+                iB[e] = take && !io ? iA[e] * qb + iB[e] : iB[e];
+                iA[e] = take ? iA[e] * qa : iA[e];
+            }
+            io |= take && qo;
+        }
+        if (tid % DH_WAVE >= DH_WAVE - LC) {
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                sA[wave][lc * VEC + e] = iA[e], sB[wave][lc * VEC + e] = iB[e];
+            sOpen[wave][lc] = io;
+        }
+        // exclusive within the wavefront
+        const int qo = __shfl_up(io, LC, DH_WAVE);
+        const bool lead = tid % DH_WAVE < LC;
+        T eA[VEC], eB[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const T qa = __shfl_up(iA[e], LC % DH_WAVE, DH_WAVE), qb = __shfl_up(iB[e], LC % DH_WAVE, DH_WAVE);
+            eA[e] = lead ? T(1) : qa;
+            eB[e] = lead ? T(0) : qb;
+        }
+        const bool eo = !lead && qo;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            pA[e] = T(1), pB[e] = T(0);
+        for (unsigned q = 0; q < wave; q++) {
+            const bool o = sOpen[q][lc];
+            popen |= o;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const T qa = sA[q][lc * VEC + e], qb = sB[q][lc * VEC + e];
+                pB[e] = o ? qb : qa * pB[e] + qb;
+                pA[e] *= qa;
+            }
+        }
+        popen |= eo;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            pB[e] = eo ? eB[e] : eA[e] * pB[e] + eB[e];
+            pA[e] *= eA[e];
+        }
+    }
+    T carry[VEC] = {}; // what enters the chunk; a chunk that no carry enters takes 0, and no row uses it
+    if (a.ws) {
+        const bool alone = chunk == 0 || (flags[0] & OPENS); // the same in all threads
+        unsigned long long *mine = a.ws + 32 + chunk * 3 * NW * a.padded + c0;
+        const size_t field = static_cast<size_t>(NW) * a.padded;
+        const bool publisher = g == RG - 1 && chunk + 1 < a.chunks;
+        const bool copen = popen || open;
+        T cA[VEC], cB[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            cA[e] = pA[e] * A[e];
+            cB[e] = open ? B[e] : A[e] * pB[e] + B[e];
+        }
+        if (publisher) {
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                if (copen || alone) {
+                    publish(mine + 2 * field + e, a.padded, cB[e]);
+                } else {
+                    publish(mine + e, a.padded, cA[e]);
+                    publish(mine + field + e, a.padded, cB[e]);
+                }
+            }
+        }
+        if (!alone) {
+            T run[VEC]; // A of what has been looked at, from the chunk's front backwards
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                run[e] = T(1);
+            bool done = false;
+            for (size_t back = 1;; back += LB) { // LB predecessors at a time, one a row group
+                T la[VEC], lb[VEC];
+                int got = 0; // 1: a composition, 2: a whole carry
+                if (g < LB && back + g <= chunk) {
+                    const unsigned long long *theirs = a.ws + 32 + (chunk - back - g) * 3 * NW * a.padded + c0;
+                    // A predecessor runs (tickets) and publishes its composition without waiting for anybody. The bound is
+                    // for a workspace that an overlapping call has overwritten: the call ends, and its results are NaN.
+                    for (unsigned tries = 0; got == 0 && tries < (1u << 20); tries++) {
+                        bool all = true;
+#pragma unroll
+                        for (int e = 0; e < VEC; e++)
+                            all &= published(theirs + 2 * field + e, a.padded, lb[e]);
+                        if (all) {
+                            got = 2;
+                            break;
+                        }
+                        all = true;
+#pragma unroll
+                        for (int e = 0; e < VEC; e++) {
+                            all &= published(theirs + e, a.padded, la[e]);
+                            all &= published(theirs + field + e, a.padded, lb[e]);
+                        }
+                        if (all)
+                            got = 1;
+                        else
+                            __builtin_amdgcn_s_sleep(1);
+                    }
+                    if (got == 0) {
+                        got = 2;
+#pragma unroll
+                        for (int e = 0; e < VEC; e++)
+                            lb[e] = static_cast<T>(dh_nan<double>());
+                    }
+                }
+                __syncthreads(); // sA and sB have been read
+                if (g < LB) {
+                    sOpen[g][lc] = got;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        sA[g][lc * VEC + e] = got == 1 ? la[e] : T(0);
+                        sB[g][lc * VEC + e] = got ? lb[e] : T(0);
+                    }
+                }
+                __syncthreads();
+                for (unsigned q = 0; q < LB && !done; q++) {
+                    done = sOpen[q][lc] != 1; // a whole carry (the first chunk always has one)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        carry[e] += run[e] * sB[q][lc * VEC + e];
+                        run[e] *= sA[q][lc * VEC + e];
+                    }
+                }
+                if (__syncthreads_and(done))
+                    break;
+            }
+            if (publisher && !copen)
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    publish(mine + 2 * field + e, a.padded, cA[e] * carry[e] + cB[e]);
+        }
+    }
+    if (!on)
+        return;
+    T v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++)
+        v[e] = popen ? pB[e] : pA[e] * carry[e] + pB[e];
+    auto rows = [&](auto simple) {
+        constexpr bool SIMPLE = decltype(simple)::value;
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            const int fl = SIMPLE ? ROW_LIVE : flags[g * R + k];
+            const size_t row = row_of(my_i + k);
+            if constexpr (BACK) {
+                T gx[VEC], gz[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; e++) {
+                    const T G = (fl & OPENS) ? d[k][e] : d[k][e] + v[e];
+                    gx[e] = xv[k][e] * G;
+                    gz[e] = G * hv[k][e] * va[k][e] * xv[k][e];
+                    v[e] = (fl & OPENS) ? vb[k][e] : va[k][e] * v[e] + vb[k][e];
+                }
+                if (fl & ROW_LIVE) {
+                    dh_store_vec_stream<T, VEC>(a.d_x + row * a.ld_dx + c0, gx);
+                    dh_store_vec_stream<T, VEC>(a.d_z + row * a.ld_dz + c0, gz);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    v[e] = (fl & OPENS) ? vb[k][e] : va[k][e] * v[e] + vb[k][e];
+                if (fl & ROW_LIVE)
+                    dh_store_vec_stream<T, VEC>(a.res + row * a.ld_res + c0, v);
+            }
+            if constexpr (!SIMPLE) {
+                T *out = BACK ? a.d_h0 : a.last;
+                if ((fl & CLOSES) && out)
+                    dh_store_vec<T, VEC>(out + static_cast<size_t>(seq_of[g * R + k]) * (BACK ? a.ld_dh0 : a.ld_last) + c0, v);
+            }
+        }
+    };
+    if (plain)
+        rows(std::true_type{});
+    else
+        rows(std::false_type{});
+}
+
+// Shape of a chunk, chosen by measurement (32768 rows; forward 2048 channels in 8 sequences, backward 1024 in 5):
+//   8 lanes of 16-byte vectors a row, so that a chunk is 128 bytes wide and 256 (backward 128) rows tall: 158 and 181 us. What a
+//   chunk reads back of its predecessors is as wide as the chunk and as long as there are chunks of its channels in
+//   flight, so tall and narrow is cheap: 16 lanes 191 and 219 us. 4 lanes take less than a memory line of a row: 273 and 250.
+//   8 rows a thread forward (4 backward, which holds twice as many arrays): 167 registers, 3 wavefronts a SIMD. 16 (8) rows leave
+//   one: 195 and 193 us; 4 rows forward 238 us.
+// Without any look-back (sequences as long as a chunk) the same rows take 147 and 157 us, a plain copy of as many bytes 155.
+constexpr int ROWS_FORWARD = 8, ROWS_BACKWARD = 4, LANES = 8;
 
 // What every entry point checks of its sequences.
 static inline dh_status check_sequences(const char *what, const long long *offsets, size_t ld_offsets, size_t num_seq, size_t tokens) {
@@ -104,7 +547,82 @@ static inline dh_status check_sequences(const char *what, const long long *offse
     return DH_OK;
 }
 
-template <typename T> size_t workspace(size_t, size_t, size_t) { return 0; }
+// Sequences short enough for a thread to walk: below this many rows each, all of one length.
+constexpr size_t SERIAL_ROWS = 8;
+
+// Shape of a pass: vectors or single values, row chunks and channel blocks. Chunks are cut as tall as the registers allow,
+// and a quarter of that where so few workgroups would leave compute units idle.
+struct Plan {
+    int vec, lanes, rows;
+    size_t blocks, chunks, padded;
+};
+template <typename T> Plan plan(size_t tokens, size_t channels, bool vec, bool back) {
+    Plan p;
+    p.vec = vec ? dh_vec<T>::N : 1;
+    p.lanes = vec ? LANES : 64;
+    p.blocks = dh_ceil_div(channels, static_cast<size_t>(p.lanes) * p.vec);
+    p.padded = p.blocks * p.lanes * p.vec;
+    const int tall = back ? ROWS_BACKWARD : ROWS_FORWARD;
+    const size_t groups = THREADS / p.lanes;
+    p.rows = p.blocks * dh_ceil_div(tokens, groups * tall) < 256 ? tall / 4 : tall;
+    p.chunks = dh_ceil_div(tokens, groups * p.rows);
+    return p;
+}
+template <typename T> size_t plan_bytes(const Plan &p) {
+    return p.chunks > 1 ? 256 + p.chunks * 3 * Words<T>::N * p.padded * sizeof(unsigned long long) : 0;
+}
+
+// Enough for every alignment and direction.
+template <typename T> size_t workspace(size_t tokens, size_t num_seq, size_t channels) {
+    (void)num_seq;
+    size_t most = 0;
+    if (tokens && channels)
+        for (int k = 0; k < 4; k++) {
+            if ((k & 1) && channels % dh_vec<T>::N)
+                continue;
+            const size_t b = plan_bytes<T>(plan<T>(tokens, channels, k & 1, k & 2));
+            most = b > most ? b : most;
+        }
+    return most;
+}
+
+template <typename T, int VEC, int LC, int R, bool BACK> static inline void launch_scan(dh_ctx *ctx, const ScanArgs<T> &a) {
+    hipLaunchKernelGGL((scan_kernel<T, VEC, LC, R, BACK>), dim3(static_cast<unsigned>(a.blocks * a.chunks)), dim3(THREADS), 0, ctx->stream, a);
+}
+
+template <typename T, bool BACK>
+dh_status scan(dh_ctx *ctx, const char *what, ScanArgs<T> &a, const Plan &p, void *ws, size_t ws_bytes) {
+    void *work = nullptr;
+    const size_t need = plan_bytes<T>(p);
+    if (dh_status st = dh_call_workspace(ctx, what, ws, ws_bytes, need, &work); st != DH_OK)
+        return st;
+    if (p.blocks * p.chunks >= (size_t(1) << 31) || a.num_seq >= (size_t(1) << 32))
+        return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
+    a.blocks = p.blocks;
+    a.chunks = p.chunks;
+    a.padded = p.padded;
+    a.ws = static_cast<unsigned long long *>(work);
+    if (work) {
+        const size_t n = need / 16, grid = dh_ceil_div(n, THREADS * 4);
+        hipLaunchKernelGGL(clear_kernel, dim3(static_cast<unsigned>(grid < 2048 ? grid : 2048)), dim3(THREADS), 0, ctx->stream,
+                           static_cast<ulonglong2 *>(work), n);
+    }
+    constexpr int V = dh_vec<T>::N, R = BACK ? ROWS_BACKWARD : ROWS_FORWARD;
+    if (p.vec > 1 && p.rows == R)
+        launch_scan<T, V, LANES, R, BACK>(ctx, a);
+    else if (p.vec > 1)
+        launch_scan<T, V, LANES, R / 4, BACK>(ctx, a);
+    else if (p.rows == R)
+        launch_scan<T, 1, 64, R, BACK>(ctx, a);
+    else
+        launch_scan<T, 1, 64, R / 4, BACK>(ctx, a);
+    DH_CHECK_LAUNCH();
+    return DH_OK;
+}
+
+template <typename T> static inline bool whole_vectors(const T *p, size_t ld) {
+    return p == nullptr || (ld % dh_vec<T>::N == 0 && dh_aligned(p, 16));
+}
 
 template <typename T>
 dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, T *last, size_t ld_last, const T *x, size_t tokens, size_t channels, size_t ld_x,
@@ -124,16 +642,24 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, T *last, size_t ld_last, c
     if (offsets)
         if (dh_status st = dh_checked_begin(ctx, what, &rec); st != DH_OK)
             return st;
-    void *work = nullptr;
-    if (dh_status st = dh_call_workspace(ctx, what, ws, ws_bytes, workspace<T>(tokens, num_seq, channels), &work); st != DH_OK)
-        return st;
-    const size_t gx = dh_ceil_div(channels, THREADS);
-    if (gx >= (size_t(1) << 31) || num_seq >= 65536)
-        return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
     const Spans sp{offsets, ld_offsets, tokens / num_seq, tokens};
-    hipLaunchKernelGGL((forward_serial_kernel<T>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(num_seq)), dim3(THREADS), 0,
-                       ctx->stream, res, ld_res, last, ld_last, x, ld_x, z, ld_z, h0, ld_h0, sp, num_seq, channels, rec);
-    DH_CHECK_LAUNCH();
+    if (tokens == 0 || (offsets == nullptr && sp.even <= SERIAL_ROWS)) {
+        const size_t gx = dh_ceil_div(channels, THREADS), gy = num_seq < 65535 ? num_seq : 65535;
+        if (gx >= (size_t(1) << 31))
+            return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
+        hipLaunchKernelGGL((forward_serial_kernel<T>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), dim3(THREADS), 0,
+                           ctx->stream, res, ld_res, last, ld_last, x, ld_x, z, ld_z, h0, ld_h0, sp, num_seq, channels, rec);
+        DH_CHECK_LAUNCH();
+        return offsets ? dh_checked_end(ctx) : DH_OK;
+    }
+    const bool vec = channels % dh_vec<T>::N == 0 && whole_vectors(x, ld_x) && whole_vectors(z, ld_z) && whole_vectors(h0, ld_h0) &&
+                     whole_vectors(res, ld_res) && whole_vectors(last, ld_last);
+    ScanArgs<T> a{};
+    a.x = x, a.ld_x = ld_x, a.z = z, a.ld_z = ld_z, a.h0 = h0, a.ld_h0 = ld_h0;
+    a.res = res, a.ld_res = ld_res, a.last = last, a.ld_last = ld_last;
+    a.sp = sp, a.num_seq = num_seq, a.channels = channels, a.tokens = tokens, a.rec = rec;
+    if (dh_status st = scan<T, false>(ctx, what, a, plan<T>(tokens, channels, vec, false), ws, ws_bytes); st != DH_OK)
+        return st;
     return offsets ? dh_checked_end(ctx) : DH_OK;
 }
 
@@ -157,17 +683,27 @@ dh_status backward(dh_ctx *ctx, T *d_x, size_t ld_dx, T *d_z, size_t ld_dz, T *d
     if (offsets)
         if (dh_status st = dh_checked_begin(ctx, what, &rec); st != DH_OK)
             return st;
-    void *work = nullptr;
-    if (dh_status st = dh_call_workspace(ctx, what, ws, ws_bytes, workspace<T>(tokens, num_seq, channels), &work); st != DH_OK)
-        return st;
-    const size_t gx = dh_ceil_div(channels, THREADS);
-    if (gx >= (size_t(1) << 31) || num_seq >= 65536)
-        return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
     const Spans sp{offsets, ld_offsets, tokens / num_seq, tokens};
-    hipLaunchKernelGGL((backward_serial_kernel<T>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(num_seq)), dim3(THREADS), 0,
-                       ctx->stream, d_x, ld_dx, d_z, ld_dz, d_h0, ld_dh0, x, ld_x, z, ld_z, h, ld_h, h0, ld_h0, d_out, ld_do, d_last, ld_dl,
-                       sp, num_seq, channels, rec);
-    DH_CHECK_LAUNCH();
+    if (tokens == 0 || (offsets == nullptr && sp.even <= SERIAL_ROWS)) {
+        const size_t gx = dh_ceil_div(channels, THREADS), gy = num_seq < 65535 ? num_seq : 65535;
+        if (gx >= (size_t(1) << 31))
+            return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
+        hipLaunchKernelGGL((backward_serial_kernel<T>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), dim3(THREADS), 0,
+                           ctx->stream, d_x, ld_dx, d_z, ld_dz, d_h0, ld_dh0, x, ld_x, z, ld_z, h, ld_h, h0, ld_h0, d_out, ld_do, d_last,
+                           ld_dl, sp, num_seq, channels, rec);
+        DH_CHECK_LAUNCH();
+        return offsets ? dh_checked_end(ctx) : DH_OK;
+    }
+    const bool vec = channels % dh_vec<T>::N == 0 && whole_vectors(x, ld_x) && whole_vectors(z, ld_z) && whole_vectors(h, ld_h) &&
+                     whole_vectors(h0, ld_h0) && whole_vectors(d_out, ld_do) && whole_vectors(d_last, ld_dl) &&
+                     whole_vectors<T>(d_x, ld_dx) && whole_vectors<T>(d_z, ld_dz) && whole_vectors<T>(d_h0, ld_dh0);
+    ScanArgs<T> a{};
+    a.x = x, a.ld_x = ld_x, a.z = z, a.ld_z = ld_z, a.h0 = h0, a.ld_h0 = ld_h0, a.h = h, a.ld_h = ld_h;
+    a.d_out = d_out, a.ld_do = ld_do, a.d_last = d_last, a.ld_dl = ld_dl;
+    a.d_x = d_x, a.ld_dx = ld_dx, a.d_z = d_z, a.ld_dz = ld_dz, a.d_h0 = d_h0, a.ld_dh0 = ld_dh0;
+    a.sp = sp, a.num_seq = num_seq, a.channels = channels, a.tokens = tokens, a.rec = rec;
+    if (dh_status st = scan<T, true>(ctx, what, a, plan<T>(tokens, channels, vec, true), ws, ws_bytes); st != DH_OK)
+        return st;
     return offsets ? dh_checked_end(ctx) : DH_OK;
 }
 
