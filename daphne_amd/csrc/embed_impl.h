@@ -11,6 +11,8 @@
 
 #include "common.h"
 
+#include <type_traits>
+
 namespace dh_embed {
 
 constexpr int THREADS = 256;
@@ -93,7 +95,7 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, const T *table, size_t voc
     return dh_checked_end(ctx);
 }
 
-// One workgroup per table row and slice of THREADS columns: the positions of its token are picked out of every THREADS
+// Tables beyond what the sorted form below takes (more than 8 Mi rows): one workgroup per table row and slice of THREADS columns; the positions of its token are picked out of every THREADS
 // token numbers in order, and their rows added.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size_t ld, long long vocab, size_t width, const T *d_out,
@@ -137,7 +139,562 @@ __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size
     }
 }
 
-template <typename T> size_t backward_workspace(size_t, size_t, size_t) { return 0; }
+// ---------------------------------------------------------------------------------------
+// backward by sorted tokens
+// ---------------------------------------------------------------------------------------
+// sort_kernel puts the positions of all tokens in the order of their rows (stable: positions stay in order) and notes where each
+// row's begin. A workgroup owns VR consecutive rows and finds their positions by reading all tokens: 16 wavefronts go through
+// a share each, once to count and once to place. Beyond SCAN_TOKENS that reading would cost too much: the tokens are first split
+// into lists, one per owner, by a stable partition (count, scan, scatter).
+// rows_kernel then writes every row, zeros where there is nothing to add: 64 lanes of 16 bytes (fewer where rows are shorter)
+// per row and step. A token that occurs more than HOT times would keep its lanes busy long after all others: its positions are
+// taken in parts of PART; a token of one part is finished there, the parts of others are added in order by join_kernel.
+// The parts' descriptors need no counters: an owner whose positions are numbers [b, e) of all sorted positions has the slots
+// [b / HOT, e / HOT), and never fewer than it has parts (a token with c > HOT positions has ceil(c / PART) <= c / HOT), and in
+// the same way the slots [b / PART, e / PART) for its tokens of several parts. It marks those that it does not use.
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / DH_WAVE;
+constexpr unsigned HOT = 8, PART = 32;
+constexpr size_t SCAN_TOKENS = 32 * SORT_THREADS; // up to here every owner reads all tokens
+constexpr int ROW_BITS = 8;             // an owner has 1 << ROW_BITS rows, more in large tables
+constexpr size_t OWNERS = 4096;         // most owners
+constexpr size_t MOST_ROWS = 2048;      // most rows of an owner
+constexpr size_t PART_THREADS = 256, PART_WAVES = PART_THREADS / DH_WAVE;
+
+struct HotPart { // positions [begin, end) of `sorted`; end = 0: none
+    unsigned begin, end, row, whole; // whole: the row's only part
+};
+struct HotRow { // parts = 0: none
+    unsigned row, first_part, parts, unused;
+};
+
+// Positions of lanes with the same key among the wavefront's `in` lanes, by one ballot per bit of the key.
+__device__ __forceinline__ unsigned long long same_key(bool in, unsigned key, int bits) {
+    unsigned long long same = __ballot(in);
+    for (int b = 0; b < bits; b++) {
+        const bool bit = (key >> b) & 1;
+        const unsigned long long m = __ballot(bit);
+        same &= bit ? m : ~m;
+    }
+    return same;
+}
+// The next places for lanes of equal keys, in lane order, from the wavefront's counters in LDS.
+__device__ __forceinline__ unsigned next_place(unsigned *counter, bool in, unsigned key, int bits) {
+    const unsigned lane = threadIdx.x % DH_WAVE;
+    const unsigned long long same = same_key(in, key, bits);
+    const unsigned rank = __popcll(same & ((1ull << lane) - 1));
+    unsigned base = 0;
+    if (in && rank == 0)
+        base = atomicAdd(&counter[key], static_cast<unsigned>(__popcll(same)));
+    return __shfl(base, in ? static_cast<int>(__ffsll(static_cast<long long>(same))) - 1 : 0, DH_WAVE) + rank;
+}
+
+struct SortArgs {
+    unsigned vocab;
+    const long long *ids;
+    size_t ld_ids, n;
+    unsigned rows_each; // a power of two
+    int row_bits;
+    const unsigned *starts; // partition: first place of owner b's list at starts[b * blocks], behind the last one the end
+    size_t blocks;
+    const unsigned long long *list; // row within the owner's << 32 | position
+    unsigned *row_starts;           // [vocab + 1]
+    unsigned *sorted;
+    HotRow *hot_rows;
+    HotPart *hot_parts;
+    unsigned parts, hots; // slots
+    int *rec;
+};
+
+// HELD: owners read all tokens, a wavefront HELD times 64 of them at most, which stay in registers between counting and
+// placing. HELD = 0: owners read their lists, once for each.
+template <int HELD> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(SortArgs a) {
+    constexpr bool SCAN = HELD != 0;
+    extern __shared__ unsigned sort_lds[];
+    const unsigned VR = a.rows_each, tid = threadIdx.x, wave = tid / DH_WAVE, lane = tid % DH_WAVE;
+    unsigned *seg = sort_lds;     // [VR + 1]
+    unsigned *cnt = seg + VR + 1; // [SORT_WAVES][VR]
+    unsigned *mine = cnt + wave * VR;
+    __shared__ unsigned front;    // SCAN: positions of all rows before this owner's
+    const unsigned row0 = blockIdx.x * VR, rows = a.vocab - row0 < VR ? a.vocab - row0 : VR;
+    const size_t begin = SCAN ? 0 : a.starts[blockIdx.x * a.blocks], end = SCAN ? a.n : a.starts[(blockIdx.x + 1) * a.blocks];
+    const size_t share = (end - begin + SORT_THREADS - 1) / SORT_THREADS * DH_WAVE; // what a wavefront goes through, in order
+    const size_t w0 = begin + wave * share < end ? begin + wave * share : end, w1 = w0 + share < end ? w0 + share : end;
+    unsigned row[SCAN ? HELD : 1], rank[SCAN ? HELD : 1];
+    if constexpr (SCAN) {
+        long long v[HELD];
+#pragma unroll
+        for (int u = 0; u < HELD; u++) {
+            const size_t i = w0 + u * DH_WAVE + lane;
+            v[u] = i < w1 ? a.ids[i * a.ld_ids] : -1;
+        }
+        unsigned lower = 0;
+#pragma unroll
+        for (int u = 0; u < HELD; u++) {
+            const bool valid = v[u] >= 0 && v[u] < static_cast<long long>(a.vocab);
+            if (blockIdx.x == 0 && !valid && w0 + u * DH_WAVE + lane < w1)
+                dh_raise(a.rec, DH_DEFERRED_TOKEN_ID, 0, v[u], a.vocab);
+            const unsigned id = valid ? static_cast<unsigned>(v[u]) : ~0u;
+            lower += id < row0;
+            row[u] = id >= row0 && id - row0 < rows ? id - row0 : ~0u;
+        }
+        for (unsigned i = tid; i < VR * SORT_WAVES; i += SORT_THREADS)
+            cnt[i] = 0;
+        if (tid == 0)
+            front = 0;
+        __syncthreads();
+        if (lower)
+            atomicAdd(&front, lower);
+#pragma unroll
+        for (int u = 0; u < HELD; u++) {
+            const bool in = row[u] != ~0u;
+            rank[u] = 0;
+            if (__ballot(in) != 0)
+                rank[u] = next_place(mine, in, in ? row[u] : 0, a.row_bits);
+        }
+    } else {
+        for (unsigned i = tid; i < VR * SORT_WAVES; i += SORT_THREADS)
+            cnt[i] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (size_t i = w0 + lane; i < w1; i += DH_WAVE)
+            atomicAdd(&mine[a.list[i] >> 32], 1u);
+    }
+    __syncthreads();
+    const unsigned all0 = SCAN ? front : static_cast<unsigned>(begin); // number of this owner's first position among all
+    for (unsigned r = tid; r < VR; r += SORT_THREADS) {
+        unsigned s = 0;
+        for (int w = 0; w < SORT_WAVES; w++)
+            s += cnt[w * VR + r];
+        seg[r] = s;
+    }
+    __syncthreads();
+    if (wave == 0) { // exclusive sums over the rows
+        unsigned before = 0;
+        for (unsigned r0 = 0; r0 < VR; r0 += DH_WAVE) {
+            const unsigned own = r0 + lane < VR ? seg[r0 + lane] : 0;
+            unsigned s = own;
+            for (int d = 1; d < DH_WAVE; d <<= 1) {
+                const unsigned o = __shfl_up(s, d, DH_WAVE);
+                s += lane >= static_cast<unsigned>(d) ? o : 0;
+            }
+            if (r0 + lane < VR)
+                seg[r0 + lane] = before + s - own;
+            before += __shfl(s, DH_WAVE - 1, DH_WAVE);
+        }
+        if (lane == 0)
+            seg[VR] = before;
+    }
+    __syncthreads();
+    for (unsigned r = tid; r < VR; r += SORT_THREADS) {
+        unsigned at = seg[r];
+        if (r < rows)
+            a.row_starts[row0 + r] = all0 + at;
+        for (int w = 0; w < SORT_WAVES; w++) {
+            const unsigned c = cnt[w * VR + r];
+            cnt[w * VR + r] = at;
+            at += c;
+        }
+    }
+    const bool last = blockIdx.x + 1 == gridDim.x;
+    if (last && tid == 0)
+        a.row_starts[a.vocab] = all0 + seg[VR];
+    __syncthreads();
+    if (wave == SORT_WAVES - 1) { // frequent tokens: their positions in parts
+        const unsigned all1 = all0 + seg[VR];
+        unsigned slot = all0 / HOT, row_slot = all0 / PART;
+        const unsigned slots = last ? a.parts : all1 / HOT, row_slots = last ? a.hots : all1 / PART;
+        for (unsigned r0 = 0; r0 < rows; r0 += DH_WAVE) {
+            const unsigned r = r0 + lane, c = r < rows ? seg[r + 1] - seg[r] : 0;
+            const unsigned parts = c > HOT ? (c + PART - 1) / PART : 0, many = parts > 1;
+            unsigned ps = parts, ms = many;
+            for (int d = 1; d < DH_WAVE; d <<= 1) {
+                const unsigned p = __shfl_up(ps, d, DH_WAVE), m = __shfl_up(ms, d, DH_WAVE);
+                ps += lane >= static_cast<unsigned>(d) ? p : 0;
+                ms += lane >= static_cast<unsigned>(d) ? m : 0;
+            }
+            const unsigned first = slot + ps - parts;
+            for (unsigned k = 0; k < parts; k++) {
+                const unsigned b = all0 + seg[r] + k * PART, e = all0 + seg[r + 1];
+                a.hot_parts[first + k] = HotPart{b, b + PART < e ? b + PART : e, row0 + r, parts == 1};
+            }
+            if (many)
+                a.hot_rows[row_slot + ms - 1] = HotRow{row0 + r, first, parts, 0};
+            slot += __shfl(ps, DH_WAVE - 1, DH_WAVE);
+            row_slot += __shfl(ms, DH_WAVE - 1, DH_WAVE);
+        }
+        for (unsigned k = slot + lane; k < slots; k += DH_WAVE)
+            a.hot_parts[k] = HotPart{0, 0, 0, 0};
+        for (unsigned k = row_slot + lane; k < row_slots; k += DH_WAVE)
+            a.hot_rows[k] = HotRow{0, 0, 0, 0};
+    }
+    if (seg[VR] == 0)
+        return;
+    if constexpr (SCAN) {
+#pragma unroll
+        for (int u = 0; u < HELD; u++)
+            if (row[u] != ~0u)
+                a.sorted[all0 + mine[row[u]] + rank[u]] = static_cast<unsigned>(w0 + u * DH_WAVE + lane);
+    } else {
+        for (size_t i0 = w0; i0 < w1; i0 += 4 * DH_WAVE) {
+            unsigned long long v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const size_t i = i0 + u * DH_WAVE + lane;
+                v[u] = a.list[i < w1 ? i : w1 - 1];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const bool in = i0 + u * DH_WAVE + lane < w1;
+                const unsigned at = next_place(mine, in, in ? static_cast<unsigned>(v[u] >> 32) : 0, a.row_bits);
+                if (in)
+                    a.sorted[all0 + at] = static_cast<unsigned>(v[u]);
+            }
+        }
+    }
+}
+
+template <typename T> struct RowArgs {
+    T *d_table;
+    size_t ld;
+    size_t vocab, width_vecs;
+    const T *d_out;
+    size_t ld_out;
+    double scale;
+    int accumulate;
+    const unsigned *row_starts, *sorted;
+    const HotRow *hot_rows;
+    const HotPart *hot_parts;
+    size_t parts;
+    double *partials;
+    unsigned lanes; // of a row: a power of two up to 64
+};
+
+// Adds rows [begin, end) of the positions to acc, in order.
+template <typename T, int VEC, class Position>
+__device__ __forceinline__ void add_rows(double (&acc)[VEC], const T *d_out, size_t ld_out, size_t begin, size_t end, Position position) {
+    auto round = [&](auto most, size_t k) { // up to that many rows, all loads in flight together
+        constexpr int N = decltype(most)::value;
+        T v[N][VEC];
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            dh_load_vec_stream<T, VEC>(d_out + static_cast<size_t>(position(k + u < end ? k + u : end - 1)) * ld_out, v[u]);
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            if (k + u < end)
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    acc[e] += static_cast<double>(v[u][e]);
+    };
+    size_t k = begin;
+    for (; k + 4 < end; k += 8)
+        round(std::integral_constant<int, 8>{}, k);
+    if (k + 1 < end)
+        round(std::integral_constant<int, 4>{}, k);
+    else if (k < end)
+        round(std::integral_constant<int, 1>{}, k);
+}
+
+template <typename T, int VEC> __device__ __forceinline__ void write_row(const RowArgs<T> &a, size_t row, size_t vec, const double (&acc)[VEC]) {
+    T *p = a.d_table + row * a.ld + vec * VEC, v[VEC];
+    if (a.accumulate)
+        dh_load_vec<T, VEC>(p, v);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        const double s = acc[e] * a.scale;
+        v[e] = static_cast<T>(a.accumulate ? s + static_cast<double>(v[e]) : s);
+    }
+    dh_store_vec_stream<T, VEC>(p, v);
+}
+
+// A group of `lanes` lanes takes blockIdx.y's slice of a part, or of AT_ONCE consecutive rows; the parts come first, since they
+// take longest. Rows with at most one position, which most rows of a table are, are loaded together.
+template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_kernel(RowArgs<T> a) {
+    constexpr int AT_ONCE = 4;
+    const unsigned lane = threadIdx.x % a.lanes, each = THREADS / a.lanes;
+    const size_t vec = static_cast<size_t>(blockIdx.y) * a.lanes + lane;
+    if (vec >= a.width_vecs)
+        return;
+    const size_t units = a.parts + (a.vocab + AT_ONCE - 1) / AT_ONCE;
+    const T *column = a.d_out + vec * VEC;
+    auto position = [&](size_t k) { return a.sorted[k]; };
+    for (size_t u = static_cast<size_t>(blockIdx.x) * each + threadIdx.x / a.lanes; u < units; u += static_cast<size_t>(gridDim.x) * each) {
+        if (u < a.parts) {
+            const HotPart p = a.hot_parts[u];
+            if (p.end == 0)
+                continue;
+            double acc[VEC] = {};
+            add_rows<T, VEC>(acc, column, a.ld_out, p.begin, p.end, position);
+            if (p.whole)
+                write_row<T, VEC>(a, p.row, vec, acc);
+            else
+#pragma unroll
+                for (int q = 0; q < VEC; q++)
+                    a.partials[(u * a.width_vecs + vec) * VEC + q] = acc[q];
+            continue;
+        }
+        const size_t row = (u - a.parts) * AT_ONCE;
+        unsigned at[AT_ONCE + 1];
+#pragma unroll
+        for (int k = 0; k <= AT_ONCE; k++)
+            at[k] = a.row_starts[row + k < a.vocab ? row + k : a.vocab];
+        bool few = true;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++)
+            few &= at[k + 1] - at[k] <= 1;
+        if (few) {
+            T v[AT_ONCE][VEC];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++)
+                if (at[k + 1] != at[k])
+                    dh_load_vec_stream<T, VEC>(column + static_cast<size_t>(a.sorted[at[k]]) * a.ld_out, v[k]);
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) {
+                const bool some = at[k + 1] != at[k];
+                if (row + k >= a.vocab || (!some && a.accumulate))
+                    continue;
+                double acc[VEC];
+#pragma unroll
+                for (int q = 0; q < VEC; q++)
+                    acc[q] = some ? static_cast<double>(v[k][q]) : 0.0;
+                write_row<T, VEC>(a, row + k, vec, acc);
+            }
+        } else {
+            for (int k = 0; k < AT_ONCE; k++) {
+                const unsigned b = a.row_starts[row + k < a.vocab ? row + k : a.vocab], e = a.row_starts[row + k + 1 < a.vocab ? row + k + 1 : a.vocab];
+                if (row + k >= a.vocab || (a.parts && e - b > HOT) || (b == e && a.accumulate))
+                    continue;
+                double acc[VEC] = {};
+                add_rows<T, VEC>(acc, column, a.ld_out, b, e, position);
+                write_row<T, VEC>(a, row + k, vec, acc);
+            }
+        }
+    }
+}
+
+template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void join_kernel(RowArgs<T> a) {
+    __shared__ double part[THREADS / DH_WAVE][DH_WAVE * VEC];
+    const HotRow h = a.hot_rows[blockIdx.x];
+    if (h.parts == 0)
+        return;
+    const unsigned wave = threadIdx.x / DH_WAVE, lane = threadIdx.x % DH_WAVE;
+    const size_t vec = static_cast<size_t>(blockIdx.y) * DH_WAVE + lane, at = vec < a.width_vecs ? vec : a.width_vecs - 1;
+    const unsigned each = (h.parts + THREADS / DH_WAVE - 1) / (THREADS / DH_WAVE);
+    const unsigned b = wave * each < h.parts ? wave * each : h.parts, e = b + each < h.parts ? b + each : h.parts;
+    double acc[VEC] = {};
+#pragma unroll 4
+    for (size_t k = h.first_part + b; k < h.first_part + e; k++)
+#pragma unroll
+        for (int q = 0; q < VEC; q++)
+            acc[q] += a.partials[(k * a.width_vecs + at) * VEC + q];
+#pragma unroll
+    for (int q = 0; q < VEC; q++)
+        part[wave][lane * VEC + q] = acc[q];
+    __syncthreads();
+    if (wave != 0 || vec >= a.width_vecs)
+        return;
+    for (int w = 1; w < THREADS / DH_WAVE; w++)
+#pragma unroll
+        for (int q = 0; q < VEC; q++)
+            acc[q] += part[w][lane * VEC + q];
+    write_row<T, VEC>(a, h.row, vec, acc);
+}
+
+// Stable partition of the tokens by owner: how many each block of tokens has for each owner, owner by owner.
+static __global__ __launch_bounds__(PART_THREADS) void count_kernel(const long long *ids, size_t ld_ids, size_t n, size_t each, long long vocab,
+                                                                    int row_bits, size_t owners, unsigned *counts, int *rec) {
+    extern __shared__ unsigned part_lds[];
+    for (size_t b = threadIdx.x; b < owners; b += PART_THREADS)
+        part_lds[b] = 0;
+    __syncthreads();
+    const size_t i0 = blockIdx.x * each, i1 = i0 + each < n ? i0 + each : n;
+#pragma unroll 4
+    for (size_t i = i0 + threadIdx.x; i < i1; i += PART_THREADS) {
+        const long long id = ids[i * ld_ids];
+        if (id < 0 || id >= vocab)
+            dh_raise(rec, DH_DEFERRED_TOKEN_ID, 0, id, vocab);
+        else
+            atomicAdd(&part_lds[id >> row_bits], 1u);
+    }
+    __syncthreads();
+    for (size_t b = threadIdx.x; b < owners; b += PART_THREADS)
+        counts[b * gridDim.x + blockIdx.x] = part_lds[b];
+}
+
+// Exclusive sums over all counts in place, the total behind them. One workgroup.
+static __global__ __launch_bounds__(1024) void scan_counts_kernel(unsigned *counts, size_t n) {
+    __shared__ unsigned sums[1024 / DH_WAVE];
+    const unsigned wave = threadIdx.x / DH_WAVE, lane = threadIdx.x % DH_WAVE;
+    unsigned before = 0;
+    constexpr int EACH = 16;
+    for (size_t base = 0; base < n; base += 1024 * EACH) {
+        const size_t i = base + threadIdx.x * EACH;
+        unsigned v[EACH], s = 0;
+#pragma unroll
+        for (int k = 0; k < EACH; k += 4) { // the array is padded to whole vectors
+            const uint4 q = i + k < n ? *reinterpret_cast<const uint4 *>(counts + i + k) : uint4{0, 0, 0, 0};
+            v[k] = q.x, v[k + 1] = i + k + 1 < n ? q.y : 0, v[k + 2] = i + k + 2 < n ? q.z : 0, v[k + 3] = i + k + 3 < n ? q.w : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < EACH; k++)
+            s += v[k];
+        const unsigned own = s;
+        for (int d = 1; d < DH_WAVE; d <<= 1) {
+            const unsigned o = __shfl_up(s, d, DH_WAVE);
+            s += lane >= static_cast<unsigned>(d) ? o : 0;
+        }
+        if (lane == DH_WAVE - 1)
+            sums[wave] = s;
+        __syncthreads();
+        unsigned in_front = 0, total = 0;
+        for (unsigned w = 0; w < 1024 / DH_WAVE; w++) {
+            in_front += w < wave ? sums[w] : 0;
+            total += sums[w];
+        }
+        unsigned at = before + in_front + s - own;
+#pragma unroll
+        for (int k = 0; k < EACH; k++)
+            if (i + k < n) {
+                counts[i + k] = at;
+                at += v[k];
+            }
+        before += total;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0)
+        counts[n] = before;
+}
+
+static __global__ __launch_bounds__(PART_THREADS) void scatter_kernel(const long long *ids, size_t ld_ids, size_t n, size_t each, long long vocab,
+                                                                      int row_bits, int owner_bits, size_t owners, const unsigned *starts,
+                                                                      unsigned long long *list) {
+    extern __shared__ unsigned part_lds[]; // [PART_WAVES][owners]
+    const unsigned wave = threadIdx.x / DH_WAVE, lane = threadIdx.x % DH_WAVE;
+    unsigned *mine = part_lds + wave * owners;
+    for (size_t b = threadIdx.x; b < owners * PART_WAVES; b += PART_THREADS)
+        part_lds[b] = 0;
+    __syncthreads();
+    const size_t i0 = blockIdx.x * each, i1 = i0 + each < n ? i0 + each : n, span = each / PART_WAVES; // a multiple of 64
+    const size_t w0 = i0 + wave * span < i1 ? i0 + wave * span : i1, w1 = w0 + span < i1 ? w0 + span : i1;
+#pragma unroll 4
+    for (size_t i = w0 + lane; i < w1; i += DH_WAVE) {
+        const long long id = ids[i * ld_ids];
+        if (id >= 0 && id < vocab)
+            atomicAdd(&mine[id >> row_bits], 1u);
+    }
+    __syncthreads();
+    for (size_t b = threadIdx.x; b < owners; b += PART_THREADS) {
+        unsigned at = starts[b * gridDim.x + blockIdx.x];
+        for (unsigned w = 0; w < PART_WAVES; w++) {
+            const unsigned c = part_lds[w * owners + b];
+            part_lds[w * owners + b] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    for (size_t i = w0; i < w1; i += DH_WAVE) {
+        const long long id = i + lane < w1 ? ids[(i + lane) * ld_ids] : -1;
+        const bool in = id >= 0 && id < vocab;
+        const unsigned at = next_place(mine, in, in ? static_cast<unsigned>(id >> row_bits) : 0, owner_bits);
+        if (in)
+            list[at] = (static_cast<unsigned long long>(id & ((1ll << row_bits) - 1)) << 32) | static_cast<unsigned>(i + lane);
+    }
+}
+
+// How a gradient is taken, by its sizes alone.
+struct BackwardPlan {
+    enum { PLAIN, SCAN, PARTITION } how;
+    int row_bits, owner_bits;
+    size_t owners, each, blocks, parts, hots;
+    size_t starts_at, sorted_at, hot_rows_at, hot_parts_at, partials_at, counts_at, list_at, bytes;
+};
+static inline BackwardPlan backward_plan(size_t n, size_t vocab, size_t width) {
+    BackwardPlan p{};
+    p.row_bits = ROW_BITS;
+    while (((vocab - 1) >> p.row_bits) >= OWNERS)
+        p.row_bits++;
+    p.owners = dh_ceil_div(vocab, size_t(1) << p.row_bits);
+    p.how = (size_t(1) << p.row_bits) > MOST_ROWS || n >= (size_t(1) << 32) ? BackwardPlan::PLAIN
+            : n <= SCAN_TOKENS                                              ? BackwardPlan::SCAN
+                                                                            : BackwardPlan::PARTITION;
+    if (p.how == BackwardPlan::PLAIN)
+        return p;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) & ~size_t(255);
+        return here;
+    };
+    p.parts = n / HOT;
+    p.hots = n / PART;
+    p.starts_at = take((vocab + 1) * sizeof(unsigned));
+    p.sorted_at = take(n * sizeof(unsigned));
+    p.hot_rows_at = take(p.hots * sizeof(HotRow));
+    p.hot_parts_at = take(p.parts * sizeof(HotPart));
+    p.partials_at = take(p.hots ? p.parts * width * sizeof(double) : 0);
+    if (p.how == BackwardPlan::PARTITION) {
+        while ((size_t(1) << p.owner_bits) < p.owners)
+            p.owner_bits++;
+        // blocks of 2048 tokens, at most 256 of them
+        p.each = 2048 * dh_ceil_div(n, 2048 * 256);
+        p.blocks = dh_ceil_div(n, p.each);
+        p.counts_at = take((p.owners * p.blocks + 4) * sizeof(unsigned));
+        p.list_at = take(n * sizeof(unsigned long long));
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <typename T> size_t backward_workspace(size_t n, size_t vocab, size_t width) {
+    return vocab && width ? backward_plan(n, vocab, width).bytes : 0;
+}
+
+template <typename T, int VEC>
+static inline dh_status backward_sorted(dh_ctx *ctx, RowArgs<T> &r, SortArgs &a, const BackwardPlan &p, void *work) {
+    r.lanes = 1;
+    while (r.lanes < DH_WAVE && r.lanes < r.width_vecs)
+        r.lanes <<= 1;
+    const size_t slices = dh_ceil_div(r.width_vecs, r.lanes);
+    if (slices >= 65536)
+        return dh_fail(DH_ERR_RUNTIME, "embeddingBackward - extents exceed one launch");
+    unsigned char *w = static_cast<unsigned char *>(work);
+    r.row_starts = a.row_starts = reinterpret_cast<unsigned *>(w + p.starts_at);
+    r.sorted = a.sorted = reinterpret_cast<unsigned *>(w + p.sorted_at);
+    r.hot_rows = a.hot_rows = reinterpret_cast<HotRow *>(w + p.hot_rows_at);
+    r.hot_parts = a.hot_parts = reinterpret_cast<HotPart *>(w + p.hot_parts_at);
+    r.partials = reinterpret_cast<double *>(w + p.partials_at);
+    r.parts = p.parts;
+    a.parts = static_cast<unsigned>(p.parts);
+    a.hots = static_cast<unsigned>(p.hots);
+    a.rows_each = 1u << p.row_bits;
+    a.row_bits = p.row_bits;
+    if (p.how == BackwardPlan::PARTITION) {
+        unsigned *counts = reinterpret_cast<unsigned *>(w + p.counts_at);
+        unsigned long long *list = reinterpret_cast<unsigned long long *>(w + p.list_at);
+        a.starts = counts;
+        a.blocks = p.blocks;
+        a.list = list;
+        const dim3 blocks(static_cast<unsigned>(p.blocks));
+        hipLaunchKernelGGL(count_kernel, blocks, dim3(PART_THREADS), p.owners * sizeof(unsigned), ctx->stream, a.ids, a.ld_ids, a.n, p.each,
+                           static_cast<long long>(a.vocab), p.row_bits, p.owners, counts, a.rec);
+        hipLaunchKernelGGL(scan_counts_kernel, dim3(1), dim3(1024), 0, ctx->stream, counts, p.owners * p.blocks);
+        hipLaunchKernelGGL(scatter_kernel, blocks, dim3(PART_THREADS), PART_WAVES * p.owners * sizeof(unsigned), ctx->stream, a.ids, a.ld_ids,
+                           a.n, p.each, static_cast<long long>(a.vocab), p.row_bits, p.owner_bits, p.owners, counts, list);
+    }
+    const size_t lds = ((1 + SORT_WAVES) * a.rows_each + 1) * sizeof(unsigned);
+    auto *sort = p.how != BackwardPlan::SCAN ? &sort_kernel<0> : a.n <= 8 * SORT_THREADS ? &sort_kernel<8> : &sort_kernel<32>;
+    if (lds > 65536)
+        DH_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(sort), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(lds)));
+    hipLaunchKernelGGL(sort, dim3(static_cast<unsigned>(p.owners)), dim3(SORT_THREADS), lds, ctx->stream, a);
+    const size_t units = p.parts + dh_ceil_div(r.vocab, 4), grid = dh_ceil_div(units, THREADS / r.lanes);
+    const size_t most = dh_ceil_div(static_cast<size_t>(ctx->num_cus) * 32, slices);
+    hipLaunchKernelGGL((rows_kernel<T, VEC>), dim3(static_cast<unsigned>(grid < most ? grid : most), static_cast<unsigned>(slices)),
+                       dim3(THREADS), 0, ctx->stream, r);
+    if (p.hots)
+        hipLaunchKernelGGL((join_kernel<T, VEC>), dim3(static_cast<unsigned>(p.hots), static_cast<unsigned>(dh_ceil_div(r.width_vecs, DH_WAVE))),
+                           dim3(THREADS), 0, ctx->stream, r);
+    return DH_OK;
+}
 
 template <typename T>
 dh_status backward(dh_ctx *ctx, T *d_table, size_t vocab, size_t width, size_t ld, const T *d_out, size_t ld_out, const long long *ids,
@@ -155,6 +712,20 @@ dh_status backward(dh_ctx *ctx, T *d_table, size_t vocab, size_t width, size_t l
     void *work = nullptr;
     if (dh_status st = dh_call_workspace(ctx, "embeddingBackward", ws, ws_bytes, backward_workspace<T>(n, vocab, width), &work); st != DH_OK)
         return st;
+    const BackwardPlan p = backward_plan(n, vocab ? vocab : 1, width);
+    if (vocab > 0 && p.how != BackwardPlan::PLAIN) {
+        constexpr int V = dh_vec<T>::N;
+        const bool vec = width % V == 0 && ld % V == 0 && ld_out % V == 0 && dh_aligned(d_table, 16) && dh_aligned(d_out, 16);
+        SortArgs a{};
+        a.vocab = static_cast<unsigned>(vocab), a.ids = ids, a.ld_ids = ld_ids, a.n = n, a.rec = rec;
+        RowArgs<T> r{};
+        r.d_table = d_table, r.ld = ld, r.vocab = vocab, r.width_vecs = vec ? width / V : width;
+        r.d_out = d_out, r.ld_out = ld_out, r.scale = static_cast<double>(scale), r.accumulate = accumulate;
+        if (dh_status st = vec ? backward_sorted<T, V>(ctx, r, a, p, work) : backward_sorted<T, 1>(ctx, r, a, p, work); st != DH_OK)
+            return st;
+        DH_CHECK_LAUNCH();
+        return dh_checked_end(ctx);
+    }
     const size_t gy = dh_ceil_div(width, THREADS), gx = vocab ? vocab : 1;
     if (gx >= (size_t(1) << 31) || gy >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "embeddingBackward - extents exceed one launch");
