@@ -13,6 +13,8 @@
 
 #include "common.h"
 
+#include <type_traits>
+
 namespace dh_rms {
 
 constexpr int THREADS = 256;
@@ -200,23 +202,54 @@ template <typename T, int VEC, int TPR, int KV, bool Q8> static inline void laun
                        ctx->stream, a);
 }
 
-// The fewest threads a row whose registers hold it with up to four vectors each.
+// The shape of a row of so many vectors: calls use(TPR, KV) as integral constants. As few threads a row as hold it with up to
+// four 16-byte vectors each, or sixteen single values of rows that are not aligned; KV = 0 beyond that.
+template <int A, int B> struct Shape {
+    static constexpr int TPR = A, KV = B;
+};
+template <int VEC, class Use> static inline void by_width(size_t vecs, Use &&use) {
+    if constexpr (VEC > 1) {
+        if (vecs <= 64)
+            use(Shape<64, 1>{});
+        else if (vecs <= 128)
+            use(Shape<64, 2>{});
+        else if (vecs <= 256)
+            use(Shape<64, 4>{});
+        else if (vecs <= 512)
+            use(Shape<256, 2>{});
+        else if (vecs <= 768)
+            use(Shape<256, 3>{});
+        else if (vecs <= 1024)
+            use(Shape<256, 4>{});
+        else if (vecs <= 2048)
+            use(Shape<1024, 2>{});
+        else if (vecs <= 4096)
+            use(Shape<1024, 4>{});
+        else
+            use(Shape<1024, 0>{});
+    } else {
+        if (vecs <= 64)
+            use(Shape<64, 1>{});
+        else if (vecs <= 256)
+            use(Shape<64, 4>{});
+        else if (vecs <= 512)
+            use(Shape<64, 8>{});
+        else if (vecs <= 1024)
+            use(Shape<256, 4>{});
+        else if (vecs <= 2048)
+            use(Shape<256, 8>{});
+        else if (vecs <= 4096)
+            use(Shape<1024, 4>{});
+        else if (vecs <= 8192)
+            use(Shape<1024, 8>{});
+        else if (vecs <= 16384)
+            use(Shape<1024, 16>{});
+        else
+            use(Shape<1024, 0>{});
+    }
+}
 template <typename T, int VEC, bool Q8> static inline void forward_by_width(dh_ctx *ctx, const ForwardArgs<T> &a) {
-    const size_t vecs = a.cols / VEC;
-    if (vecs <= 64)
-        launch_forward<T, VEC, 64, 1, Q8>(ctx, a);
-    else if (vecs <= 128)
-        launch_forward<T, VEC, 64, 2, Q8>(ctx, a);
-    else if (vecs <= 256)
-        launch_forward<T, VEC, 64, 4, Q8>(ctx, a);
-    else if (vecs <= 512)
-        launch_forward<T, VEC, 256, 2, Q8>(ctx, a);
-    else if (vecs <= 1024)
-        launch_forward<T, VEC, 256, 4, Q8>(ctx, a);
-    else if (vecs <= 4096)
-        launch_forward<T, VEC, 1024, 4, Q8>(ctx, a);
-    else
-        launch_forward<T, VEC, 1024, 0, Q8>(ctx, a);
+    by_width<VEC>(a.cols / VEC, [&](auto shape) { launch_forward<T, VEC, decltype(shape)::TPR, decltype(shape)::KV, Q8>(ctx, a); });
 }
 
 template <typename T, bool Q8> dh_status forward(dh_ctx *ctx, const ForwardArgs<T> &a) {
@@ -264,43 +297,162 @@ template <typename T> struct BackwardArgs {
     size_t rows, cols;
 };
 
-// d_h, one row to a workgroup.
-template <typename T> __global__ __launch_bounds__(THREADS) void backward_rows_kernel(BackwardArgs<T> a) {
-    __shared__ double slots[THREADS / DH_WAVE];
+// Rows and d_gamma together: a workgroup goes through every gridDim.x-th row (four rows at a time where a wavefront holds one)
+// and keeps the sums of d_y h inv of its columns in registers, which it leaves in partials[blockIdx.x].
+template <typename T, int VEC, int TPR, int KV>
+__global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kernel(BackwardArgs<T> a, T *partials) {
+    constexpr int WG = TPR > THREADS ? TPR : THREADS, RPW = WG / TPR;
+    __shared__ double slots[WG / DH_WAVE];
+    __shared__ double cols_lds[RPW > 1 ? TPR * KV * VEC : 1];
+    const unsigned lane = threadIdx.x % TPR;
+    const size_t vecs = a.cols / VEC;
+    T g[KV][VEC];
+    double acc[KV][VEC] = {};
+#pragma unroll
+    for (int k = 0; k < KV; k++) {
+        const size_t j = lane + static_cast<size_t>(k) * TPR, at = (j < vecs ? j : vecs - 1) * VEC;
+        if (a.gamma)
+            dh_load_vec<T, VEC>(a.gamma + at, g[k]);
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                g[k][e] = T(1);
+    }
+    const double cols = static_cast<double>(a.cols);
+    for (size_t row = static_cast<size_t>(blockIdx.x) * RPW + threadIdx.x / TPR; row < a.rows; row += static_cast<size_t>(gridDim.x) * RPW) {
+        const T *ph = a.h + row * a.ld_h, *py = a.dy + row * a.ld_dy, *ps = a.dsum ? a.dsum + row * a.ld_ds : nullptr;
+        T h[KV][VEC], dy[KV][VEC], ds[KV][VEC];
+        const T inv = a.inv_rms[row];
+#pragma unroll
+        for (int k = 0; k < KV; k++) { // beyond the row: its last vector again, which counts for nothing
+            const size_t j = lane + static_cast<size_t>(k) * TPR, at = (j < vecs ? j : vecs - 1) * VEC;
+            dh_load_vec_stream<T, VEC>(ph + at, h[k]);
+            dh_load_vec_stream<T, VEC>(py + at, dy[k]);
+        }
+        if (ps)
+#pragma unroll
+            for (int k = 0; k < KV; k++) {
+                const size_t j = lane + static_cast<size_t>(k) * TPR, at = (j < vecs ? j : vecs - 1) * VEC;
+                dh_load_vec_stream<T, VEC>(ps + at, ds[k]);
+            }
+        double dot = 0.0;
+        const double dinv = static_cast<double>(inv);
+#pragma unroll
+        for (int k = 0; k < KV; k++) {
+            const bool live = lane + static_cast<size_t>(k) * TPR < vecs;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const double p = live ? static_cast<double>(dy[k][e]) * static_cast<double>(h[k][e]) : 0.0;
+                dot += p * static_cast<double>(g[k][e]);
+                acc[k][e] += p * dinv;
+            }
+        }
+        dot = over_row<TPR>(dot, slots, Add());
+        const T m = static_cast<T>(dot / cols * dinv * dinv);
+        T *dx = a.dx + row * a.ld_dx;
+#pragma unroll
+        for (int k = 0; k < KV; k++) {
+            const size_t j = lane + static_cast<size_t>(k) * TPR;
+            if (j >= vecs)
+                continue;
+            T v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                v[e] = inv * (dy[k][e] * g[k][e] - h[k][e] * m);
+                if (ps)
+                    v[e] += ds[k][e];
+            }
+            dh_store_vec<T, VEC>(dx + j * VEC, v);
+        }
+    }
+    if (partials == nullptr)
+        return;
+    T *out = partials + blockIdx.x * a.cols;
+    if constexpr (RPW > 1) { // the wavefronts' sums, in order
+        for (int w = 0; w < RPW; w++) {
+            __syncthreads();
+            if (threadIdx.x / TPR == static_cast<unsigned>(w))
+#pragma unroll
+                for (int k = 0; k < KV; k++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        double &c = cols_lds[(lane + k * TPR) * VEC + e];
+                        c = w == 0 ? acc[k][e] : c + acc[k][e];
+                    }
+        }
+        __syncthreads();
+        for (size_t c = threadIdx.x; c < a.cols; c += WG)
+            out[c] = static_cast<T>(cols_lds[c]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < KV; k++) {
+            const size_t j = lane + static_cast<size_t>(k) * TPR;
+            if (j < vecs)
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    out[j * VEC + e] = static_cast<T>(acc[k][e]);
+        }
+    }
+}
+
+// Rows too wide for registers, read a second time for the result.
+template <typename T> __global__ __launch_bounds__(1024) void backward_rows_kernel(BackwardArgs<T> a) {
+    __shared__ double slots[1024 / DH_WAVE];
     const size_t row = blockIdx.x;
     const T *h = a.h + row * a.ld_h, *dy = a.dy + row * a.ld_dy, *ds = a.dsum ? a.dsum + row * a.ld_ds : nullptr;
     T *dx = a.dx + row * a.ld_dx;
     const T inv = a.inv_rms[row];
     double dot = 0.0;
-    for (size_t c = threadIdx.x; c < a.cols; c += THREADS)
-        dot += static_cast<double>(dy[c]) * static_cast<double>(a.gamma ? a.gamma[c] : T(1)) * static_cast<double>(h[c]);
-    dot = over_row<THREADS>(dot, slots, Add());
-    const T k = static_cast<T>(dot / static_cast<double>(a.cols) * static_cast<double>(inv) * static_cast<double>(inv));
-    for (size_t c = threadIdx.x; c < a.cols; c += THREADS) {
+#pragma unroll 4
+    for (size_t c = threadIdx.x; c < a.cols; c += 1024)
+        dot += static_cast<double>(dy[c]) * static_cast<double>(h[c]) * static_cast<double>(a.gamma ? a.gamma[c] : T(1));
+    dot = over_row<1024>(dot, slots, Add());
+    const T m = static_cast<T>(dot / static_cast<double>(a.cols) * static_cast<double>(inv) * static_cast<double>(inv));
+#pragma unroll 4
+    for (size_t c = threadIdx.x; c < a.cols; c += 1024) {
         const T u = dy[c] * (a.gamma ? a.gamma[c] : T(1));
-        dx[c] = inv * (u - h[c] * k) + (ds ? ds[c] : T(0));
+        dx[c] = inv * (u - h[c] * m) + (ds ? ds[c] : T(0));
     }
 }
 
-// d_gamma, one thread a column and share of the rows; the shares are added in order.
-template <typename T> __global__ __launch_bounds__(THREADS) void gamma_kernel(BackwardArgs<T> a) {
-    __shared__ double part[THREADS / 32][32];
+// Their d_gamma: a column a thread, every gridDim.y-th row.
+template <typename T> __global__ __launch_bounds__(THREADS) void gamma_kernel(BackwardArgs<T> a, T *partials) {
+    const size_t c = static_cast<size_t>(blockIdx.x) * THREADS + threadIdx.x;
+    if (c >= a.cols)
+        return;
+    double s = 0.0;
+#pragma unroll 4
+    for (size_t r = blockIdx.y; r < a.rows; r += gridDim.y)
+        s += static_cast<double>(a.dy[r * a.ld_dy + c]) * static_cast<double>(a.h[r * a.ld_h + c]) * static_cast<double>(a.inv_rms[r]);
+    partials[blockIdx.y * a.cols + c] = static_cast<T>(s);
+}
+
+// The sum of `n` partials per column, in order: 32 columns a workgroup, 32 shares of the partials.
+template <typename T> __global__ __launch_bounds__(1024) void join_gamma_kernel(T *d_gamma, const T *partials, size_t n, size_t cols) {
+    __shared__ double part[32][33];
     const size_t c = static_cast<size_t>(blockIdx.x) * 32 + threadIdx.x % 32;
     const unsigned share = threadIdx.x / 32;
+    const size_t each = (n + 31) / 32, b = share * each < n ? share * each : n, e = b + each < n ? b + each : n;
     double s = 0.0;
-    if (c < a.cols)
-        for (size_t r = share; r < a.rows; r += THREADS / 32)
-            s += static_cast<double>(a.dy[r * a.ld_dy + c]) * static_cast<double>(a.h[r * a.ld_h + c]) * static_cast<double>(a.inv_rms[r]);
+    if (c < cols)
+#pragma unroll 8
+        for (size_t r = b; r < e; r++)
+            s += static_cast<double>(partials[r * cols + c]);
     part[share][threadIdx.x % 32] = s;
     __syncthreads();
-    if (share == 0 && c < a.cols) {
-        for (int k = 1; k < THREADS / 32; k++)
+    if (share == 0 && c < cols) {
+        for (int k = 1; k < 32; k++)
             s += part[k][threadIdx.x];
-        a.d_gamma[c] = static_cast<T>(s);
+        d_gamma[c] = static_cast<T>(s);
     }
 }
 
-template <typename T> size_t backward_workspace(size_t, size_t) { return 0; }
+// Workgroups, and with them partials, of a gradient: the same for every alignment.
+static inline size_t backward_groups(size_t rows, size_t cols) {
+    const size_t most = cols <= 4096 ? 1024 : 512;
+    return rows < most ? rows : most;
+}
+template <typename T> size_t backward_workspace(size_t rows, size_t cols) { return backward_groups(rows, cols) * cols * sizeof(T); }
 
 template <typename T> dh_status backward(dh_ctx *ctx, const BackwardArgs<T> &a, void *ws, size_t ws_bytes) {
     constexpr const char *what = "rmsNormBackward";
@@ -314,12 +466,36 @@ template <typename T> dh_status backward(dh_ctx *ctx, const BackwardArgs<T> &a, 
     if (a.cols == 0)
         return DH_OK;
     void *work = nullptr;
-    if (dh_status st = dh_call_workspace(ctx, what, ws, ws_bytes, backward_workspace<T>(a.rows, a.cols), &work); st != DH_OK)
+    if (dh_status st = dh_call_workspace(ctx, what, ws, ws_bytes, a.d_gamma ? backward_workspace<T>(a.rows, a.cols) : 0, &work); st != DH_OK)
         return st;
-    if (a.d_gamma) // before d_x, which may take the place of d_y
-        hipLaunchKernelGGL((gamma_kernel<T>), dim3(static_cast<unsigned>(dh_ceil_div(a.cols, 32))), dim3(THREADS), 0, ctx->stream, a);
-    if (a.rows)
-        hipLaunchKernelGGL((backward_rows_kernel<T>), dim3(static_cast<unsigned>(a.rows)), dim3(THREADS), 0, ctx->stream, a);
+    T *partials = a.d_gamma ? static_cast<T *>(work) : nullptr;
+    size_t groups = backward_groups(a.rows, a.cols);
+    constexpr int V = dh_vec<T>::N;
+    const bool vec = a.cols % V == 0 && a.ld_dx % V == 0 && a.ld_h % V == 0 && a.ld_dy % V == 0 && dh_aligned(a.dx, 16) && dh_aligned(a.h, 16) &&
+                     dh_aligned(a.dy, 16) && (!a.gamma || dh_aligned(a.gamma, 16)) && (!a.dsum || (a.ld_ds % V == 0 && dh_aligned(a.dsum, 16)));
+    if (a.rows) {
+        auto launch = [&](auto width, auto shape) {
+            constexpr int VEC = decltype(width)::value, TPR = decltype(shape)::TPR, KV = decltype(shape)::KV;
+            if constexpr (KV == 0) {
+                if (partials) // before d_x, which may take the place of d_y
+                    hipLaunchKernelGGL((gamma_kernel<T>), dim3(static_cast<unsigned>(dh_ceil_div(a.cols, THREADS)), static_cast<unsigned>(groups)),
+                                       dim3(THREADS), 0, ctx->stream, a, partials);
+                hipLaunchKernelGGL((backward_rows_kernel<T>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, ctx->stream, a);
+            } else {
+                constexpr int WG = TPR > THREADS ? TPR : THREADS;
+                const size_t fit = dh_ceil_div(a.rows, WG / TPR);
+                groups = fit < groups ? fit : groups;
+                hipLaunchKernelGGL((backward_kernel<T, VEC, TPR, KV>), dim3(static_cast<unsigned>(groups)), dim3(WG), 0, ctx->stream, a, partials);
+            }
+        };
+        if (vec)
+            by_width<V>(a.cols / V, [&](auto shape) { launch(std::integral_constant<int, V>{}, shape); });
+        else
+            by_width<1>(a.cols, [&](auto shape) { launch(std::integral_constant<int, 1>{}, shape); });
+    }
+    if (a.d_gamma)
+        hipLaunchKernelGGL((join_gamma_kernel<T>), dim3(static_cast<unsigned>(dh_ceil_div(a.cols, 32))), dim3(1024), 0, ctx->stream, a.d_gamma,
+                           partials, groups, a.cols);
     DH_CHECK_LAUNCH();
     return DH_OK;
 }
