@@ -3,37 +3,217 @@
 //
 //   res[i][o] = sum over groups g of scale[o][g] * sum over k in g of code[o][k] x[i][k]      (x = x_scale[i] * code, if 8 bits)
 //
-// Few rows of x read every weight once, half a byte each: bound by memory. Codes are two to a byte, row by row, the even
+// Few rows of x read every weight once, half a byte each: bound by memory, so every weight is read once for up to 16 rows of x and
+// the products go to the matrix cores, which leaves the ALUs to the decoding. Codes are two to a byte, row by row, the even
 // column in the low half.
 #include "common.h"
+
+#include <type_traits>
 
 namespace dh_q4 {
 
 constexpr int THREADS = 256;
 
-// One wavefront per result, a lane per byte of codes and step.
-template <typename X>
-__global__ __launch_bounds__(THREADS) void matvec_plain_kernel(float *res, size_t ld_res, const X *x, size_t rows, size_t cols, size_t ld_x,
-                                                               const float *x_scale, const unsigned char *codes, size_t outs, size_t ld_codes,
-                                                               const float *scales, size_t ld_scales, size_t group) {
-    const size_t o = static_cast<size_t>(blockIdx.x) * (THREADS / DH_WAVE) + threadIdx.x / DH_WAVE;
-    if (o >= outs)
-        return;
-    const size_t i = blockIdx.y;
-    const unsigned lane = threadIdx.x % DH_WAVE;
-    const unsigned char *w = codes + o * ld_codes;
-    const X *xi = x + i * ld_x;
-    float acc = 0.f;
-    for (size_t b = lane; 2 * b < cols; b += DH_WAVE) {
-        const int lo = static_cast<int>(static_cast<unsigned>(w[b]) << 28) >> 28, hi = static_cast<int>(static_cast<unsigned>(w[b]) << 24) >> 28;
-        float s = static_cast<float>(lo) * static_cast<float>(xi[2 * b]);
-        if (2 * b + 1 < cols)
-            s += static_cast<float>(hi) * static_cast<float>(xi[2 * b + 1]);
-        acc += s * scales[o * ld_scales + 2 * b / group]; // groups are whole pairs of columns
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(1))); // rows of codes may begin at any byte
+typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef u32x4 u32x4_lds __attribute__((may_alias)); // parts of x in LDS, written as words
+typedef unsigned u32_lds __attribute__((may_alias));
+
+// A wavefront's LDS instructions execute in order; this keeps the compiler from reordering them.
+__device__ __forceinline__ void lds_in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wavefront multiplies 16 rows of x with T tiles of 16 outputs, STEP columns at a time; the WAVES wavefronts of a workgroup
+// share its columns and add their results at the end, in order.
+constexpr int STEP = 128, WAVES = 8, AHEAD = 4;
+constexpr int PLANE = STEP * 2 + 16; // bytes of one row of one part of x in LDS; the odd 16 keep 16 rows off each other's banks
+
+template <typename X> struct Args {
+    float *res;
+    size_t ld_res;
+    const X *x;
+    size_t rows, cols, ld_x;
+    const float *x_scale;
+    const unsigned char *codes;
+    size_t outs, ld_codes;
+    const float *scales;
+    size_t ld_scales;
+    unsigned group; // columns
+};
+
+// 4 x 4 blocks of 16 lanes and registers, transposed: register d then holds what lane block d had in register (lane block).
+__device__ __forceinline__ void transpose4(u32x4 &c) {
+    const auto p = __builtin_amdgcn_permlane32_swap(c[0], c[2], false, false), q = __builtin_amdgcn_permlane32_swap(c[1], c[3], false, false);
+    const auto r = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false), t = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
+    c = u32x4{r[0], r[1], t[0], t[1]};
+}
+
+// 32 columns: a lane has 8 consecutive ones, the same for x (rows = lane % 16) and weights (outputs = lane % 16).
+// Floats: codes become code / 16 as bfloat16, exactly; x comes as three bfloat16 parts that add up to it exactly, so that every
+// product is exact and only the sums are rounded, in 32 bits.
+struct Floats {
+    using C = f32x4;
+    static constexpr float UNIT = 16.0f;
+    bf16x8 part[3];
+    __device__ __forceinline__ C times(unsigned w, C c) const {
+        unsigned v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float lo = __builtin_amdgcn_cvt_off_f32_i4(static_cast<int>(w >> (8 * k))); // bits 0..3, over 16
+            const float hi = __builtin_amdgcn_cvt_off_f32_i4(static_cast<int>(w >> (8 * k + 4)));
+            v[k] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060302);
+        }
+        const bf16x8 b = __builtin_bit_cast(bf16x8, u32x4{v[0], v[1], v[2], v[3]});
+#pragma unroll
+        for (int p = 2; p >= 0; p--) // the smallest part first
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[p], b, c, 0, 0, 0);
+        return c;
     }
-    dh_butterfly(DH_WAVE, [&](auto peer) { acc += peer(acc); });
-    if (lane == 0)
-        res[i * ld_res + o] = x_scale ? acc * x_scale[i] : acc;
+};
+// 8-bit rows: codes become 16 code as bytes, the even columns' in front; sums are whole numbers.
+struct Bytes {
+    using C = i32x4;
+    static constexpr float UNIT = 1.0f / 16.0f;
+    long a;
+    __device__ __forceinline__ C times(unsigned w, C c) const {
+        const unsigned even = (w << 4) & 0xf0f0f0f0u, odd = w & 0xf0f0f0f0u;
+        return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, static_cast<long>((static_cast<unsigned long>(odd) << 32) | even), c, 0, 0, 0);
+    }
+};
+
+// WHOLE: groups are whole steps, so that a step has one scale.
+template <typename X, int T, bool WHOLE> __global__ __launch_bounds__(WAVES *DH_WAVE) void matvec_kernel(Args<X> a) {
+    constexpr bool FLOATS = sizeof(X) == 4;
+    using Op = std::conditional_t<FLOATS, Floats, Bytes>;
+    using C = typename Op::C;
+    extern __shared__ __attribute__((aligned(16))) unsigned char q4_lds[];
+    const unsigned tid = threadIdx.x, lane = tid % DH_WAVE, wave = tid / DH_WAVE, col = lane % 16, kb = lane / 16;
+    const size_t o0 = static_cast<size_t>(blockIdx.x) * (16 * T), m0 = static_cast<size_t>(blockIdx.y) * 16;
+    const unsigned M = a.rows - m0 < 16 ? static_cast<unsigned>(a.rows - m0) : 16u;
+    const size_t whole = a.cols / 32 * 32, steps = (whole + STEP - 1) / STEP; // columns behind `whole` are added at the end
+    const size_t each = (steps + WAVES - 1) / WAVES;
+    const size_t s0 = wave * each < steps ? wave * each : steps, s1 = s0 + each < steps ? s0 + each : steps;
+    const unsigned m = col < M ? col : M - 1; // rows that do not exist: the last one again, whose results are dropped
+    const unsigned char *w[T];
+    const float *sc[T];
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        const size_t o = o0 + t * 16 + col < a.outs ? o0 + t * 16 + col : a.outs - 1;
+        w[t] = a.codes + o * a.ld_codes;
+        sc[t] = a.scales + o * a.ld_scales;
+    }
+    const X *x = a.x + m0 * a.ld_x;
+    unsigned char *mine = q4_lds + wave * (3 * M * PLANE); // floats: this wavefront's parts of x
+    float acc[T][4] = {};
+    for (size_t sb = s0; sb < s1; sb += AHEAD) {
+        u32x4 c[AHEAD][T];
+        float one[AHEAD][T];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const size_t s = sb + u < s1 ? sb + u : s1 - 1, k = s * STEP + kb * 32; // 32 codes a lane; behind the row: its beginning, not used
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                c[u][t] = *reinterpret_cast<const u32x4_any *>(w[t] + (k < whole ? k / 2 : 0));
+                if constexpr (WHOLE)
+                    one[u][t] = sc[t][s * STEP / a.group];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const size_t s = sb + u, k0 = s * STEP;
+            if (s >= s1)
+                break;
+            const int chunks = whole - k0 < STEP ? static_cast<int>(whole - k0) / 32 : STEP / 32;
+            if constexpr (FLOATS) { // x in three parts: the upper 16 bits, those of the rest, and what then is left (8 bits)
+                for (unsigned r = 0; r < M; r++) {
+                    const bool in = k0 + 2 * lane < whole;
+                    const f32x2_any v = *reinterpret_cast<const f32x2_any *>(x + r * a.ld_x + (in ? k0 + 2 * lane : 0));
+                    unsigned q[3][2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float rest = v[e];
+                        q[0][e] = __builtin_bit_cast(unsigned, rest);
+                        const float hi = __builtin_bit_cast(float, q[0][e] & 0xffff0000u);
+                        rest = rest == hi ? 0.0f : rest - hi; // an infinity has no rest
+                        q[1][e] = __builtin_bit_cast(unsigned, rest);
+                        q[2][e] = __builtin_bit_cast(unsigned, rest - __builtin_bit_cast(float, q[1][e] & 0xffff0000u));
+                    }
+#pragma unroll
+                    for (int p = 0; p < 3; p++)
+                        *reinterpret_cast<u32_lds *>(mine + (p * M + r) * PLANE + lane * 4) = __builtin_amdgcn_perm(q[p][1], q[p][0], 0x07060302);
+                }
+                lds_in_order();
+            }
+#pragma unroll
+            for (int t = 0; t < T; t++)
+                transpose4(c[u][t]);
+            C sum[T] = {};
+#pragma unroll
+            for (int d = 0; d < STEP / 32; d++) {
+                if (d >= chunks)
+                    break;
+                Op op;
+                if constexpr (FLOATS) {
+#pragma unroll
+                    for (int p = 0; p < 3; p++)
+                        op.part[p] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_lds *>(mine + (p * M + m) * PLANE + d * 64 + kb * 16));
+                } else {
+                    const u32x2_any v = *reinterpret_cast<const u32x2_any *>(x + m * a.ld_x + k0 + d * 32 + kb * 8);
+                    const unsigned even = __builtin_amdgcn_perm(v[1], v[0], 0x06040200), odd = __builtin_amdgcn_perm(v[1], v[0], 0x07050301);
+                    op.a = static_cast<long>((static_cast<unsigned long>(odd) << 32) | even);
+                }
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    sum[t] = op.times(c[u][t][d], sum[t]);
+                    if constexpr (!WHOLE) {
+                        const float scale = sc[t][(k0 + d * 32) / a.group];
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            acc[t][i] += scale * static_cast<float>(sum[t][i]);
+                        sum[t] = C{};
+                    }
+                }
+            }
+            if constexpr (WHOLE)
+#pragma unroll
+                for (int t = 0; t < T; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        acc[t][i] += one[u][t] * static_cast<float>(sum[t][i]);
+            if constexpr (FLOATS)
+                lds_in_order();
+        }
+    }
+    __syncthreads(); // the parts of x
+    float *red = reinterpret_cast<float *>(q4_lds);
+#pragma unroll
+    for (int t = 0; t < T; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            red[((wave * T + t) * 4 + i) * DH_WAVE + lane] = acc[t][i];
+    __syncthreads();
+    for (unsigned e = tid; e < T * 256; e += WAVES * DH_WAVE) {
+        const unsigned l = e % DH_WAVE, i = e / DH_WAVE % 4, t = e / 256, row = l / 16 * 4 + i;
+        const size_t o = o0 + t * 16 + l % 16;
+        if (row >= M || o >= a.outs)
+            continue;
+        float v = 0.0f;
+        for (int q = 0; q < WAVES; q++)
+            v += red[((q * T + t) * 4 + i) * DH_WAVE + l];
+        v *= Op::UNIT;
+        for (size_t k = whole; k < a.cols; k++) {
+            const int byte = a.codes[o * a.ld_codes + k / 2], code = k % 2 ? static_cast<int>(static_cast<unsigned>(byte) << 24) >> 28 : static_cast<int>(static_cast<unsigned>(byte) << 28) >> 28;
+            v += a.scales[o * a.ld_scales + k / a.group] * (static_cast<float>(code) * static_cast<float>(x[row * a.ld_x + k]));
+        }
+        a.res[(m0 + row) * a.ld_res + o] = FLOATS ? v : v * a.x_scale[m0 + row];
+    }
 }
 
 template <typename X>
@@ -47,14 +227,26 @@ dh_status matvec(dh_ctx *ctx, float *res, size_t ld_res, const X *x, size_t rows
     if (rows > 0 && outs > 0 &&
         (res == nullptr || (cols > 0 && (x == nullptr || codes == nullptr || scales == nullptr)) || (sizeof(X) == 1 && x_scale == nullptr)))
         return dh_fail(DH_ERR_RUNTIME, "%s - a matrix is null", what);
+    if (cols >= (size_t(1) << 31) || outs >= (size_t(1) << 31) || dh_ceil_div(rows, 16) >= 65536)
+        return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
     DH_REQUIRE_CTX(ctx);
     if (rows == 0 || outs == 0)
         return DH_OK;
-    const size_t gx = dh_ceil_div(outs, THREADS / DH_WAVE);
-    if (gx >= (size_t(1) << 31) || rows >= 65536)
-        return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
-    hipLaunchKernelGGL((matvec_plain_kernel<X>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(rows)), dim3(THREADS), 0, ctx->stream,
-                       res, ld_res, x, rows, cols, ld_x, x_scale, codes, outs, ld_codes, scales, ld_scales, group);
+    // a group wider than the matrix is the whole row
+    const Args<X> a{res, ld_res, x, rows, cols, ld_x, x_scale, codes, outs, ld_codes, scales, ld_scales,
+                    static_cast<unsigned>(group < (size_t(1) << 31) ? group : size_t(1) << 31)};
+    const bool two = dh_ceil_div(outs, 32) * dh_ceil_div(rows, 16) >= static_cast<size_t>(ctx->num_cus), whole = group % STEP == 0;
+    const int tiles = two ? 2 : 1;
+    size_t lds = sizeof(X) == 4 ? WAVES * 3 * (rows < 16 ? rows : 16) * PLANE : 0;
+    const size_t red = static_cast<size_t>(WAVES) * tiles * 256 * sizeof(float);
+    lds = lds > red ? lds : red;
+    auto *kernel = two ? (whole ? &matvec_kernel<X, 2, true> : &matvec_kernel<X, 2, false>)
+                       : (whole ? &matvec_kernel<X, 1, true> : &matvec_kernel<X, 1, false>);
+    if (lds > 65536)
+        DH_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(lds)));
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(dh_ceil_div(outs, 16 * tiles)), static_cast<unsigned>(dh_ceil_div(rows, 16))),
+                       dim3(WAVES * DH_WAVE), lds, ctx->stream, a);
     DH_CHECK_LAUNCH();
     return DH_OK;
 }
