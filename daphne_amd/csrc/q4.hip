@@ -15,6 +15,7 @@ namespace dh_q4 {
 constexpr int THREADS = 256;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(1))); // rows of codes may begin at any byte
 typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
@@ -45,7 +46,10 @@ template <typename X> struct Args {
     size_t outs, ld_codes;
     const float *scales;
     size_t ld_scales;
-    unsigned group; // columns
+    unsigned long group_magic; // 2^40 over the chunks of 32 columns in a group, rounded up
+    __device__ __forceinline__ unsigned group_of(unsigned chunk) const { // exact: both below 2^20
+        return static_cast<unsigned>((chunk * group_magic) >> 40);
+    }
 };
 
 // 4 x 4 blocks of 16 lanes and registers, transposed: register d then holds what lane block d had in register (lane block).
@@ -88,18 +92,20 @@ struct Bytes {
     }
 };
 
-// WHOLE: groups are whole steps, so that a step has one scale.
-template <typename X, int T, bool WHOLE> __global__ __launch_bounds__(WAVES *DH_WAVE) void matvec_kernel(Args<X> a) {
+// WHOLE: groups are whole steps, so that a step has one scale. MT: rows of x that are staged (floats), a power of two.
+template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WAVES *DH_WAVE) void matvec_kernel(Args<X> a) {
     constexpr bool FLOATS = sizeof(X) == 4;
+    constexpr int SCALES = WHOLE ? 1 : STEP / 32, CHUNKS = STEP / 32;
     using Op = std::conditional_t<FLOATS, Floats, Bytes>;
     using C = typename Op::C;
     extern __shared__ __attribute__((aligned(16))) unsigned char q4_lds[];
-    const unsigned tid = threadIdx.x, lane = tid % DH_WAVE, wave = tid / DH_WAVE, col = lane % 16, kb = lane / 16;
+    const unsigned tid = threadIdx.x, lane = tid % DH_WAVE, col = lane % 16, kb = lane / 16;
+    const unsigned wave = __builtin_amdgcn_readfirstlane(tid / DH_WAVE);
     const size_t o0 = static_cast<size_t>(blockIdx.x) * (16 * T), m0 = static_cast<size_t>(blockIdx.y) * 16;
     const unsigned M = a.rows - m0 < 16 ? static_cast<unsigned>(a.rows - m0) : 16u;
-    const size_t whole = a.cols / 32 * 32, steps = (whole + STEP - 1) / STEP; // columns behind `whole` are added at the end
-    const size_t each = (steps + WAVES - 1) / WAVES;
-    const size_t s0 = wave * each < steps ? wave * each : steps, s1 = s0 + each < steps ? s0 + each : steps;
+    const unsigned whole = static_cast<unsigned>(a.cols) / 32 * 32, steps = (whole + STEP - 1) / STEP; // columns behind `whole`: at the end
+    const unsigned each = (steps + WAVES - 1) / WAVES;
+    const unsigned s0 = wave * each < steps ? wave * each : steps, s1 = s0 + each < steps ? s0 + each : steps;
     const unsigned m = col < M ? col : M - 1; // rows that do not exist: the last one again, whose results are dropped
     const unsigned char *w[T];
     const float *sc[T];
@@ -110,35 +116,56 @@ template <typename X, int T, bool WHOLE> __global__ __launch_bounds__(WAVES *DH_
         sc[t] = a.scales + o * a.ld_scales;
     }
     const X *x = a.x + m0 * a.ld_x;
-    unsigned char *mine = q4_lds + wave * (3 * M * PLANE); // floats: this wavefront's parts of x
+    unsigned char *mine = q4_lds + wave * (3 * MT * PLANE); // floats: this wavefront's parts of x
     float acc[T][4] = {};
-    for (size_t sb = s0; sb < s1; sb += AHEAD) {
+    for (unsigned sb = s0; sb < s1; sb += AHEAD) {
         u32x4 c[AHEAD][T];
-        float one[AHEAD][T];
+        float one[AHEAD][T][SCALES];
+        u32x2 xq[FLOATS ? 1 : AHEAD][CHUNKS];
+        f32x2_any xf[FLOATS && MT == 1 ? AHEAD : 1];
+        // what AHEAD steps need is on its way before the first of them begins
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
-            const size_t s = sb + u < s1 ? sb + u : s1 - 1, k = s * STEP + kb * 32; // 32 codes a lane; behind the row: its beginning, not used
+            const unsigned s = sb + u < s1 ? sb + u : s1 - 1, k = s * STEP + kb * 32; // 32 codes a lane; behind the row: its beginning, not used
 #pragma unroll
             for (int t = 0; t < T; t++) {
                 c[u][t] = *reinterpret_cast<const u32x4_any *>(w[t] + (k < whole ? k / 2 : 0));
-                if constexpr (WHOLE)
-                    one[u][t] = sc[t][s * STEP / a.group];
+#pragma unroll
+                for (int d = 0; d < SCALES; d++) {
+                    const unsigned chunk = s * CHUNKS + d;
+                    one[u][t][d] = sc[t][a.group_of(chunk * 32 < whole ? chunk : 0)];
+                }
             }
+            if constexpr (!FLOATS)
+#pragma unroll
+                for (int d = 0; d < CHUNKS; d++) {
+                    const unsigned k8 = s * STEP + d * 32;
+                    xq[u][d] = *reinterpret_cast<const u32x2_any *>(x + m * a.ld_x + (k8 < whole ? k8 : 0) + kb * 8);
+                }
+            else if constexpr (MT == 1)
+                xf[u] = *reinterpret_cast<const f32x2_any *>(x + (s * STEP + 2 * lane < whole ? s * STEP + 2 * lane : 0));
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
-            const size_t s = sb + u, k0 = s * STEP;
+            const unsigned s = sb + u, k0 = s * STEP;
             if (s >= s1)
                 break;
-            const int chunks = whole - k0 < STEP ? static_cast<int>(whole - k0) / 32 : STEP / 32;
+            const int chunks = whole - k0 < STEP ? static_cast<int>(whole - k0) / 32 : CHUNKS;
             if constexpr (FLOATS) { // x in three parts: the upper 16 bits, those of the rest, and what then is left (8 bits)
-                for (unsigned r = 0; r < M; r++) {
-                    const bool in = k0 + 2 * lane < whole;
-                    const f32x2_any v = *reinterpret_cast<const f32x2_any *>(x + r * a.ld_x + (in ? k0 + 2 * lane : 0));
+                f32x2_any v[MT];
+                const unsigned k2 = k0 + 2 * lane < whole ? k0 + 2 * lane : 0;
+#pragma unroll
+                for (int r = 0; r < MT; r++)
+                    if constexpr (MT == 1)
+                        v[r] = xf[u];
+                    else
+                        v[r] = *reinterpret_cast<const f32x2_any *>(x + (static_cast<unsigned>(r) < M ? r : M - 1) * a.ld_x + k2);
+#pragma unroll
+                for (int r = 0; r < MT; r++) {
                     unsigned q[3][2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float rest = v[e];
+                        float rest = v[r][e];
                         q[0][e] = __builtin_bit_cast(unsigned, rest);
                         const float hi = __builtin_bit_cast(float, q[0][e] & 0xffff0000u);
                         rest = rest == hi ? 0.0f : rest - hi; // an infinity has no rest
@@ -147,7 +174,7 @@ template <typename X, int T, bool WHOLE> __global__ __launch_bounds__(WAVES *DH_
                     }
 #pragma unroll
                     for (int p = 0; p < 3; p++)
-                        *reinterpret_cast<u32_lds *>(mine + (p * M + r) * PLANE + lane * 4) = __builtin_amdgcn_perm(q[p][1], q[p][0], 0x07060302);
+                        *reinterpret_cast<u32_lds *>(mine + (p * MT + r) * PLANE + lane * 4) = __builtin_amdgcn_perm(q[p][1], q[p][0], 0x07060302);
                 }
                 lds_in_order();
             }
@@ -156,16 +183,17 @@ template <typename X, int T, bool WHOLE> __global__ __launch_bounds__(WAVES *DH_
                 transpose4(c[u][t]);
             C sum[T] = {};
 #pragma unroll
-            for (int d = 0; d < STEP / 32; d++) {
+            for (int d = 0; d < CHUNKS; d++) {
                 if (d >= chunks)
                     break;
                 Op op;
                 if constexpr (FLOATS) {
 #pragma unroll
                     for (int p = 0; p < 3; p++)
-                        op.part[p] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4_lds *>(mine + (p * M + m) * PLANE + d * 64 + kb * 16));
+                        op.part[p] = __builtin_bit_cast(
+                            bf16x8, *reinterpret_cast<const u32x4_lds *>(mine + (p * MT + (MT == 1 ? 0 : m)) * PLANE + d * 64 + kb * 16));
                 } else {
-                    const u32x2_any v = *reinterpret_cast<const u32x2_any *>(x + m * a.ld_x + k0 + d * 32 + kb * 8);
+                    const u32x2 v = xq[u][d];
                     const unsigned even = __builtin_amdgcn_perm(v[1], v[0], 0x06040200), odd = __builtin_amdgcn_perm(v[1], v[0], 0x07050301);
                     op.a = static_cast<long>((static_cast<unsigned long>(odd) << 32) | even);
                 }
@@ -173,10 +201,9 @@ template <typename X, int T, bool WHOLE> __global__ __launch_bounds__(WAVES *DH_
                 for (int t = 0; t < T; t++) {
                     sum[t] = op.times(c[u][t][d], sum[t]);
                     if constexpr (!WHOLE) {
-                        const float scale = sc[t][(k0 + d * 32) / a.group];
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            acc[t][i] += scale * static_cast<float>(sum[t][i]);
+                            acc[t][i] += one[u][t][d] * static_cast<float>(sum[t][i]);
                         sum[t] = C{};
                     }
                 }
@@ -186,7 +213,7 @@ template <typename X, int T, bool WHOLE> __global__ __launch_bounds__(WAVES *DH_
                 for (int t = 0; t < T; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        acc[t][i] += one[u][t] * static_cast<float>(sum[t][i]);
+                        acc[t][i] += one[u][t][0] * static_cast<float>(sum[t][i]);
             if constexpr (FLOATS)
                 lds_in_order();
         }
@@ -208,12 +235,39 @@ template <typename X, int T, bool WHOLE> __global__ __launch_bounds__(WAVES *DH_
         for (int q = 0; q < WAVES; q++)
             v += red[((q * T + t) * 4 + i) * DH_WAVE + l];
         v *= Op::UNIT;
-        for (size_t k = whole; k < a.cols; k++) {
+        for (unsigned k = whole; k < a.cols; k++) {
             const int byte = a.codes[o * a.ld_codes + k / 2], code = k % 2 ? static_cast<int>(static_cast<unsigned>(byte) << 24) >> 28 : static_cast<int>(static_cast<unsigned>(byte) << 28) >> 28;
-            v += a.scales[o * a.ld_scales + k / a.group] * (static_cast<float>(code) * static_cast<float>(x[row * a.ld_x + k]));
+            v += a.scales[o * a.ld_scales + a.group_of(k / 32)] * (static_cast<float>(code) * static_cast<float>(x[row * a.ld_x + k]));
         }
         a.res[(m0 + row) * a.ld_res + o] = FLOATS ? v : v * a.x_scale[m0 + row];
     }
+}
+
+template <typename X, int T, bool WHOLE, int MT> static inline dh_status launch_staged(dh_ctx *ctx, const Args<X> &a) {
+    size_t lds = sizeof(X) == 4 ? WAVES * 3 * MT * PLANE : 0;
+    const size_t red = static_cast<size_t>(WAVES) * T * 256 * sizeof(float);
+    lds = lds > red ? lds : red;
+    auto *kernel = &matvec_kernel<X, T, WHOLE, MT>;
+    if (lds > 65536)
+        DH_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(lds)));
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(dh_ceil_div(a.outs, 16 * T)), static_cast<unsigned>(dh_ceil_div(a.rows, 16))),
+                       dim3(WAVES * DH_WAVE), lds, ctx->stream, a);
+    DH_CHECK_LAUNCH();
+    return DH_OK;
+}
+template <typename X, int T, bool WHOLE> static inline dh_status launch(dh_ctx *ctx, const Args<X> &a) {
+    if constexpr (sizeof(X) == 4) {
+        if (a.rows == 1)
+            return launch_staged<X, T, WHOLE, 1>(ctx, a);
+        if (a.rows == 2)
+            return launch_staged<X, T, WHOLE, 2>(ctx, a);
+        if (a.rows <= 4)
+            return launch_staged<X, T, WHOLE, 4>(ctx, a);
+        if (a.rows <= 8)
+            return launch_staged<X, T, WHOLE, 8>(ctx, a);
+    }
+    return launch_staged<X, T, WHOLE, 16>(ctx, a);
 }
 
 template <typename X>
@@ -227,28 +281,18 @@ dh_status matvec(dh_ctx *ctx, float *res, size_t ld_res, const X *x, size_t rows
     if (rows > 0 && outs > 0 &&
         (res == nullptr || (cols > 0 && (x == nullptr || codes == nullptr || scales == nullptr)) || (sizeof(X) == 1 && x_scale == nullptr)))
         return dh_fail(DH_ERR_RUNTIME, "%s - a matrix is null", what);
-    if (cols >= (size_t(1) << 31) || outs >= (size_t(1) << 31) || dh_ceil_div(rows, 16) >= 65536)
+    if (cols >= (size_t(1) << 25) || outs >= (size_t(1) << 31) || dh_ceil_div(rows, 16) >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
     DH_REQUIRE_CTX(ctx);
     if (rows == 0 || outs == 0)
         return DH_OK;
-    // a group wider than the matrix is the whole row
+    const size_t per_group = group / 32 < (size_t(1) << 20) ? group / 32 : size_t(1) << 20; // wider than any matrix: one group
     const Args<X> a{res, ld_res, x, rows, cols, ld_x, x_scale, codes, outs, ld_codes, scales, ld_scales,
-                    static_cast<unsigned>(group < (size_t(1) << 31) ? group : size_t(1) << 31)};
+                    dh_ceil_div(size_t(1) << 40, per_group)};
     const bool two = dh_ceil_div(outs, 32) * dh_ceil_div(rows, 16) >= static_cast<size_t>(ctx->num_cus), whole = group % STEP == 0;
-    const int tiles = two ? 2 : 1;
-    size_t lds = sizeof(X) == 4 ? WAVES * 3 * (rows < 16 ? rows : 16) * PLANE : 0;
-    const size_t red = static_cast<size_t>(WAVES) * tiles * 256 * sizeof(float);
-    lds = lds > red ? lds : red;
-    auto *kernel = two ? (whole ? &matvec_kernel<X, 2, true> : &matvec_kernel<X, 2, false>)
-                       : (whole ? &matvec_kernel<X, 1, true> : &matvec_kernel<X, 1, false>);
-    if (lds > 65536)
-        DH_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(lds)));
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(dh_ceil_div(outs, 16 * tiles)), static_cast<unsigned>(dh_ceil_div(rows, 16))),
-                       dim3(WAVES * DH_WAVE), lds, ctx->stream, a);
-    DH_CHECK_LAUNCH();
-    return DH_OK;
+    if (two)
+        return whole ? launch<X, 2, true>(ctx, a) : launch<X, 2, false>(ctx, a);
+    return whole ? launch<X, 1, true>(ctx, a) : launch<X, 1, false>(ctx, a);
 }
 
 // One wavefront per group: its largest magnitude becomes 7, values are rounded to the nearest code (ties to even).

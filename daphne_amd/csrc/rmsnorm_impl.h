@@ -249,6 +249,14 @@ template <int VEC, class Use> static inline void by_width(size_t vecs, Use &&use
     }
 }
 template <typename T, int VEC, bool Q8> static inline void forward_by_width(dh_ctx *ctx, const ForwardArgs<T> &a) {
+    // few rows: more threads on each, since nothing else hides what a thread waits for
+    if (const size_t vecs = a.cols / VEC; a.rows < static_cast<size_t>(ctx->num_cus) && vecs > 256 && vecs <= 2048) {
+        if (vecs <= 1024)
+            launch_forward<T, VEC, 1024, 1, Q8>(ctx, a);
+        else
+            launch_forward<T, VEC, 1024, 2, Q8>(ctx, a);
+        return;
+    }
     by_width<VEC>(a.cols / VEC, [&](auto shape) { launch_forward<T, VEC, decltype(shape)::TPR, decltype(shape)::KV, Q8>(ctx, a); });
 }
 
