@@ -15,11 +15,11 @@ namespace dh_q4 {
 constexpr int THREADS = 256;
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(1))); // rows of codes may begin at any byte
-typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef f32x4 f32x4_lds __attribute__((may_alias));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4_lds __attribute__((may_alias)); // parts of x in LDS, written as words
@@ -34,7 +34,12 @@ __device__ __forceinline__ void lds_in_order() {
 // A wavefront multiplies 16 rows of x with T tiles of 16 outputs, STEP columns at a time; the WAVES wavefronts of a workgroup
 // share its columns and add their results at the end, in order.
 constexpr int STEP = 128, WAVES = 8, AHEAD = 4;
+constexpr int SCALE_ROW = AHEAD * STEP / 32 + 4; // floats of one output's scales in LDS
 constexpr int PLANE = STEP * 2 + 16; // bytes of one row of one part of x in LDS; the odd 16 keep 16 rows off each other's banks
+
+constexpr unsigned own_lds(bool floats, int tiles, int rows) { // bytes of a wavefront
+    return tiles * 16 * SCALE_ROW * 4 + (floats ? 3 * rows * PLANE : 0);
+}
 
 template <typename X> struct Args {
     float *res;
@@ -95,7 +100,7 @@ struct Bytes {
 // WHOLE: groups are whole steps, so that a step has one scale. MT: rows of x that are staged (floats), a power of two.
 template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WAVES *DH_WAVE) void matvec_kernel(Args<X> a) {
     constexpr bool FLOATS = sizeof(X) == 4;
-    constexpr int SCALES = WHOLE ? 1 : STEP / 32, CHUNKS = STEP / 32;
+    constexpr int CHUNKS = STEP / 32;
     using Op = std::conditional_t<FLOATS, Floats, Bytes>;
     using C = typename Op::C;
     extern __shared__ __attribute__((aligned(16))) unsigned char q4_lds[];
@@ -116,35 +121,43 @@ template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WA
         sc[t] = a.scales + o * a.ld_scales;
     }
     const X *x = a.x + m0 * a.ld_x;
-    unsigned char *mine = q4_lds + wave * (3 * MT * PLANE); // floats: this wavefront's parts of x
+    unsigned char *mine = q4_lds + wave * own_lds(FLOATS, T, MT); // this wavefront's scales, and parts of x
+    float *my_scales = reinterpret_cast<float *>(mine);
+    mine += T * 16 * SCALE_ROW * sizeof(float);
+    const unsigned groups = a.group_of(static_cast<unsigned>((a.cols + 31) / 32 - 1)) + 1;
     float acc[T][4] = {};
     for (unsigned sb = s0; sb < s1; sb += AHEAD) {
         u32x4 c[AHEAD][T];
-        float one[AHEAD][T][SCALES];
-        u32x2 xq[FLOATS ? 1 : AHEAD][CHUNKS];
+        f32x4 scale4[T];
+        u32x4 xq[FLOATS ? 1 : AHEAD][2];
         f32x2_any xf[FLOATS && MT == 1 ? AHEAD : 1];
-        // what AHEAD steps need is on its way before the first of them begins
+        // What AHEAD steps need is on its way before the first of them begins. Their scales: at most 16 of an output, four a lane.
+        const unsigned g0 = a.group_of(sb * CHUNKS), ga = g0 + kb * 4;
+#pragma unroll
+        for (int t = 0; t < T; t++)
+            if (ga + 4 <= groups)
+                scale4[t] = *reinterpret_cast<const f32x4_any *>(sc[t] + ga);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    scale4[t][e] = sc[t][ga + e < groups ? ga + e : groups - 1];
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             const unsigned s = sb + u < s1 ? sb + u : s1 - 1, k = s * STEP + kb * 32; // 32 codes a lane; behind the row: its beginning, not used
 #pragma unroll
-            for (int t = 0; t < T; t++) {
+            for (int t = 0; t < T; t++)
                 c[u][t] = *reinterpret_cast<const u32x4_any *>(w[t] + (k < whole ? k / 2 : 0));
-#pragma unroll
-                for (int d = 0; d < SCALES; d++) {
-                    const unsigned chunk = s * CHUNKS + d;
-                    one[u][t][d] = sc[t][a.group_of(chunk * 32 < whole ? chunk : 0)];
-                }
-            }
             if constexpr (!FLOATS)
 #pragma unroll
-                for (int d = 0; d < CHUNKS; d++) {
-                    const unsigned k8 = s * STEP + d * 32;
-                    xq[u][d] = *reinterpret_cast<const u32x2_any *>(x + m * a.ld_x + (k8 < whole ? k8 : 0) + kb * 8);
-                }
+                for (int h = 0; h < 2; h++)
+                    xq[u][h] = *reinterpret_cast<const u32x4_any *>(x + m * a.ld_x + (k < whole ? k : 0) + h * 16);
             else if constexpr (MT == 1)
                 xf[u] = *reinterpret_cast<const f32x2_any *>(x + (s * STEP + 2 * lane < whole ? s * STEP + 2 * lane : 0));
         }
+#pragma unroll
+        for (int t = 0; t < T; t++)
+            *reinterpret_cast<f32x4_lds *>(my_scales + (t * 16 + col) * SCALE_ROW + kb * 4) = scale4[t];
+        lds_in_order();
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             const unsigned s = sb + u, k0 = s * STEP;
@@ -181,6 +194,14 @@ template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WA
 #pragma unroll
             for (int t = 0; t < T; t++)
                 transpose4(c[u][t]);
+            u32x4 lo, hi; // 8-bit rows: the halves of a lane's four times 8 columns
+            if constexpr (!FLOATS) {
+                lo = u32x4{xq[u][0][0], xq[u][0][2], xq[u][1][0], xq[u][1][2]};
+                hi = u32x4{xq[u][0][1], xq[u][0][3], xq[u][1][1], xq[u][1][3]};
+                transpose4(lo);
+                transpose4(hi);
+            }
+            auto scale = [&](int t, int d) { return my_scales[(t * 16 + col) * SCALE_ROW + a.group_of(s * CHUNKS + d) - g0]; };
             C sum[T] = {};
 #pragma unroll
             for (int d = 0; d < CHUNKS; d++) {
@@ -193,29 +214,30 @@ template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WA
                         op.part[p] = __builtin_bit_cast(
                             bf16x8, *reinterpret_cast<const u32x4_lds *>(mine + (p * MT + (MT == 1 ? 0 : m)) * PLANE + d * 64 + kb * 16));
                 } else {
-                    const u32x2 v = xq[u][d];
-                    const unsigned even = __builtin_amdgcn_perm(v[1], v[0], 0x06040200), odd = __builtin_amdgcn_perm(v[1], v[0], 0x07050301);
+                    const unsigned even = __builtin_amdgcn_perm(hi[d], lo[d], 0x06040200), odd = __builtin_amdgcn_perm(hi[d], lo[d], 0x07050301);
                     op.a = static_cast<long>((static_cast<unsigned long>(odd) << 32) | even);
                 }
 #pragma unroll
                 for (int t = 0; t < T; t++) {
                     sum[t] = op.times(c[u][t][d], sum[t]);
                     if constexpr (!WHOLE) {
+                        const float one = scale(t, d);
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            acc[t][i] += one[u][t][d] * static_cast<float>(sum[t][i]);
+                            acc[t][i] += one * static_cast<float>(sum[t][i]);
                         sum[t] = C{};
                     }
                 }
             }
             if constexpr (WHOLE)
 #pragma unroll
-                for (int t = 0; t < T; t++)
+                for (int t = 0; t < T; t++) {
+                    const float one = scale(t, 0);
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        acc[t][i] += one[u][t][0] * static_cast<float>(sum[t][i]);
-            if constexpr (FLOATS)
-                lds_in_order();
+                        acc[t][i] += one * static_cast<float>(sum[t][i]);
+                }
+            lds_in_order();
         }
     }
     __syncthreads(); // the parts of x
@@ -244,7 +266,7 @@ template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WA
 }
 
 template <typename X, int T, bool WHOLE, int MT> static inline dh_status launch_staged(dh_ctx *ctx, const Args<X> &a) {
-    size_t lds = sizeof(X) == 4 ? WAVES * 3 * MT * PLANE : 0;
+    size_t lds = WAVES * own_lds(sizeof(X) == 4, T, MT);
     const size_t red = static_cast<size_t>(WAVES) * T * 256 * sizeof(float);
     lds = lds > red ? lds : red;
     auto *kernel = &matvec_kernel<X, T, WHOLE, MT>;
