@@ -11,7 +11,7 @@
 // 64 bits: the conversions hide behind the loads, and a row of any length keeps T's precision.
 #pragma once
 
-#include "common.h"
+#include "seq_common.h"
 
 #include <type_traits>
 
@@ -59,35 +59,39 @@ template <typename T> struct ForwardArgs {
     double eps;
 };
 
+typedef unsigned u32_any __attribute__((aligned(1)));
+
 // What follows the reductions, for one vector of a row.
 template <typename T, int VEC, bool Q8>
-__device__ __forceinline__ void write_vec(const ForwardArgs<T> &a, size_t row, size_t at, const T (&h)[VEC], const T (&g)[VEC], T inv,
+__device__ __forceinline__ void write_vec(const ForwardArgs<T> &a, size_t row, dh_seq::Piece at, const T (&h)[VEC], const T (&g)[VEC], T inv,
                                           double to_code) {
     if constexpr (Q8) {
-        signed char q[VEC];
+        signed char *p = a.codes + row * a.ld_res + at.at;
+        unsigned q[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; e++)
-            q[e] = static_cast<signed char>(static_cast<int>(rint(static_cast<double>(h[e]) * static_cast<double>(g[e]) * to_code)));
-        if constexpr (VEC == 4) {
-            *reinterpret_cast<unsigned *>(a.codes + row * a.ld_res + at) =
-                (static_cast<unsigned char>(q[0])) | (static_cast<unsigned>(static_cast<unsigned char>(q[1])) << 8) |
-                (static_cast<unsigned>(static_cast<unsigned char>(q[2])) << 16) | (static_cast<unsigned>(static_cast<unsigned char>(q[3])) << 24);
-        } else {
+            q[e] = static_cast<unsigned>(static_cast<int>(rint(static_cast<double>(h[e]) * static_cast<double>(g[e]) * to_code))) & 255u;
+        if constexpr (VEC == 4)
+            if (at.shift == 0) {
+                *reinterpret_cast<u32_any *>(p) = q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24);
+                return;
+            }
 #pragma unroll
-            for (int e = 0; e < VEC; e++)
-                a.codes[row * a.ld_res + at + e] = q[e];
-        }
+        for (int e = 0; e < VEC; e++)
+            if (static_cast<size_t>(e) >= at.shift)
+                p[e] = static_cast<signed char>(q[e]);
     } else {
         T y[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; e++)
             y[e] = h[e] * inv * g[e];
-        dh_store_vec<T, VEC>(a.res + row * a.ld_res + at, y);
+        dh_seq::store<T, VEC>(a.res + row * a.ld_res + at.at, y, at.shift);
     }
 }
 
 // KV vectors of VEC values a thread, TPR threads a row, max(TPR, THREADS) threads a workgroup. KV = 0: rows of any
 // length, read a second time for the result (from `sum` where there is one, since x may have been replaced by it).
+// Threads behind the last vector read it, too; a value counts for the vector that it belongs to.
 template <typename T, int VEC, int TPR, int KV, bool Q8>
 __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void forward_kernel(ForwardArgs<T> a) {
     constexpr int WG = TPR > THREADS ? TPR : THREADS, RPW = WG / TPR, K = KV ? KV : 1;
@@ -96,63 +100,65 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void forward_kerne
     const size_t row = static_cast<size_t>(blockIdx.x) * RPW + threadIdx.x / TPR;
     if (RPW > 1 && row >= a.rows) // whole wavefronts: a row of TPR = 64 meets no barrier
         return;
-    const size_t vecs = a.cols / VEC;
+    const size_t vecs = (a.cols + VEC - 1) / VEC;
     const T *x = a.x + row * a.ld_x, *r = a.residual ? a.residual + row * a.ld_r : nullptr;
     T *sum = a.sum ? a.sum + row * a.ld_sum : nullptr;
     double sq = 0.0, most = 0.0;
     T h[K][VEC], g[K][VEC];
+    auto gamma = [&](size_t at, T(&v)[VEC]) {
+        if (a.gamma)
+            dh_seq::load<T, VEC>(a.gamma + at, v);
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                v[e] = T(1);
+    };
+    auto reduce = [&](const T(&hv)[VEC], const T(&gv)[VEC], size_t shift) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const double v = static_cast<size_t>(e) >= shift ? static_cast<double>(hv[e]) : 0.0;
+            sq += v * v;
+            if constexpr (Q8)
+                most = Max()(most, static_cast<size_t>(e) >= shift ? fabs(v * static_cast<double>(gv[e])) : 0.0);
+        }
+    };
     if constexpr (KV != 0) {
         T b[K][VEC];
 #pragma unroll
-        for (int k = 0; k < KV; k++) { // beyond the row: its last vector again, which counts for nothing
-            const size_t j = lane + static_cast<size_t>(k) * TPR, at = (j < vecs ? j : vecs - 1) * VEC;
-            dh_load_vec<T, VEC>(x + at, h[k]);
+        for (int k = 0; k < KV; k++) {
+            const size_t at = dh_seq::piece<VEC>(lane + static_cast<size_t>(k) * TPR, a.cols).at;
+            dh_seq::load<T, VEC>(x + at, h[k]);
             if (r)
-                dh_load_vec<T, VEC>(r + at, b[k]);
-            if (a.gamma)
-                dh_load_vec<T, VEC>(a.gamma + at, g[k]);
-            else
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    g[k][e] = T(1);
+                dh_seq::load<T, VEC>(r + at, b[k]);
+            gamma(at, g[k]);
         }
 #pragma unroll
         for (int k = 0; k < KV; k++) {
-            const size_t j = lane + static_cast<size_t>(k) * TPR;
-            const bool live = j < vecs;
+            const dh_seq::Piece at = dh_seq::piece<VEC>(lane + static_cast<size_t>(k) * TPR, a.cols);
             if (r)
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
                     h[k][e] += b[k][e];
-            if (live && sum)
-                dh_store_vec<T, VEC>(sum + j * VEC, h[k]);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const double v = live ? static_cast<double>(h[k][e]) : 0.0;
-                sq += v * v;
-                if constexpr (Q8)
-                    most = Max()(most, live ? fabs(v * static_cast<double>(g[k][e])) : 0.0);
-            }
+            if (sum)
+                dh_seq::store<T, VEC>(sum + at.at, h[k], at.shift);
+            reduce(h[k], g[k], at.shift);
         }
     } else {
         for (size_t j = lane; j < vecs; j += TPR) {
-            dh_load_vec<T, VEC>(x + j * VEC, h[0]);
+            const dh_seq::Piece at = dh_seq::piece<VEC>(j, a.cols);
+            dh_seq::load<T, VEC>(x + at.at, h[0]);
             if (r) {
                 T b[VEC];
-                dh_load_vec<T, VEC>(r + j * VEC, b);
+                dh_seq::load<T, VEC>(r + at.at, b);
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
                     h[0][e] += b[e];
             }
             if (sum)
-                dh_store_vec<T, VEC>(sum + j * VEC, h[0]);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const double v = static_cast<double>(h[0][e]);
-                sq += v * v;
-                if constexpr (Q8)
-                    most = Max()(most, fabs(v * (a.gamma ? static_cast<double>(a.gamma[j * VEC + e]) : 1.0)));
-            }
+                dh_seq::store<T, VEC>(sum + at.at, h[0], at.shift);
+            if constexpr (Q8)
+                gamma(at.at, g[0]);
+            reduce(h[0], g[0], at.shift);
         }
     }
     sq = over_row<TPR>(sq, slots, Add());
@@ -176,22 +182,21 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void forward_kerne
     }
     if constexpr (KV != 0) {
 #pragma unroll
-        for (int k = 0; k < KV; k++) {
-            const size_t j = lane + static_cast<size_t>(k) * TPR;
-            if (j < vecs)
-                write_vec<T, VEC, Q8>(a, row, j * VEC, h[k], g[k], static_cast<T>(inv), to_code);
-        }
+        for (int k = 0; k < KV; k++)
+            write_vec<T, VEC, Q8>(a, row, dh_seq::piece<VEC>(lane + static_cast<size_t>(k) * TPR, a.cols), h[k], g[k], static_cast<T>(inv), to_code);
     } else {
         for (size_t j = lane; j < vecs; j += TPR) {
-            dh_load_vec<T, VEC>((sum ? sum : x) + j * VEC, h[0]);
-            if (r && !sum)
+            const dh_seq::Piece at = dh_seq::piece<VEC>(j, a.cols);
+            dh_seq::load<T, VEC>((sum ? sum : x) + at.at, h[0]);
+            if (r && !sum) {
+                T b[VEC];
+                dh_seq::load<T, VEC>(r + at.at, b);
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
-                    h[0][e] += r[j * VEC + e];
-#pragma unroll
-            for (int e = 0; e < VEC; e++)
-                g[0][e] = a.gamma ? a.gamma[j * VEC + e] : T(1);
-            write_vec<T, VEC, Q8>(a, row, j * VEC, h[0], g[0], static_cast<T>(inv), to_code);
+                    h[0][e] += b[e];
+            }
+            gamma(at.at, g[0]);
+            write_vec<T, VEC, Q8>(a, row, at, h[0], g[0], static_cast<T>(inv), to_code);
         }
     }
 }
@@ -203,61 +208,43 @@ template <typename T, int VEC, int TPR, int KV, bool Q8> static inline void laun
 }
 
 // The shape of a row of so many vectors: calls use(TPR, KV) as integral constants. As few threads a row as hold it with up to
-// four 16-byte vectors each, or sixteen single values of rows that are not aligned; KV = 0 beyond that.
+// four vectors each; KV = 0 beyond that.
 template <int A, int B> struct Shape {
     static constexpr int TPR = A, KV = B;
 };
 template <int VEC, class Use> static inline void by_width(size_t vecs, Use &&use) {
-    if constexpr (VEC > 1) {
-        if (vecs <= 64)
-            use(Shape<64, 1>{});
-        else if (vecs <= 128)
-            use(Shape<64, 2>{});
-        else if (vecs <= 256)
-            use(Shape<64, 4>{});
-        else if (vecs <= 512)
-            use(Shape<256, 2>{});
-        else if (vecs <= 768)
-            use(Shape<256, 3>{});
-        else if (vecs <= 1024)
-            use(Shape<256, 4>{});
-        else if (vecs <= 2048)
-            use(Shape<1024, 2>{});
-        else if (vecs <= 4096)
-            use(Shape<1024, 4>{});
-        else
-            use(Shape<1024, 0>{});
-    } else {
-        if (vecs <= 64)
-            use(Shape<64, 1>{});
-        else if (vecs <= 256)
-            use(Shape<64, 4>{});
-        else if (vecs <= 512)
-            use(Shape<64, 8>{});
-        else if (vecs <= 1024)
-            use(Shape<256, 4>{});
-        else if (vecs <= 2048)
-            use(Shape<256, 8>{});
-        else if (vecs <= 4096)
-            use(Shape<1024, 4>{});
-        else if (vecs <= 8192)
-            use(Shape<1024, 8>{});
-        else if (vecs <= 16384)
-            use(Shape<1024, 16>{});
-        else
-            use(Shape<1024, 0>{});
-    }
+    if constexpr (VEC == 1) // rows shorter than a vector
+        use(Shape<64, 1>{});
+    else if (vecs <= 64)
+        use(Shape<64, 1>{});
+    else if (vecs <= 128)
+        use(Shape<64, 2>{});
+    else if (vecs <= 256)
+        use(Shape<64, 4>{});
+    else if (vecs <= 512)
+        use(Shape<256, 2>{});
+    else if (vecs <= 768)
+        use(Shape<256, 3>{});
+    else if (vecs <= 1024)
+        use(Shape<256, 4>{});
+    else if (vecs <= 2048)
+        use(Shape<1024, 2>{});
+    else if (vecs <= 4096)
+        use(Shape<1024, 4>{});
+    else
+        use(Shape<1024, 0>{});
 }
 template <typename T, int VEC, bool Q8> static inline void forward_by_width(dh_ctx *ctx, const ForwardArgs<T> &a) {
     // few rows: more threads on each, since nothing else hides what a thread waits for
-    if (const size_t vecs = a.cols / VEC; a.rows < static_cast<size_t>(ctx->num_cus) && vecs > 256 && vecs <= 2048) {
+    const size_t vecs = dh_ceil_div(a.cols, VEC);
+    if (VEC > 1 && a.rows < static_cast<size_t>(ctx->num_cus) && vecs > 256 && vecs <= 2048) {
         if (vecs <= 1024)
             launch_forward<T, VEC, 1024, 1, Q8>(ctx, a);
         else
             launch_forward<T, VEC, 1024, 2, Q8>(ctx, a);
         return;
     }
-    by_width<VEC>(a.cols / VEC, [&](auto shape) { launch_forward<T, VEC, decltype(shape)::TPR, decltype(shape)::KV, Q8>(ctx, a); });
+    by_width<VEC>(vecs, [&](auto shape) { launch_forward<T, VEC, decltype(shape)::TPR, decltype(shape)::KV, Q8>(ctx, a); });
 }
 
 template <typename T, bool Q8> dh_status forward(dh_ctx *ctx, const ForwardArgs<T> &a) {
@@ -276,10 +263,7 @@ template <typename T, bool Q8> dh_status forward(dh_ctx *ctx, const ForwardArgs<
     if (a.rows == 0 || a.cols == 0)
         return DH_OK;
     constexpr int V = dh_vec<T>::N;
-    const bool vec = a.cols % V == 0 && a.ld_x % V == 0 && dh_aligned(a.x, 16) && (!a.sum || (a.ld_sum % V == 0 && dh_aligned(a.sum, 16))) &&
-                     (!a.residual || (a.ld_r % V == 0 && dh_aligned(a.residual, 16))) && (!a.gamma || dh_aligned(a.gamma, 16)) &&
-                     (Q8 ? a.ld_res % 4 == 0 && dh_aligned(a.codes, 4) : a.ld_res % V == 0 && dh_aligned(a.res, 16));
-    if (vec)
+    if (a.cols >= V)
         forward_by_width<T, V, Q8>(ctx, a);
     else
         forward_by_width<T, 1, Q8>(ctx, a);
@@ -313,14 +297,13 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kern
     __shared__ double slots[WG / DH_WAVE];
     __shared__ double cols_lds[RPW > 1 ? TPR * KV * VEC : 1];
     const unsigned lane = threadIdx.x % TPR;
-    const size_t vecs = a.cols / VEC;
+    auto place = [&](int k) { return dh_seq::piece<VEC>(lane + static_cast<size_t>(k) * TPR, a.cols); };
     T g[KV][VEC];
     double acc[KV][VEC] = {};
 #pragma unroll
     for (int k = 0; k < KV; k++) {
-        const size_t j = lane + static_cast<size_t>(k) * TPR, at = (j < vecs ? j : vecs - 1) * VEC;
         if (a.gamma)
-            dh_load_vec<T, VEC>(a.gamma + at, g[k]);
+            dh_seq::load<T, VEC>(a.gamma + place(k).at, g[k]);
         else
 #pragma unroll
             for (int e = 0; e < VEC; e++)
@@ -332,25 +315,23 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kern
         T h[KV][VEC], dy[KV][VEC], ds[KV][VEC];
         const T inv = a.inv_rms[row];
 #pragma unroll
-        for (int k = 0; k < KV; k++) { // beyond the row: its last vector again, which counts for nothing
-            const size_t j = lane + static_cast<size_t>(k) * TPR, at = (j < vecs ? j : vecs - 1) * VEC;
-            dh_load_vec_stream<T, VEC>(ph + at, h[k]);
-            dh_load_vec_stream<T, VEC>(py + at, dy[k]);
+        for (int k = 0; k < KV; k++) {
+            const size_t at = place(k).at;
+            dh_seq::load_stream<T, VEC>(ph + at, h[k]);
+            dh_seq::load_stream<T, VEC>(py + at, dy[k]);
         }
         if (ps)
 #pragma unroll
-            for (int k = 0; k < KV; k++) {
-                const size_t j = lane + static_cast<size_t>(k) * TPR, at = (j < vecs ? j : vecs - 1) * VEC;
-                dh_load_vec_stream<T, VEC>(ps + at, ds[k]);
-            }
+            for (int k = 0; k < KV; k++)
+                dh_seq::load_stream<T, VEC>(ps + place(k).at, ds[k]);
         double dot = 0.0;
         const double dinv = static_cast<double>(inv);
 #pragma unroll
         for (int k = 0; k < KV; k++) {
-            const bool live = lane + static_cast<size_t>(k) * TPR < vecs;
+            const size_t shift = place(k).shift;
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                const double p = live ? static_cast<double>(dy[k][e]) * static_cast<double>(h[k][e]) : 0.0;
+                const double p = static_cast<size_t>(e) >= shift ? static_cast<double>(dy[k][e]) * static_cast<double>(h[k][e]) : 0.0;
                 dot += p * static_cast<double>(g[k][e]);
                 acc[k][e] += p * dinv;
             }
@@ -360,9 +341,7 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kern
         T *dx = a.dx + row * a.ld_dx;
 #pragma unroll
         for (int k = 0; k < KV; k++) {
-            const size_t j = lane + static_cast<size_t>(k) * TPR;
-            if (j >= vecs)
-                continue;
+            const dh_seq::Piece at = place(k);
             T v[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
@@ -370,7 +349,7 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kern
                 if (ps)
                     v[e] += ds[k][e];
             }
-            dh_store_vec<T, VEC>(dx + j * VEC, v);
+            dh_seq::store<T, VEC>(dx + at.at, v, at.shift);
         }
     }
     if (partials == nullptr)
@@ -381,12 +360,15 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kern
             __syncthreads();
             if (threadIdx.x / TPR == static_cast<unsigned>(w))
 #pragma unroll
-                for (int k = 0; k < KV; k++)
+                for (int k = 0; k < KV; k++) {
+                    const dh_seq::Piece at = place(k);
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        double &c = cols_lds[(lane + k * TPR) * VEC + e];
-                        c = w == 0 ? acc[k][e] : c + acc[k][e];
-                    }
+                    for (int e = 0; e < VEC; e++)
+                        if (static_cast<size_t>(e) >= at.shift) {
+                            double &c = cols_lds[at.at + e];
+                            c = w == 0 ? acc[k][e] : c + acc[k][e];
+                        }
+                }
         }
         __syncthreads();
         for (size_t c = threadIdx.x; c < a.cols; c += WG)
@@ -394,32 +376,62 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kern
     } else {
 #pragma unroll
         for (int k = 0; k < KV; k++) {
-            const size_t j = lane + static_cast<size_t>(k) * TPR;
-            if (j < vecs)
+            const dh_seq::Piece at = place(k);
+            T v[VEC];
 #pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    out[j * VEC + e] = static_cast<T>(acc[k][e]);
+            for (int e = 0; e < VEC; e++)
+                v[e] = static_cast<T>(acc[k][e]);
+            dh_seq::store<T, VEC>(out + at.at, v, at.shift);
         }
     }
 }
 
 // Rows too wide for registers, read a second time for the result.
 template <typename T> __global__ __launch_bounds__(1024) void backward_rows_kernel(BackwardArgs<T> a) {
+    constexpr int VEC = dh_vec<T>::N;
     __shared__ double slots[1024 / DH_WAVE];
-    const size_t row = blockIdx.x;
+    const size_t row = blockIdx.x, vecs = (a.cols + VEC - 1) / VEC;
     const T *h = a.h + row * a.ld_h, *dy = a.dy + row * a.ld_dy, *ds = a.dsum ? a.dsum + row * a.ld_ds : nullptr;
     T *dx = a.dx + row * a.ld_dx;
     const T inv = a.inv_rms[row];
+    T hv[VEC], yv[VEC], gv[VEC], sv[VEC];
+    auto read = [&](size_t at) {
+        dh_seq::load<T, VEC>(h + at, hv);
+        dh_seq::load<T, VEC>(dy + at, yv);
+        if (a.gamma)
+            dh_seq::load<T, VEC>(a.gamma + at, gv);
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                gv[e] = T(1);
+    };
     double dot = 0.0;
 #pragma unroll 4
-    for (size_t c = threadIdx.x; c < a.cols; c += 1024)
-        dot += static_cast<double>(dy[c]) * static_cast<double>(h[c]) * static_cast<double>(a.gamma ? a.gamma[c] : T(1));
+    for (size_t j = threadIdx.x; j < vecs; j += 1024) {
+        const dh_seq::Piece at = dh_seq::piece<VEC>(j, a.cols);
+        read(at.at);
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            dot += static_cast<size_t>(e) >= at.shift ? static_cast<double>(yv[e]) * static_cast<double>(hv[e]) * static_cast<double>(gv[e]) : 0.0;
+    }
     dot = over_row<1024>(dot, slots, Add());
     const T m = static_cast<T>(dot / static_cast<double>(a.cols) * static_cast<double>(inv) * static_cast<double>(inv));
+    // A moved last vector shares values with the one before it, which may be written by then where dx takes an input's place:
+    // only values of its own are stored, and those nobody else writes.
 #pragma unroll 4
-    for (size_t c = threadIdx.x; c < a.cols; c += 1024) {
-        const T u = dy[c] * (a.gamma ? a.gamma[c] : T(1));
-        dx[c] = inv * (u - h[c] * m) + (ds ? ds[c] : T(0));
+    for (size_t j = threadIdx.x; j < vecs; j += 1024) {
+        const dh_seq::Piece at = dh_seq::piece<VEC>(j, a.cols);
+        read(at.at);
+        if (ds)
+            dh_seq::load<T, VEC>(ds + at.at, sv);
+        T v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            v[e] = inv * (yv[e] * gv[e] - hv[e] * m);
+            if (ds)
+                v[e] += sv[e];
+        }
+        dh_seq::store<T, VEC>(dx + at.at, v, at.shift);
     }
 }
 
@@ -479,8 +491,6 @@ template <typename T> dh_status backward(dh_ctx *ctx, const BackwardArgs<T> &a, 
     T *partials = a.d_gamma ? static_cast<T *>(work) : nullptr;
     size_t groups = backward_groups(a.rows, a.cols);
     constexpr int V = dh_vec<T>::N;
-    const bool vec = a.cols % V == 0 && a.ld_dx % V == 0 && a.ld_h % V == 0 && a.ld_dy % V == 0 && dh_aligned(a.dx, 16) && dh_aligned(a.h, 16) &&
-                     dh_aligned(a.dy, 16) && (!a.gamma || dh_aligned(a.gamma, 16)) && (!a.dsum || (a.ld_ds % V == 0 && dh_aligned(a.dsum, 16)));
     if (a.rows) {
         auto launch = [&](auto width, auto shape) {
             constexpr int VEC = decltype(width)::value, TPR = decltype(shape)::TPR, KV = decltype(shape)::KV;
@@ -496,8 +506,8 @@ template <typename T> dh_status backward(dh_ctx *ctx, const BackwardArgs<T> &a, 
                 hipLaunchKernelGGL((backward_kernel<T, VEC, TPR, KV>), dim3(static_cast<unsigned>(groups)), dim3(WG), 0, ctx->stream, a, partials);
             }
         };
-        if (vec)
-            by_width<V>(a.cols / V, [&](auto shape) { launch(std::integral_constant<int, V>{}, shape); });
+        if (a.cols >= V)
+            by_width<V>(dh_ceil_div(a.cols, V), [&](auto shape) { launch(std::integral_constant<int, V>{}, shape); });
         else
             by_width<1>(a.cols, [&](auto shape) { launch(std::integral_constant<int, 1>{}, shape); });
     }
