@@ -9,7 +9,7 @@
 // results do not depend on timing.
 #pragma once
 
-#include "common.h"
+#include "seq_common.h"
 
 #include <type_traits>
 
@@ -21,7 +21,7 @@ constexpr int THREADS = 256;
 // takes UN * LPR vectors of a row each.
 template <typename T, int VEC, int UN>
 __global__ __launch_bounds__(THREADS) void forward_kernel(T *res, size_t ld_res, const T *table, size_t ld_table, long long vocab,
-                                                          size_t width_vecs, const long long *ids, size_t ld_ids, size_t n, T scale,
+                                                          size_t width, const long long *ids, size_t ld_ids, size_t n, T scale,
                                                           unsigned lpr, int *rec) {
     const unsigned lane = threadIdx.x % lpr;
     const size_t row = static_cast<size_t>(blockIdx.x) * (THREADS / lpr) + threadIdx.x / lpr;
@@ -38,19 +38,15 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(T *res, size_t ld_res,
     T *dst = res + row * ld_res;
     T v[UN][VEC];
 #pragma unroll
-    for (int u = 0; u < UN; u++) {
-        const size_t j = v0 + static_cast<size_t>(u) * lpr;
-        dh_load_vec<T, VEC>(src + (j < width_vecs ? j : width_vecs - 1) * VEC, v[u]); // beyond the row: its last vector, never stored
-    }
+    for (int u = 0; u < UN; u++) // beyond the row: its last vector, never stored
+        dh_seq::load<T, VEC>(src + dh_seq::piece<VEC>(v0 + static_cast<size_t>(u) * lpr, width).at, v[u]);
 #pragma unroll
     for (int u = 0; u < UN; u++) {
-        const size_t j = v0 + static_cast<size_t>(u) * lpr;
-        if (j >= width_vecs)
-            break;
+        const dh_seq::Piece at = dh_seq::piece<VEC>(v0 + static_cast<size_t>(u) * lpr, width);
 #pragma unroll
         for (int e = 0; e < VEC; e++)
             v[u][e] *= scale;
-        dh_store_vec<T, VEC>(dst + j * VEC, v[u]);
+        dh_seq::store<T, VEC>(dst + at.at, v[u], at.shift);
     }
 }
 
@@ -68,8 +64,8 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, const T *table, size_t voc
     if (dh_status st = dh_checked_begin(ctx, "embeddingForward", &rec); st != DH_OK)
         return st;
     constexpr int V = dh_vec<T>::N;
-    const bool vec = width % V == 0 && ld_res % V == 0 && ld_table % V == 0 && dh_aligned(res, 16) && dh_aligned(table, 16);
-    const size_t wv = vec ? width / V : width;
+    const bool vec = width >= V;
+    const size_t wv = vec ? dh_ceil_div(width, V) : width;
     unsigned lpr = 1;
     while (lpr < THREADS && lpr < wv)
         lpr <<= 1;
@@ -81,7 +77,7 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, const T *table, size_t voc
     const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
 #define DH_EMBED_FORWARD(VEC, UN)                                                                                                          \
     hipLaunchKernelGGL((forward_kernel<T, VEC, UN>), grid, dim3(THREADS), 0, ctx->stream, res, ld_res, table, ld_table,                   \
-                       static_cast<long long>(vocab), wv, ids, ld_ids, n, scale, lpr, rec)
+                       static_cast<long long>(vocab), width, ids, ld_ids, n, scale, lpr, rec)
     if (vec && four)
         DH_EMBED_FORWARD(V, 4);
     else if (vec)
@@ -356,7 +352,7 @@ template <int HELD> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(
 template <typename T> struct RowArgs {
     T *d_table;
     size_t ld;
-    size_t vocab, width_vecs;
+    size_t vocab, width, width_vecs;
     const T *d_out;
     size_t ld_out;
     double scale;
@@ -377,7 +373,7 @@ __device__ __forceinline__ void add_rows(double (&acc)[VEC], const T *d_out, siz
         T v[N][VEC];
 #pragma unroll
         for (int u = 0; u < N; u++)
-            dh_load_vec_stream<T, VEC>(d_out + static_cast<size_t>(position(k + u < end ? k + u : end - 1)) * ld_out, v[u]);
+            dh_seq::load_stream<T, VEC>(d_out + static_cast<size_t>(position(k + u < end ? k + u : end - 1)) * ld_out, v[u]);
 #pragma unroll
         for (int u = 0; u < N; u++)
             if (k + u < end)
@@ -394,16 +390,17 @@ __device__ __forceinline__ void add_rows(double (&acc)[VEC], const T *d_out, siz
         round(std::integral_constant<int, 1>{}, k);
 }
 
-template <typename T, int VEC> __device__ __forceinline__ void write_row(const RowArgs<T> &a, size_t row, size_t vec, const double (&acc)[VEC]) {
-    T *p = a.d_table + row * a.ld + vec * VEC, v[VEC];
+template <typename T, int VEC>
+__device__ __forceinline__ void write_row(const RowArgs<T> &a, size_t row, dh_seq::Piece at, const double (&acc)[VEC]) {
+    T *p = a.d_table + row * a.ld + at.at, v[VEC];
     if (a.accumulate)
-        dh_load_vec<T, VEC>(p, v);
+        dh_seq::load<T, VEC>(p, v);
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
         const double s = acc[e] * a.scale;
         v[e] = static_cast<T>(a.accumulate ? s + static_cast<double>(v[e]) : s);
     }
-    dh_store_vec_stream<T, VEC>(p, v);
+    dh_seq::store<T, VEC, true>(p, v, at.shift);
 }
 
 // A group of `lanes` lanes takes blockIdx.y's slice of a part, or of AT_ONCE consecutive rows; the parts come first, since they
@@ -415,7 +412,8 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
     if (vec >= a.width_vecs)
         return;
     const size_t units = a.parts + (a.vocab + AT_ONCE - 1) / AT_ONCE;
-    const T *column = a.d_out + vec * VEC;
+    const dh_seq::Piece piece = dh_seq::piece<VEC>(vec, a.width);
+    const T *column = a.d_out + piece.at;
     auto position = [&](size_t k) { return a.sorted[k]; };
     for (size_t u = static_cast<size_t>(blockIdx.x) * each + threadIdx.x / a.lanes; u < units; u += static_cast<size_t>(gridDim.x) * each) {
         if (u < a.parts) {
@@ -425,7 +423,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
             double acc[VEC] = {};
             add_rows<T, VEC>(acc, column, a.ld_out, p.begin, p.end, position);
             if (p.whole)
-                write_row<T, VEC>(a, p.row, vec, acc);
+                write_row<T, VEC>(a, p.row, piece, acc);
             else
 #pragma unroll
                 for (int q = 0; q < VEC; q++)
@@ -446,7 +444,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++)
                 if (at[k + 1] != at[k])
-                    dh_load_vec_stream<T, VEC>(column + static_cast<size_t>(a.sorted[at[k]]) * a.ld_out, v[k]);
+                    dh_seq::load_stream<T, VEC>(column + static_cast<size_t>(a.sorted[at[k]]) * a.ld_out, v[k]);
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++) {
                 const bool some = at[k + 1] != at[k];
@@ -456,7 +454,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
 #pragma unroll
                 for (int q = 0; q < VEC; q++)
                     acc[q] = some ? static_cast<double>(v[k][q]) : 0.0;
-                write_row<T, VEC>(a, row + k, vec, acc);
+                write_row<T, VEC>(a, row + k, piece, acc);
             }
         } else {
             for (int k = 0; k < AT_ONCE; k++) {
@@ -465,7 +463,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
                     continue;
                 double acc[VEC] = {};
                 add_rows<T, VEC>(acc, column, a.ld_out, b, e, position);
-                write_row<T, VEC>(a, row + k, vec, acc);
+                write_row<T, VEC>(a, row + k, piece, acc);
             }
         }
     }
@@ -496,7 +494,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void join_k
 #pragma unroll
         for (int q = 0; q < VEC; q++)
             acc[q] += part[w][lane * VEC + q];
-    write_row<T, VEC>(a, h.row, vec, acc);
+    write_row<T, VEC>(a, h.row, dh_seq::piece<VEC>(vec, a.width), acc);
 }
 
 // Stable partition of the tokens by owner: how many each block of tokens has for each owner, owner by owner.
@@ -630,7 +628,7 @@ static inline BackwardPlan backward_plan(size_t n, size_t vocab, size_t width) {
     p.sorted_at = take(n * sizeof(unsigned));
     p.hot_rows_at = take(p.hots * sizeof(HotRow));
     p.hot_parts_at = take(p.parts * sizeof(HotPart));
-    p.partials_at = take(p.hots ? p.parts * width * sizeof(double) : 0);
+    p.partials_at = take(p.hots ? p.parts * (width + 3) * sizeof(double) : 0);
     if (p.how == BackwardPlan::PARTITION) {
         while ((size_t(1) << p.owner_bits) < p.owners)
             p.owner_bits++;
@@ -715,11 +713,11 @@ dh_status backward(dh_ctx *ctx, T *d_table, size_t vocab, size_t width, size_t l
     const BackwardPlan p = backward_plan(n, vocab ? vocab : 1, width);
     if (vocab > 0 && p.how != BackwardPlan::PLAIN) {
         constexpr int V = dh_vec<T>::N;
-        const bool vec = width % V == 0 && ld % V == 0 && ld_out % V == 0 && dh_aligned(d_table, 16) && dh_aligned(d_out, 16);
+        const bool vec = width >= V;
         SortArgs a{};
         a.vocab = static_cast<unsigned>(vocab), a.ids = ids, a.ld_ids = ld_ids, a.n = n, a.rec = rec;
         RowArgs<T> r{};
-        r.d_table = d_table, r.ld = ld, r.vocab = vocab, r.width_vecs = vec ? width / V : width;
+        r.d_table = d_table, r.ld = ld, r.vocab = vocab, r.width = width, r.width_vecs = vec ? dh_ceil_div(width, V) : width;
         r.d_out = d_out, r.ld_out = ld_out, r.scale = static_cast<double>(scale), r.accumulate = accumulate;
         if (dh_status st = vec ? backward_sorted<T, V>(ctx, r, a, p, work) : backward_sorted<T, 1>(ctx, r, a, p, work); st != DH_OK)
             return st;

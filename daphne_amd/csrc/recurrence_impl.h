@@ -16,7 +16,7 @@
 // predecessors' until it meets a carry that is already whole, publishes its own, and writes its rows.
 #pragma once
 
-#include "common.h"
+#include "seq_common.h"
 
 #include <type_traits>
 
@@ -194,9 +194,10 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
         ticket = ticket_lds;
     }
     const size_t chunk = ticket / a.blocks, block = ticket % a.blocks;
-    const size_t c0 = block * CW + lc * VEC;
-    const bool on = c0 < a.channels; // vectors are whole: channels is a multiple of VEC
-    const size_t cc = on ? c0 : 0;
+    const size_t c0 = block * CW + lc * VEC; // as the workspace counts channels; vectors behind the last one read it and write nothing
+    const dh_seq::Piece piece = dh_seq::piece<VEC>(block * LC + lc, a.channels);
+    const size_t cc = piece.at, shift = piece.shift;
+    const bool on = shift < VEC;
     const size_t first_i = chunk * ROWS, my_i = first_i + static_cast<size_t>(g) * R;
     // scanning order number -> row; numbers past the last one read the last one and count for nothing
     auto row_of = [&](size_t i) -> size_t {
@@ -209,15 +210,15 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
 #pragma unroll
     for (int k = 0; k < R; k++) {
         const size_t row = row_of(my_i + k);
-        dh_load_vec_stream<T, VEC>(a.z + row * a.ld_z + cc, va[k]);
-        dh_load_vec_stream<T, VEC>(BACK ? a.d_out + row * a.ld_do + cc : a.x + row * a.ld_x + cc, vb[k]);
+        dh_seq::load_stream<T, VEC>(a.z + row * a.ld_z + cc, va[k]);
+        dh_seq::load_stream<T, VEC>(BACK ? a.d_out + row * a.ld_do + cc : a.x + row * a.ld_x + cc, vb[k]);
     }
     if constexpr (BACK)
 #pragma unroll
         for (int k = 0; k < R; k++) {
             const size_t row = row_of(my_i + k);
-            dh_load_vec_stream<T, VEC>(a.x + row * a.ld_x + cc, xv[k]);
-            dh_load_vec_stream<T, VEC>(a.h + (row ? row - 1 : 0) * a.ld_h + cc, hv[k]);
+            dh_seq::load_stream<T, VEC>(a.x + row * a.ld_x + cc, xv[k]);
+            dh_seq::load_stream<T, VEC>(a.h + (row ? row - 1 : 0) * a.ld_h + cc, hv[k]);
         }
     // which sequence each row belongs to
     bool plain = true; // rows that are all live and neither first nor last: most chunks of long sequences
@@ -261,9 +262,9 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
                     const T *src = BACK ? a.d_last : a.h0;
                     T *dst = BACK ? a.d_h0 : a.last;
                     if (src)
-                        dh_load_vec<T, VEC>(src + s * (BACK ? a.ld_dl : a.ld_h0) + c0, v);
+                        dh_seq::load<T, VEC>(src + s * (BACK ? a.ld_dl : a.ld_h0) + cc, v);
                     if (dst)
-                        dh_store_vec<T, VEC>(dst + s * (BACK ? a.ld_dh0 : a.ld_last) + c0, v);
+                        dh_seq::store<T, VEC>(dst + s * (BACK ? a.ld_dh0 : a.ld_last) + cc, v, shift);
                 }
     }
     plain = __syncthreads_and(plain);
@@ -286,11 +287,11 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
                 const size_t s = seq_of[g * R + k];
                 const T *src = BACK ? a.d_last : a.h0;
                 if ((fl & OPENS) && src)
-                    dh_load_vec<T, VEC>(src + s * (BACK ? a.ld_dl : a.ld_h0) + cc, given);
+                    dh_seq::load<T, VEC>(src + s * (BACK ? a.ld_dl : a.ld_h0) + cc, given);
                 if constexpr (BACK)
                     if (fl & ROW_FIRST) {
                         if (a.h0)
-                            dh_load_vec<T, VEC>(a.h0 + s * a.ld_h0 + cc, hv[k]);
+                            dh_seq::load<T, VEC>(a.h0 + s * a.ld_h0 + cc, hv[k]);
                         else
 #pragma unroll
                             for (int e = 0; e < VEC; e++)
@@ -505,20 +506,20 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
                     v[e] = (fl & OPENS) ? vb[k][e] : va[k][e] * v[e] + vb[k][e];
                 }
                 if (fl & ROW_LIVE) {
-                    dh_store_vec_stream<T, VEC>(a.d_x + row * a.ld_dx + c0, gx);
-                    dh_store_vec_stream<T, VEC>(a.d_z + row * a.ld_dz + c0, gz);
+                    dh_seq::store<T, VEC, true>(a.d_x + row * a.ld_dx + cc, gx, shift);
+                    dh_seq::store<T, VEC, true>(a.d_z + row * a.ld_dz + cc, gz, shift);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
                     v[e] = (fl & OPENS) ? vb[k][e] : va[k][e] * v[e] + vb[k][e];
                 if (fl & ROW_LIVE)
-                    dh_store_vec_stream<T, VEC>(a.res + row * a.ld_res + c0, v);
+                    dh_seq::store<T, VEC, true>(a.res + row * a.ld_res + cc, v, shift);
             }
             if constexpr (!SIMPLE) {
                 T *out = BACK ? a.d_h0 : a.last;
                 if ((fl & CLOSES) && out)
-                    dh_store_vec<T, VEC>(out + static_cast<size_t>(seq_of[g * R + k]) * (BACK ? a.ld_dh0 : a.ld_last) + c0, v);
+                    dh_seq::store<T, VEC>(out + static_cast<size_t>(seq_of[g * R + k]) * (BACK ? a.ld_dh0 : a.ld_last) + cc, v, shift);
             }
         }
     };
@@ -550,16 +551,16 @@ static inline dh_status check_sequences(const char *what, const long long *offse
 // Sequences short enough for a thread to walk: below this many rows each, all of one length.
 constexpr size_t SERIAL_ROWS = 8;
 
-// Shape of a pass: vectors or single values, row chunks and channel blocks. Chunks are cut as tall as the registers allow,
+// Shape of a pass: vectors (single values if there is not even one vector of channels), row chunks and channel blocks. Chunks are cut as tall as the registers allow,
 // and a quarter of that where so few workgroups would leave compute units idle.
 struct Plan {
     int vec, lanes, rows;
     size_t blocks, chunks, padded;
 };
-template <typename T> Plan plan(size_t tokens, size_t channels, bool vec, bool back) {
+template <typename T> Plan plan(size_t tokens, size_t channels, bool back) {
     Plan p;
-    p.vec = vec ? dh_vec<T>::N : 1;
-    p.lanes = vec ? LANES : 64;
+    p.vec = channels >= static_cast<size_t>(dh_vec<T>::N) ? dh_vec<T>::N : 1;
+    p.lanes = LANES;
     p.blocks = dh_ceil_div(channels, static_cast<size_t>(p.lanes) * p.vec);
     p.padded = p.blocks * p.lanes * p.vec;
     const int tall = back ? ROWS_BACKWARD : ROWS_FORWARD;
@@ -572,18 +573,13 @@ template <typename T> size_t plan_bytes(const Plan &p) {
     return p.chunks > 1 ? 256 + p.chunks * 3 * Words<T>::N * p.padded * sizeof(unsigned long long) : 0;
 }
 
-// Enough for every alignment and direction.
+// Enough for both directions.
 template <typename T> size_t workspace(size_t tokens, size_t num_seq, size_t channels) {
     (void)num_seq;
-    size_t most = 0;
-    if (tokens && channels)
-        for (int k = 0; k < 4; k++) {
-            if ((k & 1) && channels % dh_vec<T>::N)
-                continue;
-            const size_t b = plan_bytes<T>(plan<T>(tokens, channels, k & 1, k & 2));
-            most = b > most ? b : most;
-        }
-    return most;
+    if (tokens == 0 || channels == 0)
+        return 0;
+    const size_t f = plan_bytes<T>(plan<T>(tokens, channels, false)), b = plan_bytes<T>(plan<T>(tokens, channels, true));
+    return f > b ? f : b;
 }
 
 template <typename T, int VEC, int LC, int R, bool BACK> static inline void launch_scan(dh_ctx *ctx, const ScanArgs<T> &a) {
@@ -613,15 +609,11 @@ dh_status scan(dh_ctx *ctx, const char *what, ScanArgs<T> &a, const Plan &p, voi
     else if (p.vec > 1)
         launch_scan<T, V, LANES, R / 4, BACK>(ctx, a);
     else if (p.rows == R)
-        launch_scan<T, 1, 64, R, BACK>(ctx, a);
+        launch_scan<T, 1, LANES, R, BACK>(ctx, a);
     else
-        launch_scan<T, 1, 64, R / 4, BACK>(ctx, a);
+        launch_scan<T, 1, LANES, R / 4, BACK>(ctx, a);
     DH_CHECK_LAUNCH();
     return DH_OK;
-}
-
-template <typename T> static inline bool whole_vectors(const T *p, size_t ld) {
-    return p == nullptr || (ld % dh_vec<T>::N == 0 && dh_aligned(p, 16));
 }
 
 template <typename T>
@@ -652,13 +644,11 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, T *last, size_t ld_last, c
         DH_CHECK_LAUNCH();
         return offsets ? dh_checked_end(ctx) : DH_OK;
     }
-    const bool vec = channels % dh_vec<T>::N == 0 && whole_vectors(x, ld_x) && whole_vectors(z, ld_z) && whole_vectors(h0, ld_h0) &&
-                     whole_vectors(res, ld_res) && whole_vectors(last, ld_last);
     ScanArgs<T> a{};
     a.x = x, a.ld_x = ld_x, a.z = z, a.ld_z = ld_z, a.h0 = h0, a.ld_h0 = ld_h0;
     a.res = res, a.ld_res = ld_res, a.last = last, a.ld_last = ld_last;
     a.sp = sp, a.num_seq = num_seq, a.channels = channels, a.tokens = tokens, a.rec = rec;
-    if (dh_status st = scan<T, false>(ctx, what, a, plan<T>(tokens, channels, vec, false), ws, ws_bytes); st != DH_OK)
+    if (dh_status st = scan<T, false>(ctx, what, a, plan<T>(tokens, channels, false), ws, ws_bytes); st != DH_OK)
         return st;
     return offsets ? dh_checked_end(ctx) : DH_OK;
 }
@@ -694,15 +684,12 @@ dh_status backward(dh_ctx *ctx, T *d_x, size_t ld_dx, T *d_z, size_t ld_dz, T *d
         DH_CHECK_LAUNCH();
         return offsets ? dh_checked_end(ctx) : DH_OK;
     }
-    const bool vec = channels % dh_vec<T>::N == 0 && whole_vectors(x, ld_x) && whole_vectors(z, ld_z) && whole_vectors(h, ld_h) &&
-                     whole_vectors(h0, ld_h0) && whole_vectors(d_out, ld_do) && whole_vectors(d_last, ld_dl) &&
-                     whole_vectors<T>(d_x, ld_dx) && whole_vectors<T>(d_z, ld_dz) && whole_vectors<T>(d_h0, ld_dh0);
     ScanArgs<T> a{};
     a.x = x, a.ld_x = ld_x, a.z = z, a.ld_z = ld_z, a.h0 = h0, a.ld_h0 = ld_h0, a.h = h, a.ld_h = ld_h;
     a.d_out = d_out, a.ld_do = ld_do, a.d_last = d_last, a.ld_dl = ld_dl;
     a.d_x = d_x, a.ld_dx = ld_dx, a.d_z = d_z, a.ld_dz = ld_dz, a.d_h0 = d_h0, a.ld_dh0 = ld_dh0;
     a.sp = sp, a.num_seq = num_seq, a.channels = channels, a.tokens = tokens, a.rec = rec;
-    if (dh_status st = scan<T, true>(ctx, what, a, plan<T>(tokens, channels, vec, true), ws, ws_bytes); st != DH_OK)
+    if (dh_status st = scan<T, true>(ctx, what, a, plan<T>(tokens, channels, true), ws, ws_bytes); st != DH_OK)
         return st;
     return offsets ? dh_checked_end(ctx) : DH_OK;
 }
