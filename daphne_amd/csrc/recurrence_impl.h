@@ -169,11 +169,19 @@ template <typename T> struct ScanArgs {
     int *rec;
 };
 
+template <typename T, int VEC, bool LINES> __device__ __forceinline__ void read_rows(const T *p, T (&v)[VEC]) {
+    if constexpr (LINES)
+        dh_seq::load_stream<T, VEC>(p, v);
+    else
+        dh_seq::load<T, VEC>(p, v);
+}
+
 constexpr int ROW_LIVE = 1, ROW_FIRST = 2, ROW_LAST = 4;
 
 // A workgroup takes LC lanes x VEC channels and LC lanes share a row; its THREADS / LC row groups take R rows each. BACK: rows in
-// reverse; the number i of a row counts in scanning order.
-template <typename T, int VEC, int LC, int R, bool BACK>
+// reverse; the number i of a row counts in scanning order. LINES: all rows begin at whole memory lines, so that no line is
+// touched by two workgroups and none needs to stay in a cache.
+template <typename T, int VEC, int LC, int R, bool BACK, bool LINES>
 __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
     constexpr int RG = THREADS / LC, ROWS = RG * R, CW = LC * VEC, NW = Words<T>::N, WAVES = THREADS / DH_WAVE;
     constexpr int LB = RG < 16 ? RG : 16; // predecessors looked at in one round
@@ -210,15 +218,15 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
 #pragma unroll
     for (int k = 0; k < R; k++) {
         const size_t row = row_of(my_i + k);
-        dh_seq::load_stream<T, VEC>(a.z + row * a.ld_z + cc, va[k]);
-        dh_seq::load_stream<T, VEC>(BACK ? a.d_out + row * a.ld_do + cc : a.x + row * a.ld_x + cc, vb[k]);
+        read_rows<T, VEC, LINES>(a.z + row * a.ld_z + cc, va[k]);
+        read_rows<T, VEC, LINES>(BACK ? a.d_out + row * a.ld_do + cc : a.x + row * a.ld_x + cc, vb[k]);
     }
     if constexpr (BACK)
 #pragma unroll
         for (int k = 0; k < R; k++) {
             const size_t row = row_of(my_i + k);
-            dh_seq::load_stream<T, VEC>(a.x + row * a.ld_x + cc, xv[k]);
-            dh_seq::load_stream<T, VEC>(a.h + (row ? row - 1 : 0) * a.ld_h + cc, hv[k]);
+            read_rows<T, VEC, LINES>(a.x + row * a.ld_x + cc, xv[k]);
+            read_rows<T, VEC, LINES>(a.h + (row ? row - 1 : 0) * a.ld_h + cc, hv[k]);
         }
     // which sequence each row belongs to
     bool plain = true; // rows that are all live and neither first nor last: most chunks of long sequences
@@ -506,15 +514,15 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
                     v[e] = (fl & OPENS) ? vb[k][e] : va[k][e] * v[e] + vb[k][e];
                 }
                 if (fl & ROW_LIVE) {
-                    dh_seq::store<T, VEC, true>(a.d_x + row * a.ld_dx + cc, gx, shift);
-                    dh_seq::store<T, VEC, true>(a.d_z + row * a.ld_dz + cc, gz, shift);
+                    dh_seq::store<T, VEC, LINES>(a.d_x + row * a.ld_dx + cc, gx, shift);
+                    dh_seq::store<T, VEC, LINES>(a.d_z + row * a.ld_dz + cc, gz, shift);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
                     v[e] = (fl & OPENS) ? vb[k][e] : va[k][e] * v[e] + vb[k][e];
                 if (fl & ROW_LIVE)
-                    dh_seq::store<T, VEC, true>(a.res + row * a.ld_res + cc, v, shift);
+                    dh_seq::store<T, VEC, LINES>(a.res + row * a.ld_res + cc, v, shift);
             }
             if constexpr (!SIMPLE) {
                 T *out = BACK ? a.d_h0 : a.last;
@@ -536,6 +544,8 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
 //   8 rows a thread forward (4 backward, which holds twice as many arrays): 167 registers, 3 wavefronts a SIMD. 16 (8) rows leave
 //   one: 195 and 193 us; 4 rows forward 238 us.
 // Without any look-back (sequences as long as a chunk) the same rows take 147 and 157 us, a plain copy of as many bytes 155.
+// Rows that do not begin at memory lines (2047 and 1023 channels) have every line in two chunks: 237 and 250 us by way of the
+// caches, 315 and 308 past them.
 constexpr int ROWS_FORWARD = 8, ROWS_BACKWARD = 4, LANES = 8;
 
 // What every entry point checks of its sequences.
@@ -582,9 +592,11 @@ template <typename T> size_t workspace(size_t tokens, size_t num_seq, size_t cha
     return f > b ? f : b;
 }
 
-template <typename T, int VEC, int LC, int R, bool BACK> static inline void launch_scan(dh_ctx *ctx, const ScanArgs<T> &a) {
-    hipLaunchKernelGGL((scan_kernel<T, VEC, LC, R, BACK>), dim3(static_cast<unsigned>(a.blocks * a.chunks)), dim3(THREADS), 0, ctx->stream, a);
+template <typename T, int VEC, int R, bool BACK, bool LINES> static inline void launch_scan(dh_ctx *ctx, const ScanArgs<T> &a) {
+    hipLaunchKernelGGL((scan_kernel<T, VEC, LANES, R, BACK, LINES>), dim3(static_cast<unsigned>(a.blocks * a.chunks)), dim3(THREADS), 0,
+                       ctx->stream, a);
 }
+template <typename T> static inline bool at_lines(const T *p, size_t ld) { return ld * sizeof(T) % 128 == 0 && dh_aligned(p, 128); }
 
 template <typename T, bool BACK>
 dh_status scan(dh_ctx *ctx, const char *what, ScanArgs<T> &a, const Plan &p, void *ws, size_t ws_bytes) {
@@ -604,14 +616,17 @@ dh_status scan(dh_ctx *ctx, const char *what, ScanArgs<T> &a, const Plan &p, voi
                            static_cast<ulonglong2 *>(work), n);
     }
     constexpr int V = dh_vec<T>::N, R = BACK ? ROWS_BACKWARD : ROWS_FORWARD;
+    const bool lines = at_lines(a.x, a.ld_x) && at_lines(a.z, a.ld_z) &&
+                       (BACK ? at_lines(a.h, a.ld_h) && at_lines(a.d_out, a.ld_do) && at_lines(a.d_x, a.ld_dx) && at_lines(a.d_z, a.ld_dz)
+                             : at_lines(a.res, a.ld_res));
     if (p.vec > 1 && p.rows == R)
-        launch_scan<T, V, LANES, R, BACK>(ctx, a);
+        lines ? launch_scan<T, V, R, BACK, true>(ctx, a) : launch_scan<T, V, R, BACK, false>(ctx, a);
     else if (p.vec > 1)
-        launch_scan<T, V, LANES, R / 4, BACK>(ctx, a);
+        launch_scan<T, V, R / 4, BACK, false>(ctx, a);
     else if (p.rows == R)
-        launch_scan<T, 1, LANES, R, BACK>(ctx, a);
+        launch_scan<T, 1, R, BACK, false>(ctx, a);
     else
-        launch_scan<T, 1, LANES, R / 4, BACK>(ctx, a);
+        launch_scan<T, 1, R / 4, BACK, false>(ctx, a);
     DH_CHECK_LAUNCH();
     return DH_OK;
 }
