@@ -138,10 +138,12 @@ __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size
 // ---------------------------------------------------------------------------------------
 // backward by sorted tokens
 // ---------------------------------------------------------------------------------------
-// sort_kernel puts the positions of all tokens in the order of their rows (stable: positions stay in order) and notes where each
-// row's begin. A workgroup owns VR consecutive rows and finds their positions by reading all tokens: 16 wavefronts go through
-// a share each, once to count and once to place. Beyond SCAN_TOKENS that reading would cost too much: the tokens are first split
-// into lists, one per owner, by a stable partition (count, scan, scatter).
+// sort_kernel puts the positions of all tokens in the order of owner and row (stable: positions stay in order) and notes where each
+// row's begin and end. An owner is a workgroup that has every `owners`-th row of the table, so that the frequent tokens, whose
+// numbers often lie together, are spread over all of them. It finds its positions by reading all tokens: 16 wavefronts go through a
+// share each (32768 tokens: 28 us, as much as by way of the partition, 65536: 35 against 27).
+// Beyond SCAN_TOKENS that reading would cost too much: the tokens are first split into lists, one per owner, by a stable
+// partition (count, scan, scatter).
 // rows_kernel then writes every row, zeros where there is nothing to add: 64 lanes of 16 bytes (fewer where rows are shorter)
 // per row and step. A token that occurs more than HOT times would keep its lanes busy long after all others: its positions are
 // taken in parts of PART; a token of one part is finished there, the parts of others are added in order by join_kernel.
@@ -150,10 +152,11 @@ __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size
 // the same way the slots [b / PART, e / PART) for its tokens of several parts. It marks those that it does not use.
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / DH_WAVE;
 constexpr unsigned HOT = 8, PART = 32;
-constexpr size_t SCAN_TOKENS = 32 * SORT_THREADS; // up to here every owner reads all tokens
-constexpr int ROW_BITS = 8;             // an owner has 1 << ROW_BITS rows, more in large tables
-constexpr size_t OWNERS = 4096;         // most owners
-constexpr size_t MOST_ROWS = 2048;      // most rows of an owner
+constexpr size_t SCAN_TOKENS = 32768;   // up to here every owner reads all tokens
+constexpr unsigned KEEP = 4096;                   // positions an owner keeps in LDS
+constexpr int OWNER_BITS = 8;                     // 1 << OWNER_BITS owners, more for large tables
+constexpr int MOST_OWNER_BITS = 12;
+constexpr size_t MOST_ROWS = 2048;                // most rows of an owner
 constexpr size_t PART_THREADS = 256, PART_WAVES = PART_THREADS / DH_WAVE;
 
 struct HotPart { // positions [begin, end) of `sorted`; end = 0: none
@@ -184,16 +187,35 @@ __device__ __forceinline__ unsigned next_place(unsigned *counter, bool in, unsig
     return __shfl(base, in ? static_cast<int>(__ffsll(static_cast<long long>(same))) - 1 : 0, DH_WAVE) + rank;
 }
 
+// The same where few lanes have a key, and few of them differ: one round per key.
+__device__ __forceinline__ unsigned next_place_of_few(unsigned *counter, bool in, unsigned key) {
+    const unsigned lane = threadIdx.x % DH_WAVE;
+    unsigned at = 0;
+    for (unsigned long long left = __ballot(in); left != 0;) {
+        const int first = static_cast<int>(__ffsll(static_cast<long long>(left))) - 1;
+        const unsigned k = __builtin_amdgcn_readlane(key, first);
+        const unsigned long long same = __ballot(in && key == k);
+        unsigned base = 0;
+        if (lane == static_cast<unsigned>(first))
+            base = atomicAdd(&counter[k], static_cast<unsigned>(__popcll(same)));
+        base = __builtin_amdgcn_readlane(base, first);
+        if (in && key == k)
+            at = base + __popcll(same & ((1ull << lane) - 1));
+        left &= ~same;
+    }
+    return at;
+}
+
 struct SortArgs {
     unsigned vocab;
     const long long *ids;
     size_t ld_ids, n;
-    unsigned rows_each; // a power of two
-    int row_bits;
+    unsigned rows_each;       // at most: an owner's rows are blockIdx.x + r * owners
+    int row_bits, owner_bits; // of a row within its owner, and of an owner
     const unsigned *starts; // partition: first place of owner b's list at starts[b * blocks], behind the last one the end
     size_t blocks;
     const unsigned long long *list; // row within the owner's << 32 | position
-    unsigned *row_starts;           // [vocab + 1]
+    uint2 *spans;                   // [vocab]: the row's first position in `sorted` and the one behind its last
     unsigned *sorted;
     HotRow *hot_rows;
     HotPart *hot_parts;
@@ -201,60 +223,72 @@ struct SortArgs {
     int *rec;
 };
 
-// HELD: owners read all tokens, a wavefront HELD times 64 of them at most, which stay in registers between counting and
-// placing. HELD = 0: owners read their lists, once for each.
-template <int HELD> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(SortArgs a) {
-    constexpr bool SCAN = HELD != 0;
+// SCAN: owners read all tokens. Otherwise: their lists. Twice, to count and to place, eight steps of 64 requested together.
+template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(SortArgs a) {
     extern __shared__ unsigned sort_lds[];
     const unsigned VR = a.rows_each, tid = threadIdx.x, wave = tid / DH_WAVE, lane = tid % DH_WAVE;
     unsigned *seg = sort_lds;     // [VR + 1]
     unsigned *cnt = seg + VR + 1; // [SORT_WAVES][VR]
     unsigned *mine = cnt + wave * VR;
     __shared__ unsigned front;    // SCAN: positions of all rows before this owner's
-    const unsigned row0 = blockIdx.x * VR, rows = a.vocab - row0 < VR ? a.vocab - row0 : VR;
+    __shared__ unsigned keep[KEEP]; // SCAN: what is placed goes out together (each store by itself would hold up the loads behind it)
+    const unsigned owner = blockIdx.x, mask = (1u << a.owner_bits) - 1;
+    const unsigned rows = a.vocab > owner ? (a.vocab - owner - 1) / (mask + 1) + 1 : 0;
+    auto number = [&](unsigned r) { return owner + (r << a.owner_bits); };
     const size_t begin = SCAN ? 0 : a.starts[blockIdx.x * a.blocks], end = SCAN ? a.n : a.starts[(blockIdx.x + 1) * a.blocks];
-    const size_t share = (end - begin + SORT_THREADS - 1) / SORT_THREADS * DH_WAVE; // what a wavefront goes through, in order
+    // What a wavefront goes through, in order. Shares that are whole multiples of 4 KiB would have all wavefronts of all owners at the
+    // same few channels of the cache at a time (32768 tokens: 40 us).
+    size_t share = (end - begin + SORT_THREADS - 1) / SORT_THREADS * DH_WAVE;
+    share += share % 512 == 0 ? DH_WAVE : 0;
     const size_t w0 = begin + wave * share < end ? begin + wave * share : end, w1 = w0 + share < end ? w0 + share : end;
-    unsigned row[SCAN ? HELD : 1], rank[SCAN ? HELD : 1];
+    constexpr int EIGHT = 8;
+    auto walk = [&](auto &&take) { // take(row or ~0, position, whether there is one, token)
+        for (size_t i0 = w0; i0 < w1; i0 += EIGHT * DH_WAVE) {
+            long long v[EIGHT];
+#pragma unroll
+            for (int u = 0; u < EIGHT; u++) { // behind the share: its last, not used (a guard would make each load wait for the one before)
+                const size_t i = i0 + u * DH_WAVE + lane, at = i < w1 ? i : w1 - 1;
+                v[u] = SCAN ? a.ids[at * a.ld_ids] : static_cast<long long>(a.list[at]);
+            }
+#pragma unroll
+            for (int u = 0; u < EIGHT; u++) {
+                const size_t i = i0 + u * DH_WAVE + lane;
+                const bool here = i < w1;
+                if constexpr (SCAN) {
+                    const bool valid = here && v[u] >= 0 && v[u] < static_cast<long long>(a.vocab);
+                    const unsigned id = static_cast<unsigned>(v[u]);
+                    take(valid && (id & mask) == owner ? id >> a.owner_bits : ~0u, static_cast<unsigned>(i), here && !valid,
+                         valid && (id & mask) < owner);
+                } else {
+                    take(here ? static_cast<unsigned>(static_cast<unsigned long long>(v[u]) >> 32) : ~0u, static_cast<unsigned>(v[u]), false, false);
+                }
+            }
+        }
+    };
+    for (unsigned i = tid; i < VR * SORT_WAVES; i += SORT_THREADS)
+        cnt[i] = 0;
+    if (tid == 0)
+        front = 0;
+    __syncthreads();
+    unsigned lower = 0;
+    bool bad = false;
+    walk([&](unsigned r, unsigned, bool wrong, bool before) {
+        lower += before;
+        bad |= wrong;
+        if (r != ~0u)
+            atomicAdd(&mine[r], 1u);
+    });
     if constexpr (SCAN) {
-        long long v[HELD];
-#pragma unroll
-        for (int u = 0; u < HELD; u++) {
-            const size_t i = w0 + u * DH_WAVE + lane;
-            v[u] = i < w1 ? a.ids[i * a.ld_ids] : -1;
-        }
-        unsigned lower = 0;
-#pragma unroll
-        for (int u = 0; u < HELD; u++) {
-            const bool valid = v[u] >= 0 && v[u] < static_cast<long long>(a.vocab);
-            if (blockIdx.x == 0 && !valid && w0 + u * DH_WAVE + lane < w1)
-                dh_raise(a.rec, DH_DEFERRED_TOKEN_ID, 0, v[u], a.vocab);
-            const unsigned id = valid ? static_cast<unsigned>(v[u]) : ~0u;
-            lower += id < row0;
-            row[u] = id >= row0 && id - row0 < rows ? id - row0 : ~0u;
-        }
-        for (unsigned i = tid; i < VR * SORT_WAVES; i += SORT_THREADS)
-            cnt[i] = 0;
-        if (tid == 0)
-            front = 0;
-        __syncthreads();
-        if (lower)
+        dh_butterfly(DH_WAVE, [&](auto peer) { lower += peer(lower); });
+        if (lane == 0)
             atomicAdd(&front, lower);
-#pragma unroll
-        for (int u = 0; u < HELD; u++) {
-            const bool in = row[u] != ~0u;
-            rank[u] = 0;
-            if (__ballot(in) != 0)
-                rank[u] = next_place(mine, in, in ? row[u] : 0, a.row_bits);
-        }
-    } else {
-        for (unsigned i = tid; i < VR * SORT_WAVES; i += SORT_THREADS)
-            cnt[i] = 0;
-        __syncthreads();
-#pragma unroll 4
-        for (size_t i = w0 + lane; i < w1; i += DH_WAVE)
-            atomicAdd(&mine[a.list[i] >> 32], 1u);
     }
+    if (SCAN && bad && blockIdx.x == 0)
+        for (size_t i = w0 + lane; i < w1; i += DH_WAVE) {
+            const long long id = a.ids[i * a.ld_ids];
+            if (id < 0 || id >= static_cast<long long>(a.vocab))
+                dh_raise(a.rec, DH_DEFERRED_TOKEN_ID, 0, id, a.vocab);
+        }
     __syncthreads();
     const unsigned all0 = SCAN ? front : static_cast<unsigned>(begin); // number of this owner's first position among all
     for (unsigned r = tid; r < VR; r += SORT_THREADS) {
@@ -284,7 +318,7 @@ template <int HELD> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(
     for (unsigned r = tid; r < VR; r += SORT_THREADS) {
         unsigned at = seg[r];
         if (r < rows)
-            a.row_starts[row0 + r] = all0 + at;
+            a.spans[number(r)] = uint2{all0 + at, all0 + seg[r + 1]};
         for (int w = 0; w < SORT_WAVES; w++) {
             const unsigned c = cnt[w * VR + r];
             cnt[w * VR + r] = at;
@@ -292,8 +326,6 @@ template <int HELD> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(
         }
     }
     const bool last = blockIdx.x + 1 == gridDim.x;
-    if (last && tid == 0)
-        a.row_starts[a.vocab] = all0 + seg[VR];
     __syncthreads();
     if (wave == SORT_WAVES - 1) { // frequent tokens: their positions in parts
         const unsigned all1 = all0 + seg[VR];
@@ -311,10 +343,10 @@ template <int HELD> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(
             const unsigned first = slot + ps - parts;
             for (unsigned k = 0; k < parts; k++) {
                 const unsigned b = all0 + seg[r] + k * PART, e = all0 + seg[r + 1];
-                a.hot_parts[first + k] = HotPart{b, b + PART < e ? b + PART : e, row0 + r, parts == 1};
+                a.hot_parts[first + k] = HotPart{b, b + PART < e ? b + PART : e, number(r), parts == 1};
             }
             if (many)
-                a.hot_rows[row_slot + ms - 1] = HotRow{row0 + r, first, parts, 0};
+                a.hot_rows[row_slot + ms - 1] = HotRow{number(r), first, parts, 0};
             slot += __shfl(ps, DH_WAVE - 1, DH_WAVE);
             row_slot += __shfl(ms, DH_WAVE - 1, DH_WAVE);
         }
@@ -325,27 +357,26 @@ template <int HELD> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(
     }
     if (seg[VR] == 0)
         return;
-    if constexpr (SCAN) {
-#pragma unroll
-        for (int u = 0; u < HELD; u++)
-            if (row[u] != ~0u)
-                a.sorted[all0 + mine[row[u]] + rank[u]] = static_cast<unsigned>(w0 + u * DH_WAVE + lane);
-    } else {
-        for (size_t i0 = w0; i0 < w1; i0 += 4 * DH_WAVE) {
-            unsigned long long v[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const size_t i = i0 + u * DH_WAVE + lane;
-                v[u] = a.list[i < w1 ? i : w1 - 1];
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const bool in = i0 + u * DH_WAVE + lane < w1;
-                const unsigned at = next_place(mine, in, in ? static_cast<unsigned>(v[u] >> 32) : 0, a.row_bits);
-                if (in)
-                    a.sorted[all0 + at] = static_cast<unsigned>(v[u]);
-            }
+    walk([&](unsigned r, unsigned position, bool, bool) {
+        const bool in = r != ~0u;
+        if constexpr (SCAN) {
+            if (__ballot(in) == 0)
+                return;
+            const unsigned at = next_place_of_few(mine, in, in ? r : 0);
+            if (in && at < KEEP)
+                keep[at] = position;
+            else if (in)
+                a.sorted[all0 + at] = position;
+        } else {
+            const unsigned at = next_place(mine, in, in ? r : 0, a.row_bits);
+            if (in)
+                a.sorted[all0 + at] = position;
         }
+    });
+    if constexpr (SCAN) {
+        __syncthreads();
+        for (unsigned i = tid; i < seg[VR] && i < KEEP; i += SORT_THREADS)
+            a.sorted[all0 + i] = keep[i];
     }
 }
 
@@ -357,7 +388,8 @@ template <typename T> struct RowArgs {
     size_t ld_out;
     double scale;
     int accumulate;
-    const unsigned *row_starts, *sorted;
+    const uint2 *spans;
+    const unsigned *sorted;
     const HotRow *hot_rows;
     const HotPart *hot_parts;
     size_t parts;
@@ -431,23 +463,22 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
             continue;
         }
         const size_t row = (u - a.parts) * AT_ONCE;
-        unsigned at[AT_ONCE + 1];
-#pragma unroll
-        for (int k = 0; k <= AT_ONCE; k++)
-            at[k] = a.row_starts[row + k < a.vocab ? row + k : a.vocab];
+        uint2 at[AT_ONCE];
         bool few = true;
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; k++)
-            few &= at[k + 1] - at[k] <= 1;
+        for (int k = 0; k < AT_ONCE; k++) {
+            at[k] = a.spans[row + k < a.vocab ? row + k : a.vocab - 1];
+            few &= at[k].y - at[k].x <= 1;
+        }
         if (few) {
             T v[AT_ONCE][VEC];
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++)
-                if (at[k + 1] != at[k])
-                    dh_seq::load_stream<T, VEC>(column + static_cast<size_t>(a.sorted[at[k]]) * a.ld_out, v[k]);
+                if (at[k].y != at[k].x)
+                    dh_seq::load_stream<T, VEC>(column + static_cast<size_t>(a.sorted[at[k].x]) * a.ld_out, v[k]);
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++) {
-                const bool some = at[k + 1] != at[k];
+                const bool some = at[k].y != at[k].x;
                 if (row + k >= a.vocab || (!some && a.accumulate))
                     continue;
                 double acc[VEC];
@@ -457,8 +488,9 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
                 write_row<T, VEC>(a, row + k, piece, acc);
             }
         } else {
+#pragma unroll
             for (int k = 0; k < AT_ONCE; k++) {
-                const unsigned b = a.row_starts[row + k < a.vocab ? row + k : a.vocab], e = a.row_starts[row + k + 1 < a.vocab ? row + k + 1 : a.vocab];
+                const unsigned b = at[k].x, e = at[k].y;
                 if (row + k >= a.vocab || (a.parts && e - b > HOT) || (b == e && a.accumulate))
                     continue;
                 double acc[VEC] = {};
@@ -499,7 +531,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void join_k
 
 // Stable partition of the tokens by owner: how many each block of tokens has for each owner, owner by owner.
 static __global__ __launch_bounds__(PART_THREADS) void count_kernel(const long long *ids, size_t ld_ids, size_t n, size_t each, long long vocab,
-                                                                    int row_bits, size_t owners, unsigned *counts, int *rec) {
+                                                                    size_t owners, unsigned *counts, int *rec) {
     extern __shared__ unsigned part_lds[];
     for (size_t b = threadIdx.x; b < owners; b += PART_THREADS)
         part_lds[b] = 0;
@@ -511,7 +543,7 @@ static __global__ __launch_bounds__(PART_THREADS) void count_kernel(const long l
         if (id < 0 || id >= vocab)
             dh_raise(rec, DH_DEFERRED_TOKEN_ID, 0, id, vocab);
         else
-            atomicAdd(&part_lds[id >> row_bits], 1u);
+            atomicAdd(&part_lds[id & (owners - 1)], 1u);
     }
     __syncthreads();
     for (size_t b = threadIdx.x; b < owners; b += PART_THREADS)
@@ -563,7 +595,7 @@ static __global__ __launch_bounds__(1024) void scan_counts_kernel(unsigned *coun
 }
 
 static __global__ __launch_bounds__(PART_THREADS) void scatter_kernel(const long long *ids, size_t ld_ids, size_t n, size_t each, long long vocab,
-                                                                      int row_bits, int owner_bits, size_t owners, const unsigned *starts,
+                                                                      int owner_bits, size_t owners, const unsigned *starts,
                                                                       unsigned long long *list) {
     extern __shared__ unsigned part_lds[]; // [PART_WAVES][owners]
     const unsigned wave = threadIdx.x / DH_WAVE, lane = threadIdx.x % DH_WAVE;
@@ -577,7 +609,7 @@ static __global__ __launch_bounds__(PART_THREADS) void scatter_kernel(const long
     for (size_t i = w0 + lane; i < w1; i += DH_WAVE) {
         const long long id = ids[i * ld_ids];
         if (id >= 0 && id < vocab)
-            atomicAdd(&mine[id >> row_bits], 1u);
+            atomicAdd(&mine[id & (owners - 1)], 1u);
     }
     __syncthreads();
     for (size_t b = threadIdx.x; b < owners; b += PART_THREADS) {
@@ -589,12 +621,21 @@ static __global__ __launch_bounds__(PART_THREADS) void scatter_kernel(const long
         }
     }
     __syncthreads();
-    for (size_t i = w0; i < w1; i += DH_WAVE) {
-        const long long id = i + lane < w1 ? ids[(i + lane) * ld_ids] : -1;
-        const bool in = id >= 0 && id < vocab;
-        const unsigned at = next_place(mine, in, in ? static_cast<unsigned>(id >> row_bits) : 0, owner_bits);
-        if (in)
-            list[at] = (static_cast<unsigned long long>(id & ((1ll << row_bits) - 1)) << 32) | static_cast<unsigned>(i + lane);
+    for (size_t i0 = w0; i0 < w1; i0 += 8 * DH_WAVE) {
+        long long v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const size_t i = i0 + u * DH_WAVE + lane;
+            v[u] = ids[(i < w1 ? i : w1 - 1) * ld_ids];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const size_t i = i0 + u * DH_WAVE + lane;
+            const bool in = i < w1 && v[u] >= 0 && v[u] < vocab;
+            const unsigned at = next_place(mine, in, in ? static_cast<unsigned>(v[u] & (owners - 1)) : 0, owner_bits);
+            if (in)
+                list[at] = (static_cast<unsigned long long>(v[u] >> owner_bits) << 32) | static_cast<unsigned>(i);
+        }
     }
 }
 
@@ -602,18 +643,21 @@ static __global__ __launch_bounds__(PART_THREADS) void scatter_kernel(const long
 struct BackwardPlan {
     enum { PLAIN, SCAN, PARTITION } how;
     int row_bits, owner_bits;
-    size_t owners, each, blocks, parts, hots;
+    size_t owners, rows_each, each, blocks, parts, hots;
     size_t starts_at, sorted_at, hot_rows_at, hot_parts_at, partials_at, counts_at, list_at, bytes;
 };
 static inline BackwardPlan backward_plan(size_t n, size_t vocab, size_t width) {
     BackwardPlan p{};
-    p.row_bits = ROW_BITS;
-    while (((vocab - 1) >> p.row_bits) >= OWNERS)
+    p.owner_bits = OWNER_BITS;
+    while (p.owner_bits < MOST_OWNER_BITS && (vocab >> p.owner_bits) >= MOST_ROWS)
+        p.owner_bits++;
+    p.owners = size_t(1) << p.owner_bits;
+    p.rows_each = dh_ceil_div(vocab, p.owners);
+    while ((size_t(1) << p.row_bits) < p.rows_each)
         p.row_bits++;
-    p.owners = dh_ceil_div(vocab, size_t(1) << p.row_bits);
-    p.how = (size_t(1) << p.row_bits) > MOST_ROWS || n >= (size_t(1) << 32) ? BackwardPlan::PLAIN
-            : n <= SCAN_TOKENS                                              ? BackwardPlan::SCAN
-                                                                            : BackwardPlan::PARTITION;
+    p.how = p.rows_each > MOST_ROWS || n >= (size_t(1) << 32) ? BackwardPlan::PLAIN
+            : n <= SCAN_TOKENS                                ? BackwardPlan::SCAN
+                                                              : BackwardPlan::PARTITION;
     if (p.how == BackwardPlan::PLAIN)
         return p;
     size_t at = 0;
@@ -624,14 +668,12 @@ static inline BackwardPlan backward_plan(size_t n, size_t vocab, size_t width) {
     };
     p.parts = n / HOT;
     p.hots = n / PART;
-    p.starts_at = take((vocab + 1) * sizeof(unsigned));
+    p.starts_at = take(vocab * sizeof(uint2));
     p.sorted_at = take(n * sizeof(unsigned));
     p.hot_rows_at = take(p.hots * sizeof(HotRow));
     p.hot_parts_at = take(p.parts * sizeof(HotPart));
     p.partials_at = take(p.hots ? p.parts * (width + 3) * sizeof(double) : 0);
     if (p.how == BackwardPlan::PARTITION) {
-        while ((size_t(1) << p.owner_bits) < p.owners)
-            p.owner_bits++;
         // blocks of 2048 tokens, at most 256 of them
         p.each = 2048 * dh_ceil_div(n, 2048 * 256);
         p.blocks = dh_ceil_div(n, p.each);
@@ -655,7 +697,7 @@ static inline dh_status backward_sorted(dh_ctx *ctx, RowArgs<T> &r, SortArgs &a,
     if (slices >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "embeddingBackward - extents exceed one launch");
     unsigned char *w = static_cast<unsigned char *>(work);
-    r.row_starts = a.row_starts = reinterpret_cast<unsigned *>(w + p.starts_at);
+    r.spans = a.spans = reinterpret_cast<uint2 *>(w + p.starts_at);
     r.sorted = a.sorted = reinterpret_cast<unsigned *>(w + p.sorted_at);
     r.hot_rows = a.hot_rows = reinterpret_cast<HotRow *>(w + p.hot_rows_at);
     r.hot_parts = a.hot_parts = reinterpret_cast<HotPart *>(w + p.hot_parts_at);
@@ -663,8 +705,9 @@ static inline dh_status backward_sorted(dh_ctx *ctx, RowArgs<T> &r, SortArgs &a,
     r.parts = p.parts;
     a.parts = static_cast<unsigned>(p.parts);
     a.hots = static_cast<unsigned>(p.hots);
-    a.rows_each = 1u << p.row_bits;
+    a.rows_each = static_cast<unsigned>(p.rows_each);
     a.row_bits = p.row_bits;
+    a.owner_bits = p.owner_bits;
     if (p.how == BackwardPlan::PARTITION) {
         unsigned *counts = reinterpret_cast<unsigned *>(w + p.counts_at);
         unsigned long long *list = reinterpret_cast<unsigned long long *>(w + p.list_at);
@@ -673,13 +716,13 @@ static inline dh_status backward_sorted(dh_ctx *ctx, RowArgs<T> &r, SortArgs &a,
         a.list = list;
         const dim3 blocks(static_cast<unsigned>(p.blocks));
         hipLaunchKernelGGL(count_kernel, blocks, dim3(PART_THREADS), p.owners * sizeof(unsigned), ctx->stream, a.ids, a.ld_ids, a.n, p.each,
-                           static_cast<long long>(a.vocab), p.row_bits, p.owners, counts, a.rec);
+                           static_cast<long long>(a.vocab), p.owners, counts, a.rec);
         hipLaunchKernelGGL(scan_counts_kernel, dim3(1), dim3(1024), 0, ctx->stream, counts, p.owners * p.blocks);
         hipLaunchKernelGGL(scatter_kernel, blocks, dim3(PART_THREADS), PART_WAVES * p.owners * sizeof(unsigned), ctx->stream, a.ids, a.ld_ids,
-                           a.n, p.each, static_cast<long long>(a.vocab), p.row_bits, p.owner_bits, p.owners, counts, list);
+                           a.n, p.each, static_cast<long long>(a.vocab), p.owner_bits, p.owners, counts, list);
     }
     const size_t lds = ((1 + SORT_WAVES) * a.rows_each + 1) * sizeof(unsigned);
-    auto *sort = p.how != BackwardPlan::SCAN ? &sort_kernel<0> : a.n <= 8 * SORT_THREADS ? &sort_kernel<8> : &sort_kernel<32>;
+    auto *sort = p.how == BackwardPlan::SCAN ? &sort_kernel<true> : &sort_kernel<false>;
     if (lds > 65536)
         DH_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(sort), hipFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(lds)));
