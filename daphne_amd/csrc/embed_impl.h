@@ -397,10 +397,10 @@ template <typename T> struct RowArgs {
     unsigned lanes; // of a row: a power of two up to 64
 };
 
-// Adds rows [begin, end) of the positions to acc, in order.
+// Adds rows [begin, end) of the positions to acc, in order, eight of them requested together.
 template <typename T, int VEC, class Position>
 __device__ __forceinline__ void add_rows(double (&acc)[VEC], const T *d_out, size_t ld_out, size_t begin, size_t end, Position position) {
-    auto round = [&](auto most, size_t k) { // up to that many rows, all loads in flight together
+    auto round = [&](auto most, size_t k) {
         constexpr int N = decltype(most)::value;
         T v[N][VEC];
 #pragma unroll
@@ -440,9 +440,7 @@ __device__ __forceinline__ void write_row(const RowArgs<T> &a, size_t row, dh_se
 template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_kernel(RowArgs<T> a) {
     constexpr int AT_ONCE = 4;
     const unsigned lane = threadIdx.x % a.lanes, each = THREADS / a.lanes;
-    const size_t vec = static_cast<size_t>(blockIdx.y) * a.lanes + lane;
-    if (vec >= a.width_vecs)
-        return;
+    const size_t vec = static_cast<size_t>(blockIdx.y) * a.lanes + lane; // behind the last one: reads the last one, writes nothing
     const size_t units = a.parts + (a.vocab + AT_ONCE - 1) / AT_ONCE;
     const dh_seq::Piece piece = dh_seq::piece<VEC>(vec, a.width);
     const T *column = a.d_out + piece.at;
@@ -453,10 +451,16 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
             if (p.end == 0)
                 continue;
             double acc[VEC] = {};
-            add_rows<T, VEC>(acc, column, a.ld_out, p.begin, p.end, position);
+            if (a.lanes >= PART) { // the part's positions in one load, handed around
+                const unsigned have = p.end - p.begin, mine = a.sorted[p.begin + (lane < have ? lane : have - 1)];
+                const int base = static_cast<int>(threadIdx.x % DH_WAVE - lane);
+                add_rows<T, VEC>(acc, column, a.ld_out, 0, have, [&](size_t k) { return __shfl(mine, base + static_cast<int>(k), DH_WAVE); });
+            } else {
+                add_rows<T, VEC>(acc, column, a.ld_out, p.begin, p.end, position);
+            }
             if (p.whole)
                 write_row<T, VEC>(a, p.row, piece, acc);
-            else
+            else if (vec < a.width_vecs)
 #pragma unroll
                 for (int q = 0; q < VEC; q++)
                     a.partials[(u * a.width_vecs + vec) * VEC + q] = acc[q];
