@@ -19,7 +19,7 @@ typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(1))); // r
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-typedef f32x4 f32x4_lds __attribute__((may_alias));
+
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4_lds __attribute__((may_alias)); // parts of x in LDS, written as words
@@ -34,11 +34,11 @@ __device__ __forceinline__ void lds_in_order() {
 // A wavefront multiplies 16 rows of x with T tiles of 16 outputs, STEP columns at a time; the WAVES wavefronts of a workgroup
 // share its columns and add their results at the end, in order.
 constexpr int STEP = 128, WAVES = 8, AHEAD = 4;
-constexpr int SCALE_ROW = AHEAD * STEP / 32 + 4; // floats of one output's scales in LDS
+constexpr int SCALE_ROW = 4 + AHEAD * STEP / 32 + 5; // floats of one output's scales in LDS; odd, for its banks
 constexpr int PLANE = STEP * 2 + 16; // bytes of one row of one part of x in LDS; the odd 16 keep 16 rows off each other's banks
 
 constexpr unsigned own_lds(bool floats, int tiles, int rows) { // bytes of a wavefront
-    return tiles * 16 * SCALE_ROW * 4 + (floats ? 3 * rows * PLANE : 0);
+    return (tiles * 16 * SCALE_ROW * 4 + 15) / 16 * 16 + (floats ? 3 * rows * PLANE : 0);
 }
 
 template <typename X> struct Args {
@@ -108,9 +108,11 @@ template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WA
     const unsigned wave = __builtin_amdgcn_readfirstlane(tid / DH_WAVE);
     const size_t o0 = static_cast<size_t>(blockIdx.x) * (16 * T), m0 = static_cast<size_t>(blockIdx.y) * 16;
     const unsigned M = a.rows - m0 < 16 ? static_cast<unsigned>(a.rows - m0) : 16u;
-    const unsigned whole = static_cast<unsigned>(a.cols) / 32 * 32, steps = (whole + STEP - 1) / STEP; // columns behind `whole`: at the end
+    // Steps whose chunks of 32 columns are all complete go four at a time; one that ends within a chunk comes last, by itself.
+    const unsigned cols = static_cast<unsigned>(a.cols), steps = (cols + STEP - 1) / STEP, rest = cols % 32 ? 1u : 0u;
     const unsigned each = (steps + WAVES - 1) / WAVES;
     const unsigned s0 = wave * each < steps ? wave * each : steps, s1 = s0 + each < steps ? s0 + each : steps;
+    const unsigned full = s1 == steps && s1 > s0 ? s1 - rest : s1; // of this wavefront's steps
     const unsigned m = col < M ? col : M - 1; // rows that do not exist: the last one again, whose results are dropped
     const unsigned char *w[T];
     const float *sc[T];
@@ -121,124 +123,190 @@ template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WA
         sc[t] = a.scales + o * a.ld_scales;
     }
     const X *x = a.x + m0 * a.ld_x;
-    unsigned char *mine = q4_lds + wave * own_lds(FLOATS, T, MT); // this wavefront's scales, and parts of x
-    float *my_scales = reinterpret_cast<float *>(mine);
-    mine += T * 16 * SCALE_ROW * sizeof(float);
-    const unsigned groups = a.group_of(static_cast<unsigned>((a.cols + 31) / 32 - 1)) + 1;
+    float *my_scales = reinterpret_cast<float *>(q4_lds + wave * own_lds(FLOATS, T, MT)); // this wavefront's scales, and parts of x
+    unsigned char *mine = reinterpret_cast<unsigned char *>(my_scales + T * 16 * SCALE_ROW);
+    const unsigned groups = a.group_of((cols + 31) / 32 - 1) + 1;
     float acc[T][4] = {};
-    for (unsigned sb = s0; sb < s1; sb += AHEAD) {
-        u32x4 c[AHEAD][T];
-        f32x4 scale4[T];
-        u32x4 xq[FLOATS ? 1 : AHEAD][2];
-        f32x2_any xf[FLOATS && MT == 1 ? AHEAD : 1];
-        // What AHEAD steps need is on its way before the first of them begins. Their scales: at most 16 of an output, four a lane.
-        const unsigned g0 = a.group_of(sb * CHUNKS), ga = g0 + kb * 4;
-#pragma unroll
-        for (int t = 0; t < T; t++)
-            if (ga + 4 <= groups)
-                scale4[t] = *reinterpret_cast<const f32x4_any *>(sc[t] + ga);
-            else
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    scale4[t][e] = sc[t][ga + e < groups ? ga + e : groups - 1];
-#pragma unroll
-        for (int u = 0; u < AHEAD; u++) {
-            const unsigned s = sb + u < s1 ? sb + u : s1 - 1, k = s * STEP + kb * 32; // 32 codes a lane; behind the row: its beginning, not used
+
+    // The scales of AHEAD steps, at most 16 an output: four a lane. Near the end of a row the four move back; SCALE_ROW begins with room
+    // for that.
+    f32x4 scale4[T];
+    auto request_scales = [&](unsigned g0) {
+        const unsigned ga = g0 + kb * 4 + 4 <= groups ? g0 + kb * 4 : groups - 4;
+        if (groups >= 4) {
 #pragma unroll
             for (int t = 0; t < T; t++)
-                c[u][t] = *reinterpret_cast<const u32x4_any *>(w[t] + (k < whole ? k / 2 : 0));
+                scale4[t] = *reinterpret_cast<const f32x4_any *>(sc[t] + ga);
+        } else {
+#pragma unroll
+            for (int t = 0; t < T; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    scale4[t][e] = sc[t][kb * 4 + e < groups ? kb * 4 + e : groups - 1];
+        }
+    };
+    auto keep_scales = [&](unsigned g0) {
+        const unsigned ga = groups < 4 ? kb * 4 : g0 + kb * 4 + 4 <= groups ? g0 + kb * 4 : groups - 4;
+#pragma unroll
+        for (int t = 0; t < T; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                my_scales[(t * 16 + col) * SCALE_ROW + 4 + ga + e - (groups < 4 ? 0 : g0)] = scale4[t][e];
+        lds_in_order();
+    };
+    auto scale = [&](int t, unsigned chunk, unsigned g0) {
+        return my_scales[(t * 16 + col) * SCALE_ROW + 4 + a.group_of(chunk) - (groups < 4 ? 0 : g0)];
+    };
+    // x in three parts: the upper 16 bits, those of the rest, and what then is left (8 bits)
+    auto stage = [&](const f32x2_any(&v)[MT]) {
+#pragma unroll
+        for (int r = 0; r < MT; r++) {
+            unsigned q[3][2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float rest = v[r][e];
+                q[0][e] = __builtin_bit_cast(unsigned, rest);
+                const float hi = __builtin_bit_cast(float, q[0][e] & 0xffff0000u);
+                rest = rest == hi ? 0.0f : rest - hi; // an infinity has no rest
+                q[1][e] = __builtin_bit_cast(unsigned, rest);
+                q[2][e] = __builtin_bit_cast(unsigned, rest - __builtin_bit_cast(float, q[1][e] & 0xffff0000u));
+            }
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+                *reinterpret_cast<u32_lds *>(mine + (p * MT + r) * PLANE + lane * 4) = __builtin_amdgcn_perm(q[p][1], q[p][0], 0x07060302);
+        }
+        lds_in_order();
+    };
+    auto multiply = [&](u32x4(&c)[T], const u32x4(&xq)[2], unsigned s, unsigned g0) {
+        const unsigned k0 = s * STEP;
+        const int chunks = cols - k0 < STEP ? static_cast<int>(cols - k0 + 31) / 32 : CHUNKS;
+#pragma unroll
+        for (int t = 0; t < T; t++)
+            transpose4(c[t]);
+        u32x4 lo, hi; // 8-bit rows: the halves of a lane's four times 8 columns
+        if constexpr (!FLOATS) {
+            lo = u32x4{xq[0][0], xq[0][2], xq[1][0], xq[1][2]};
+            hi = u32x4{xq[0][1], xq[0][3], xq[1][1], xq[1][3]};
+            transpose4(lo);
+            transpose4(hi);
+        }
+        C sum[T] = {};
+#pragma unroll
+        for (int d = 0; d < CHUNKS; d++) {
+            if (d >= chunks)
+                break;
+            Op op;
+            if constexpr (FLOATS) {
+#pragma unroll
+                for (int p = 0; p < 3; p++)
+                    op.part[p] = __builtin_bit_cast(
+                        bf16x8, *reinterpret_cast<const u32x4_lds *>(mine + (p * MT + (MT == 1 ? 0 : m)) * PLANE + d * 64 + kb * 16));
+            } else {
+                const unsigned even = __builtin_amdgcn_perm(hi[d], lo[d], 0x06040200), odd = __builtin_amdgcn_perm(hi[d], lo[d], 0x07050301);
+                op.a = static_cast<long>((static_cast<unsigned long>(odd) << 32) | even);
+            }
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                sum[t] = op.times(c[t][d], sum[t]);
+                if constexpr (!WHOLE) {
+                    const float one = scale(t, s * CHUNKS + d, g0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        acc[t][i] += one * static_cast<float>(sum[t][i]);
+                    sum[t] = C{};
+                }
+            }
+        }
+        if constexpr (WHOLE)
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                const float one = scale(t, s * CHUNKS, g0);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc[t][i] += one * static_cast<float>(sum[t][i]);
+            }
+        lds_in_order();
+    };
+
+    for (unsigned sb = s0; sb < full; sb += AHEAD) { // what AHEAD steps need is on its way before the first of them begins
+        u32x4 c[AHEAD][T], xq[AHEAD][2];
+        f32x2_any xf[FLOATS && MT == 1 ? AHEAD : 1];
+        const unsigned g0 = a.group_of(sb * CHUNKS);
+        request_scales(g0);
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const unsigned s = sb + u < full ? sb + u : full - 1, k = s * STEP + kb * 32; // 32 codes a lane
+            const unsigned at = k < cols ? k : 0;                                        // behind the row: its beginning, not used
+#pragma unroll
+            for (int t = 0; t < T; t++)
+                c[u][t] = *reinterpret_cast<const u32x4_any *>(w[t] + at / 2);
             if constexpr (!FLOATS)
 #pragma unroll
                 for (int h = 0; h < 2; h++)
-                    xq[u][h] = *reinterpret_cast<const u32x4_any *>(x + m * a.ld_x + (k < whole ? k : 0) + h * 16);
+                    xq[u][h] = *reinterpret_cast<const u32x4_any *>(x + m * a.ld_x + at + h * 16);
             else if constexpr (MT == 1)
-                xf[u] = *reinterpret_cast<const f32x2_any *>(x + (s * STEP + 2 * lane < whole ? s * STEP + 2 * lane : 0));
+                xf[u] = *reinterpret_cast<const f32x2_any *>(x + (s * STEP + 2 * lane < cols ? s * STEP + 2 * lane : 0));
         }
-#pragma unroll
-        for (int t = 0; t < T; t++)
-            *reinterpret_cast<f32x4_lds *>(my_scales + (t * 16 + col) * SCALE_ROW + kb * 4) = scale4[t];
-        lds_in_order();
+        keep_scales(g0);
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
-            const unsigned s = sb + u, k0 = s * STEP;
-            if (s >= s1)
+            if (sb + u >= full)
                 break;
-            const int chunks = whole - k0 < STEP ? static_cast<int>(whole - k0) / 32 : CHUNKS;
-            if constexpr (FLOATS) { // x in three parts: the upper 16 bits, those of the rest, and what then is left (8 bits)
+            if constexpr (FLOATS) {
                 f32x2_any v[MT];
-                const unsigned k2 = k0 + 2 * lane < whole ? k0 + 2 * lane : 0;
+                const unsigned k2 = (sb + u) * STEP + 2 * lane;
 #pragma unroll
                 for (int r = 0; r < MT; r++)
                     if constexpr (MT == 1)
                         v[r] = xf[u];
                     else
-                        v[r] = *reinterpret_cast<const f32x2_any *>(x + (static_cast<unsigned>(r) < M ? r : M - 1) * a.ld_x + k2);
-#pragma unroll
-                for (int r = 0; r < MT; r++) {
-                    unsigned q[3][2];
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float rest = v[r][e];
-                        q[0][e] = __builtin_bit_cast(unsigned, rest);
-                        const float hi = __builtin_bit_cast(float, q[0][e] & 0xffff0000u);
-                        rest = rest == hi ? 0.0f : rest - hi; // an infinity has no rest
-                        q[1][e] = __builtin_bit_cast(unsigned, rest);
-                        q[2][e] = __builtin_bit_cast(unsigned, rest - __builtin_bit_cast(float, q[1][e] & 0xffff0000u));
-                    }
-#pragma unroll
-                    for (int p = 0; p < 3; p++)
-                        *reinterpret_cast<u32_lds *>(mine + (p * MT + r) * PLANE + lane * 4) = __builtin_amdgcn_perm(q[p][1], q[p][0], 0x07060302);
-                }
-                lds_in_order();
+                        v[r] = *reinterpret_cast<const f32x2_any *>(x + (static_cast<unsigned>(r) < M ? r : M - 1) * a.ld_x + (k2 < cols ? k2 : 0));
+                stage(v);
             }
-#pragma unroll
-            for (int t = 0; t < T; t++)
-                transpose4(c[u][t]);
-            u32x4 lo, hi; // 8-bit rows: the halves of a lane's four times 8 columns
-            if constexpr (!FLOATS) {
-                lo = u32x4{xq[u][0][0], xq[u][0][2], xq[u][1][0], xq[u][1][2]};
-                hi = u32x4{xq[u][0][1], xq[u][0][3], xq[u][1][1], xq[u][1][3]};
-                transpose4(lo);
-                transpose4(hi);
-            }
-            auto scale = [&](int t, int d) { return my_scales[(t * 16 + col) * SCALE_ROW + a.group_of(s * CHUNKS + d) - g0]; };
-            C sum[T] = {};
-#pragma unroll
-            for (int d = 0; d < CHUNKS; d++) {
-                if (d >= chunks)
-                    break;
-                Op op;
-                if constexpr (FLOATS) {
-#pragma unroll
-                    for (int p = 0; p < 3; p++)
-                        op.part[p] = __builtin_bit_cast(
-                            bf16x8, *reinterpret_cast<const u32x4_lds *>(mine + (p * MT + (MT == 1 ? 0 : m)) * PLANE + d * 64 + kb * 16));
-                } else {
-                    const unsigned even = __builtin_amdgcn_perm(hi[d], lo[d], 0x06040200), odd = __builtin_amdgcn_perm(hi[d], lo[d], 0x07050301);
-                    op.a = static_cast<long>((static_cast<unsigned long>(odd) << 32) | even);
-                }
-#pragma unroll
-                for (int t = 0; t < T; t++) {
-                    sum[t] = op.times(c[u][t][d], sum[t]);
-                    if constexpr (!WHOLE) {
-                        const float one = scale(t, d);
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            acc[t][i] += one * static_cast<float>(sum[t][i]);
-                        sum[t] = C{};
-                    }
-                }
-            }
-            if constexpr (WHOLE)
-#pragma unroll
-                for (int t = 0; t < T; t++) {
-                    const float one = scale(t, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        acc[t][i] += one * static_cast<float>(sum[t][i]);
-                }
-            lds_in_order();
+            multiply(c[u], xq[u], sb + u, g0);
         }
+    }
+    if (full < s1) { // the step that ends within a chunk: byte by byte, what lies behind the row as zeros
+        const unsigned k = full * STEP + kb * 32, g0 = a.group_of(full * CHUNKS);
+        u32x4 c[T], xq[2];
+#pragma unroll
+        for (int t = 0; t < T; t++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                unsigned v = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const unsigned at = k + (q * 4 + e) * 2, byte = w[t][(at < cols ? at : cols - 1) / 2];
+                    v |= (at + 1 < cols ? byte : at < cols ? byte & 15u : 0u) << (8 * e);
+                }
+                c[t][q] = v;
+            }
+        if constexpr (FLOATS) {
+            f32x2_any v[MT];
+            const unsigned k2 = full * STEP + 2 * lane;
+#pragma unroll
+            for (int r = 0; r < MT; r++) {
+                const float *xr = x + (static_cast<unsigned>(r) < M ? r : M - 1) * a.ld_x;
+                const float v0 = xr[k2 < cols ? k2 : cols - 1], v1 = xr[k2 + 1 < cols ? k2 + 1 : cols - 1];
+                v[r][0] = k2 < cols ? v0 : 0.0f;
+                v[r][1] = k2 + 1 < cols ? v1 : 0.0f;
+            }
+            stage(v);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                unsigned v = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const unsigned at = k + q * 4 + e, byte = static_cast<unsigned char>(x[m * a.ld_x + (at < cols ? at : cols - 1)]);
+                    v |= (at < cols ? byte : 0u) << (8 * e);
+                }
+                xq[q / 4][q % 4] = v;
+            }
+        }
+        request_scales(g0);
+        keep_scales(g0);
+        multiply(c, xq, full, g0);
     }
     __syncthreads(); // the parts of x
     float *red = reinterpret_cast<float *>(q4_lds);
@@ -257,10 +325,6 @@ template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WA
         for (int q = 0; q < WAVES; q++)
             v += red[((q * T + t) * 4 + i) * DH_WAVE + l];
         v *= Op::UNIT;
-        for (unsigned k = whole; k < a.cols; k++) {
-            const int byte = a.codes[o * a.ld_codes + k / 2], code = k % 2 ? static_cast<int>(static_cast<unsigned>(byte) << 24) >> 28 : static_cast<int>(static_cast<unsigned>(byte) << 28) >> 28;
-            v += a.scales[o * a.ld_scales + a.group_of(k / 32)] * (static_cast<float>(code) * static_cast<float>(x[row * a.ld_x + k]));
-        }
         a.res[(m0 + row) * a.ld_res + o] = FLOATS ? v : v * a.x_scale[m0 + row];
     }
 }
@@ -311,8 +375,13 @@ dh_status matvec(dh_ctx *ctx, float *res, size_t ld_res, const X *x, size_t rows
     const size_t per_group = group / 32 < (size_t(1) << 20) ? group / 32 : size_t(1) << 20; // wider than any matrix: one group
     const Args<X> a{res, ld_res, x, rows, cols, ld_x, x_scale, codes, outs, ld_codes, scales, ld_scales,
                     dh_ceil_div(size_t(1) << 40, per_group)};
-    const bool two = dh_ceil_div(outs, 32) * dh_ceil_div(rows, 16) >= static_cast<size_t>(ctx->num_cus), whole = group % STEP == 0;
-    if (two)
+    // As many tiles a wavefront as leave every compute unit a workgroup. Four: where rows of floats are many, whose splitting then
+    // serves twice the outputs.
+    const size_t row_tiles = dh_ceil_div(rows, 16), cus = static_cast<size_t>(ctx->num_cus);
+    const bool whole = group % STEP == 0;
+    if (sizeof(X) == 4 && rows > 4 && dh_ceil_div(outs, 64) * row_tiles >= cus)
+        return whole ? launch<X, 4, true>(ctx, a) : launch<X, 4, false>(ctx, a);
+    if (dh_ceil_div(outs, 32) * row_tiles >= cus)
         return whole ? launch<X, 2, true>(ctx, a) : launch<X, 2, false>(ctx, a);
     return whole ? launch<X, 1, true>(ctx, a) : launch<X, 1, false>(ctx, a);
 }

@@ -42,6 +42,24 @@ template <int TPR, class Op> __device__ __forceinline__ double over_row(double v
     return v;
 }
 
+// The sum of one value and the maximum of another, together.
+template <int TPR> __device__ __forceinline__ void over_row(double &sum, double &most, double *slots, double *slots2) {
+    dh_butterfly(DH_WAVE, [&](auto peer) {
+        sum += peer(sum);
+        most = Max()(most, peer(most));
+    });
+    if constexpr (TPR > DH_WAVE) {
+        __syncthreads();
+        if (threadIdx.x % DH_WAVE == 0)
+            slots[threadIdx.x / DH_WAVE] = sum, slots2[threadIdx.x / DH_WAVE] = most;
+        __syncthreads();
+        sum = slots[0], most = slots2[0];
+#pragma unroll
+        for (int w = 1; w < TPR / DH_WAVE; w++)
+            sum += slots[w], most = Max()(most, slots2[w]);
+    }
+}
+
 template <typename T> struct ForwardArgs {
     T *res;
     signed char *codes; // the 8-bit result instead of res
@@ -95,7 +113,7 @@ __device__ __forceinline__ void write_vec(const ForwardArgs<T> &a, size_t row, d
 template <typename T, int VEC, int TPR, int KV, bool Q8>
 __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void forward_kernel(ForwardArgs<T> a) {
     constexpr int WG = TPR > THREADS ? TPR : THREADS, RPW = WG / TPR, K = KV ? KV : 1;
-    __shared__ double slots[WG / DH_WAVE];
+    __shared__ double slots[WG / DH_WAVE], slots2[Q8 ? WG / DH_WAVE : 1];
     const unsigned lane = threadIdx.x % TPR;
     const size_t row = static_cast<size_t>(blockIdx.x) * RPW + threadIdx.x / TPR;
     if (RPW > 1 && row >= a.rows) // whole wavefronts: a row of TPR = 64 meets no barrier
@@ -161,13 +179,15 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void forward_kerne
             reduce(h[0], g[0], at.shift);
         }
     }
-    sq = over_row<TPR>(sq, slots, Add());
+    if constexpr (Q8)
+        over_row<TPR>(sq, most, slots, slots2);
+    else
+        sq = over_row<TPR>(sq, slots, Add());
     const double inv = 1.0 / sqrt(sq / static_cast<double>(a.cols) + a.eps);
     if (a.inv_rms && lane == 0)
         a.inv_rms[row] = static_cast<T>(inv);
     double to_code = 0.0;
     if constexpr (Q8) {
-        most = over_row<TPR>(most, slots, Max());
         // a row of zeros has scale 0; one that holds an infinity or a NaN has no scale: codes 0 and the scale NaN
         const bool finite = most <= 1.7976931348623157e308;
         const double unit = static_cast<double>(static_cast<T>(inv));
