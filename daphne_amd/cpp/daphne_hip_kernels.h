@@ -35,6 +35,7 @@
 #include <runtime/local/kernels/HIP/PipelineProgramBuilder.h>
 #include <runtime/local/kernels/HIP/Pooling.h>
 #include <runtime/local/kernels/HIP/PoolingBackward.h>
+#include <runtime/local/kernels/HIP/SequenceModel.h>
 #include <runtime/local/kernels/HIP/Softmax.h>
 #include <runtime/local/kernels/HIP/Solve.h>
 #include <runtime/local/kernels/HIP/Syrk.h>

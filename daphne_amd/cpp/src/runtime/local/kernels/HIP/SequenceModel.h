@@ -1,0 +1,305 @@
+// Kernels of models over token sequences (rows are tokens, the sequences of a batch one behind the other):
+//   embeddingForward / embeddingBackward              rows of a table by token number, scaled; the table's gradient
+//   rmsNormForward / rmsNormForwardQ8 / rmsNormBackward   root-mean-square norm on a residual stream; its 8-bit form; its gradient
+//   gatedRecurrenceForward / gatedRecurrenceBackward  h_t = f_t h_{t-1} + (1 - f_t) x_t, f = sigmoid(z), per sequence and channel
+//   quantizeQ4 / matVecQ4 / matVecQ4Q8                weights as 4-bit codes with group scales, and products with them
+// The reference has no kernels for them; signatures follow its convention (results first as DT *&, nullptr: allocated here;
+// the DaphneContext last). Arguments that may be missing are nullptr: residual, gamma, dSum, h0, dLast, and offsets (all
+// sequences then have equally many rows, as many sequences as h0 has rows).
+// The mathematics and the checks are those of the dh_* entry points (daphne_hip.h).
+#pragma once
+
+#include <runtime/local/kernels/HIP/HostUtils.h>
+
+#include <tuple>
+
+namespace HIP {
+
+#define DH_OVERLOAD2(NAME)                                                                                              \
+    template <typename... A> inline dh_status NAME(float, A... a) { return NAME##_f32(a...); }                          \
+    template <typename... A> inline dh_status NAME(double, A... a) { return NAME##_f64(a...); }
+DH_OVERLOAD2(dh_embedding_forward)
+DH_OVERLOAD2(dh_embedding_backward)
+DH_OVERLOAD2(dh_rmsnorm_forward)
+DH_OVERLOAD2(dh_rmsnorm_backward)
+DH_OVERLOAD2(dh_gated_recurrence_forward)
+DH_OVERLOAD2(dh_gated_recurrence_backward)
+#undef DH_OVERLOAD2
+
+namespace detail {
+// The shape a matrix has to have (nullptr: it is missing, which its caller allows).
+template <class DT> void shape(const char *kernel, const char *what, const DT *m, size_t rows, size_t cols) {
+    if (m != nullptr && (m->getNumRows() != rows || m->getNumCols() != cols))
+        throw std::runtime_error(std::string(kernel) + ": " + what + " is " + std::to_string(m->getNumRows()) + " x " +
+                                 std::to_string(m->getNumCols()) + ", " + std::to_string(rows) + " x " + std::to_string(cols) + " is needed");
+}
+// The values of a row or a column without gaps.
+template <class DT> void vector(const char *kernel, const char *what, const DT *m, size_t n) {
+    if (m == nullptr)
+        return;
+    const size_t r = m->getNumRows(), c = m->getNumCols();
+    if (r * c != n || std::min(r, c) > 1 || (r > 1 && m->getRowSkip() != c))
+        throw std::runtime_error(std::string(kernel) + ": " + what + " is not a vector of " + std::to_string(n) + " values without gaps");
+}
+template <class DTSel> void column(const char *kernel, const char *what, const DTSel *m, size_t rows) {
+    static_assert(std::is_same<typename DTSel::VT, int64_t>::value, "token numbers and offsets are int64_t");
+    shape(kernel, what, m, rows, 1);
+}
+template <class DT> const typename DT::VT *values(const DT *m, const IAllocationDescriptor *desc) {
+    return m == nullptr ? nullptr : m->getValues(desc);
+}
+template <class DT> size_t skip(const DT *m) { return m == nullptr ? 0 : m->getRowSkip(); }
+template <class DT> void provide(DT *&m, size_t rows, size_t cols, AllocationDescriptorHIP *desc) {
+    if (m == nullptr)
+        m = DataObjectFactory::create<DT>(rows, cols, false, desc);
+}
+} // namespace detail
+
+template <class DTRes, class DTArg, class DTSel> struct EmbeddingForward {
+    static void apply(DTRes *&res, const DTArg *table, const DTSel *ids, const typename DTArg::VT scale, DCTX(ctx)) {
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        using VT = typename DTArg::VT;
+        detail::column("embeddingForward", "ids", ids, ids->getNumRows());
+        detail::provide(res, ids->getNumRows(), table->getNumCols(), &alloc_desc);
+        detail::shape("embeddingForward", "the result", res, ids->getNumRows(), table->getNumCols());
+        check(dh_embedding_forward(VT(), detail::raw(ctx), res->getValues(&alloc_desc), res->getRowSkip(), table->getValues(&alloc_desc),
+                                   table->getNumRows(), table->getNumCols(), table->getRowSkip(), ids->getValues(&alloc_desc),
+                                   ids->getNumRows(), ids->getRowSkip(), scale));
+    }
+};
+template <class DTRes, class DTArg, class DTSel>
+void embeddingForward(DTRes *&res, const DTArg *table, const DTSel *ids, const typename DTArg::VT scale, DCTX(ctx)) {
+    EmbeddingForward<DTRes, DTArg, DTSel>::apply(res, table, ids, scale, ctx);
+}
+
+template <class DTRes, class DTArg, class DTSel> struct EmbeddingBackward {
+    static void apply(DTRes *&dTable, const DTArg *dOut, const DTSel *ids, const size_t vocab, const typename DTArg::VT scale, DCTX(ctx)) {
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        using VT = typename DTArg::VT;
+        detail::column("embeddingBackward", "ids", ids, dOut->getNumRows());
+        detail::provide(dTable, vocab, dOut->getNumCols(), &alloc_desc);
+        detail::shape("embeddingBackward", "the result", dTable, vocab, dOut->getNumCols());
+        check(dh_embedding_backward(VT(), detail::raw(ctx), dTable->getValues(&alloc_desc), vocab, dOut->getNumCols(), dTable->getRowSkip(),
+                                    dOut->getValues(&alloc_desc), dOut->getRowSkip(), ids->getValues(&alloc_desc), ids->getNumRows(),
+                                    ids->getRowSkip(), scale, 0, static_cast<void *>(nullptr), size_t(0)));
+    }
+};
+template <class DTRes, class DTArg, class DTSel>
+void embeddingBackward(DTRes *&dTable, const DTArg *dOut, const DTSel *ids, const size_t vocab, const typename DTArg::VT scale, DCTX(ctx)) {
+    EmbeddingBackward<DTRes, DTArg, DTSel>::apply(dTable, dOut, ids, vocab, scale, ctx);
+}
+
+// Without a residual the sum is x itself: resSum is then left as it is.
+template <class DTRes, class DTArg> struct RmsNormForward {
+    static void apply(DTRes *&res, DTRes *&resSum, DTRes *&invRms, const DTArg *x, const DTArg *residual, const DTArg *gamma,
+                      const typename DTArg::VT eps, DCTX(ctx)) {
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        using VT = typename DTArg::VT;
+        const size_t rows = x->getNumRows(), cols = x->getNumCols();
+        detail::provide(res, rows, cols, &alloc_desc);
+        detail::provide(invRms, rows, 1, &alloc_desc);
+        if (residual != nullptr)
+            detail::provide(resSum, rows, cols, &alloc_desc);
+        detail::shape("rmsNormForward", "the result", res, rows, cols);
+        detail::shape("rmsNormForward", "residual", residual, rows, cols);
+        detail::vector("rmsNormForward", "invRms", invRms, rows);
+        detail::vector("rmsNormForward", "gamma", gamma, cols);
+        DTRes *sum = residual != nullptr ? resSum : nullptr;
+        detail::shape("rmsNormForward", "the sum", sum, rows, cols);
+        check(dh_rmsnorm_forward(VT(), detail::raw(ctx), res->getValues(&alloc_desc), res->getRowSkip(),
+                                 sum != nullptr ? sum->getValues(&alloc_desc) : static_cast<VT *>(nullptr), detail::skip(sum),
+                                 invRms->getValues(&alloc_desc), x->getValues(&alloc_desc), rows, cols, x->getRowSkip(),
+                                 detail::values(residual, &alloc_desc), detail::skip(residual), detail::values(gamma, &alloc_desc), eps));
+    }
+};
+template <class DTRes, class DTArg>
+void rmsNormForward(DTRes *&res, DTRes *&resSum, DTRes *&invRms, const DTArg *x, const DTArg *residual, const DTArg *gamma,
+                    const typename DTArg::VT eps, DCTX(ctx)) {
+    RmsNormForward<DTRes, DTArg>::apply(res, resSum, invRms, x, residual, gamma, eps, ctx);
+}
+
+template <class DTRes, class DTArg> struct RmsNormForwardQ8 {
+    static void apply(DTRes *&res, DTArg *&resScale, DTArg *&resSum, DTArg *&invRms, const DTArg *x, const DTArg *residual, const DTArg *gamma,
+                      const typename DTArg::VT eps, DCTX(ctx)) {
+        static_assert(std::is_same<typename DTRes::VT, int8_t>::value && std::is_same<typename DTArg::VT, float>::value,
+                      "8-bit rows of floats");
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        const size_t rows = x->getNumRows(), cols = x->getNumCols();
+        detail::provide(res, rows, cols, &alloc_desc);
+        detail::provide(resScale, rows, 1, &alloc_desc);
+        detail::provide(invRms, rows, 1, &alloc_desc);
+        if (residual != nullptr)
+            detail::provide(resSum, rows, cols, &alloc_desc);
+        detail::shape("rmsNormForwardQ8", "the result", res, rows, cols);
+        detail::shape("rmsNormForwardQ8", "residual", residual, rows, cols);
+        detail::vector("rmsNormForwardQ8", "resScale", resScale, rows);
+        detail::vector("rmsNormForwardQ8", "invRms", invRms, rows);
+        detail::vector("rmsNormForwardQ8", "gamma", gamma, cols);
+        DTArg *sum = residual != nullptr ? resSum : nullptr;
+        detail::shape("rmsNormForwardQ8", "the sum", sum, rows, cols);
+        check(dh_rmsnorm_forward_q8_f32(detail::raw(ctx), res->getValues(&alloc_desc), res->getRowSkip(), resScale->getValues(&alloc_desc),
+                                        sum != nullptr ? sum->getValues(&alloc_desc) : nullptr, detail::skip(sum),
+                                        invRms->getValues(&alloc_desc), x->getValues(&alloc_desc), rows, cols, x->getRowSkip(),
+                                        detail::values(residual, &alloc_desc), detail::skip(residual), detail::values(gamma, &alloc_desc),
+                                        eps));
+    }
+};
+template <class DTRes, class DTArg>
+void rmsNormForwardQ8(DTRes *&res, DTArg *&resScale, DTArg *&resSum, DTArg *&invRms, const DTArg *x, const DTArg *residual,
+                      const DTArg *gamma, const typename DTArg::VT eps, DCTX(ctx)) {
+    RmsNormForwardQ8<DTRes, DTArg>::apply(res, resScale, resSum, invRms, x, residual, gamma, eps, ctx);
+}
+
+template <class DTRes, class DTArg> struct RmsNormBackward {
+    static void apply(DTRes *&dX, DTRes *&dGamma, const DTArg *h, const DTArg *invRms, const DTArg *gamma, const DTArg *dRes,
+                      const DTArg *dSum, DCTX(ctx)) {
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        using VT = typename DTArg::VT;
+        const size_t rows = h->getNumRows(), cols = h->getNumCols();
+        detail::provide(dX, rows, cols, &alloc_desc);
+        detail::provide(dGamma, 1, cols, &alloc_desc);
+        detail::shape("rmsNormBackward", "the result", dX, rows, cols);
+        detail::shape("rmsNormBackward", "dRes", dRes, rows, cols);
+        detail::shape("rmsNormBackward", "dSum", dSum, rows, cols);
+        detail::vector("rmsNormBackward", "dGamma", dGamma, cols);
+        detail::vector("rmsNormBackward", "gamma", gamma, cols);
+        detail::vector("rmsNormBackward", "invRms", invRms, rows);
+        check(dh_rmsnorm_backward(VT(), detail::raw(ctx), dX->getValues(&alloc_desc), dX->getRowSkip(), dGamma->getValues(&alloc_desc),
+                                  h->getValues(&alloc_desc), rows, cols, h->getRowSkip(), invRms->getValues(&alloc_desc),
+                                  detail::values(gamma, &alloc_desc), dRes->getValues(&alloc_desc), dRes->getRowSkip(),
+                                  detail::values(dSum, &alloc_desc), detail::skip(dSum), static_cast<void *>(nullptr), size_t(0)));
+    }
+};
+template <class DTRes, class DTArg>
+void rmsNormBackward(DTRes *&dX, DTRes *&dGamma, const DTArg *h, const DTArg *invRms, const DTArg *gamma, const DTArg *dRes, const DTArg *dSum,
+                     DCTX(ctx)) {
+    RmsNormBackward<DTRes, DTArg>::apply(dX, dGamma, h, invRms, gamma, dRes, dSum, ctx);
+}
+
+namespace detail {
+// How many sequences there are: by the offsets, else by the states given, else one.
+template <class DTArg, class DTSel> size_t sequences(const char *kernel, const DTSel *offsets, const DTArg *state) {
+    if (offsets != nullptr && offsets->getNumRows() == 0)
+        throw std::runtime_error(std::string(kernel) + ": offsets need a value more than there are sequences");
+    const size_t n = offsets != nullptr ? offsets->getNumRows() - 1 : state != nullptr ? state->getNumRows() : 1;
+    column(kernel, "offsets", offsets, n + 1);
+    return n;
+}
+} // namespace detail
+
+template <class DTRes, class DTArg, class DTSel> struct GatedRecurrenceForward {
+    static void apply(DTRes *&res, DTRes *&resLast, const DTArg *x, const DTArg *z, const DTArg *h0, const DTSel *offsets, DCTX(ctx)) {
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        using VT = typename DTArg::VT;
+        const char *kernel = "gatedRecurrenceForward";
+        const size_t tokens = x->getNumRows(), channels = x->getNumCols(), n = detail::sequences(kernel, offsets, h0);
+        detail::provide(res, tokens, channels, &alloc_desc);
+        detail::provide(resLast, n, channels, &alloc_desc);
+        detail::shape(kernel, "z", z, tokens, channels);
+        detail::shape(kernel, "the result", res, tokens, channels);
+        detail::shape(kernel, "h0", h0, n, channels);
+        detail::shape(kernel, "the last state", resLast, n, channels);
+        check(dh_gated_recurrence_forward(VT(), detail::raw(ctx), res->getValues(&alloc_desc), res->getRowSkip(), resLast->getValues(&alloc_desc),
+                                          resLast->getRowSkip(), x->getValues(&alloc_desc), tokens, channels, x->getRowSkip(),
+                                          z->getValues(&alloc_desc), z->getRowSkip(), detail::values(h0, &alloc_desc), detail::skip(h0),
+                                          detail::values(offsets, &alloc_desc), detail::skip(offsets), n, static_cast<void *>(nullptr),
+                                          size_t(0)));
+    }
+};
+template <class DTRes, class DTArg, class DTSel>
+void gatedRecurrenceForward(DTRes *&res, DTRes *&resLast, const DTArg *x, const DTArg *z, const DTArg *h0, const DTSel *offsets, DCTX(ctx)) {
+    GatedRecurrenceForward<DTRes, DTArg, DTSel>::apply(res, resLast, x, z, h0, offsets, ctx);
+}
+
+template <class DTRes, class DTArg, class DTSel> struct GatedRecurrenceBackward {
+    static void apply(DTRes *&dX, DTRes *&dZ, DTRes *&dH0, const DTArg *x, const DTArg *z, const DTArg *h, const DTArg *h0, const DTArg *dRes,
+                      const DTArg *dLast, const DTSel *offsets, DCTX(ctx)) {
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        using VT = typename DTArg::VT;
+        const char *kernel = "gatedRecurrenceBackward";
+        const size_t tokens = x->getNumRows(), channels = x->getNumCols(), n = detail::sequences(kernel, offsets, h0 != nullptr ? h0 : dLast);
+        detail::provide(dX, tokens, channels, &alloc_desc);
+        detail::provide(dZ, tokens, channels, &alloc_desc);
+        detail::provide(dH0, n, channels, &alloc_desc);
+        for (const auto &[what, m, rows] : {std::tuple<const char *, const DTArg *, size_t>{"z", z, tokens}, {"h", h, tokens},
+                                            {"dRes", dRes, tokens}, {"dX", dX, tokens}, {"dZ", dZ, tokens}, {"h0", h0, n}, {"dLast", dLast, n},
+                                            {"dH0", dH0, n}})
+            detail::shape(kernel, what, m, rows, channels);
+        check(dh_gated_recurrence_backward(
+            VT(), detail::raw(ctx), dX->getValues(&alloc_desc), dX->getRowSkip(), dZ->getValues(&alloc_desc), dZ->getRowSkip(),
+            dH0->getValues(&alloc_desc), dH0->getRowSkip(), x->getValues(&alloc_desc), tokens, channels, x->getRowSkip(),
+            z->getValues(&alloc_desc), z->getRowSkip(), h->getValues(&alloc_desc), h->getRowSkip(), detail::values(h0, &alloc_desc),
+            detail::skip(h0), dRes->getValues(&alloc_desc), dRes->getRowSkip(), detail::values(dLast, &alloc_desc), detail::skip(dLast),
+            detail::values(offsets, &alloc_desc), detail::skip(offsets), n, static_cast<void *>(nullptr), size_t(0)));
+    }
+};
+template <class DTRes, class DTArg, class DTSel>
+void gatedRecurrenceBackward(DTRes *&dX, DTRes *&dZ, DTRes *&dH0, const DTArg *x, const DTArg *z, const DTArg *h, const DTArg *h0,
+                             const DTArg *dRes, const DTArg *dLast, const DTSel *offsets, DCTX(ctx)) {
+    GatedRecurrenceBackward<DTRes, DTArg, DTSel>::apply(dX, dZ, dH0, x, z, h, h0, dRes, dLast, offsets, ctx);
+}
+
+template <class DTCodes, class DTArg> struct QuantizeQ4 {
+    static void apply(DTCodes *&codes, DTArg *&scales, const DTArg *weights, const size_t group, DCTX(ctx)) {
+        static_assert(std::is_same<typename DTCodes::VT, uint8_t>::value && std::is_same<typename DTArg::VT, float>::value,
+                      "4-bit codes of floats");
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        if (group == 0)
+            throw std::invalid_argument("quantizeQ4: the group of 0 columns is not a multiple of 32");
+        const size_t rows = weights->getNumRows(), cols = weights->getNumCols();
+        detail::provide(codes, rows, (cols + 1) / 2, &alloc_desc);
+        detail::provide(scales, rows, (cols + group - 1) / group, &alloc_desc);
+        detail::shape("quantizeQ4", "codes", codes, rows, (cols + 1) / 2);
+        detail::shape("quantizeQ4", "scales", scales, rows, (cols + group - 1) / group);
+        check(dh_quantize_q4_f32(detail::raw(ctx), codes->getValues(&alloc_desc), codes->getRowSkip(), scales->getValues(&alloc_desc),
+                                 scales->getRowSkip(), weights->getValues(&alloc_desc), rows, cols, weights->getRowSkip(), group));
+    }
+};
+template <class DTCodes, class DTArg> void quantizeQ4(DTCodes *&codes, DTArg *&scales, const DTArg *weights, const size_t group, DCTX(ctx)) {
+    QuantizeQ4<DTCodes, DTArg>::apply(codes, scales, weights, group, ctx);
+}
+
+namespace detail {
+template <class DTRes, class DTX, class DTCodes, class DTScale>
+void q4Shapes(const char *kernel, DTRes *&res, const DTX *x, const DTCodes *codes, const DTScale *scales, size_t group,
+              AllocationDescriptorHIP *desc) {
+    if (group == 0)
+        throw std::invalid_argument(std::string(kernel) + ": the group of 0 columns is not a multiple of 32");
+    const size_t cols = x->getNumCols(), outs = codes->getNumRows();
+    shape(kernel, "codes", codes, outs, (cols + 1) / 2);
+    shape(kernel, "scales", scales, outs, (cols + group - 1) / group);
+    provide(res, x->getNumRows(), outs, desc);
+    shape(kernel, "the result", res, x->getNumRows(), outs);
+}
+} // namespace detail
+
+template <class DTRes, class DTCodes> struct MatVecQ4 {
+    static void apply(DTRes *&res, const DTRes *x, const DTCodes *codes, const DTRes *scales, const size_t group, DCTX(ctx)) {
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        detail::q4Shapes("matVecQ4", res, x, codes, scales, group, &alloc_desc);
+        check(dh_matvec_q4_f32(detail::raw(ctx), res->getValues(&alloc_desc), res->getRowSkip(), x->getValues(&alloc_desc), x->getNumRows(),
+                               x->getNumCols(), x->getRowSkip(), codes->getValues(&alloc_desc), codes->getNumRows(), codes->getRowSkip(),
+                               scales->getValues(&alloc_desc), scales->getRowSkip(), group));
+    }
+};
+template <class DTRes, class DTCodes>
+void matVecQ4(DTRes *&res, const DTRes *x, const DTCodes *codes, const DTRes *scales, const size_t group, DCTX(ctx)) {
+    MatVecQ4<DTRes, DTCodes>::apply(res, x, codes, scales, group, ctx);
+}
+
+template <class DTRes, class DTX, class DTCodes> struct MatVecQ4Q8 {
+    static void apply(DTRes *&res, const DTX *x, const DTRes *xScale, const DTCodes *codes, const DTRes *scales, const size_t group, DCTX(ctx)) {
+        AllocationDescriptorHIP alloc_desc(ctx, detail::deviceID);
+        detail::vector("matVecQ4Q8", "xScale", xScale, x->getNumRows());
+        detail::q4Shapes("matVecQ4Q8", res, x, codes, scales, group, &alloc_desc);
+        check(dh_matvec_q4_q8_f32(detail::raw(ctx), res->getValues(&alloc_desc), res->getRowSkip(), x->getValues(&alloc_desc), x->getNumRows(),
+                                  x->getNumCols(), x->getRowSkip(), xScale->getValues(&alloc_desc), codes->getValues(&alloc_desc),
+                                  codes->getNumRows(), codes->getRowSkip(), scales->getValues(&alloc_desc), scales->getRowSkip(), group));
+    }
+};
+template <class DTRes, class DTX, class DTCodes>
+void matVecQ4Q8(DTRes *&res, const DTX *x, const DTRes *xScale, const DTCodes *codes, const DTRes *scales, const size_t group, DCTX(ctx)) {
+    MatVecQ4Q8<DTRes, DTX, DTCodes>::apply(res, x, xScale, codes, scales, group, ctx);
+}
+
+} // namespace HIP

@@ -19,9 +19,9 @@ ROOT = Path(__file__).resolve().parent.parent
 sys.path.insert(0, str(ROOT / "tests"))
 
 SUFFIX = {np.dtype(np.float32): "f32", np.dtype(np.float64): "f64", np.dtype(np.int64): "si64", np.dtype(np.uint64): "ui64",
-          np.dtype(np.int32): "si32", np.dtype(np.uint32): "ui32"}
+          np.dtype(np.int32): "si32", np.dtype(np.uint32): "ui32", np.dtype(np.int8): "si8", np.dtype(np.uint8): "ui8"}
 CPP_VT = {"float": np.float32, "double": np.float64, "int64_t": np.int64, "uint64_t": np.uint64, "size_t": np.uint64,
-          "int32_t": np.int32, "uint32_t": np.uint32}
+          "int32_t": np.int32, "uint32_t": np.uint32, "int8_t": np.int8, "uint8_t": np.uint8}
 SCALAR_CT = {"float": C.c_float, "double": C.c_double, "int64_t": C.c_int64, "uint64_t": C.c_uint64, "size_t": C.c_size_t,
              "int32_t": C.c_int32, "uint32_t": C.c_uint32, "bool": C.c_bool}
 

@@ -107,7 +107,33 @@ TH_MATRIX(si64, int64_t)
 TH_MATRIX(ui64, uint64_t)
 TH_MATRIX(si32, int32_t)
 TH_MATRIX(ui32, uint32_t)
+TH_MATRIX(si8, int8_t)
+TH_MATRIX(ui8, uint8_t)
 #undef TH_MATRIX
+
+// Sequence-model kernels whose arguments they refuse: 1 if the call threw (its text in th_last_error).
+#define TH_SEQ(NAME, CALL)                                                                                              \
+    int th_seq_##NAME(void *ctx_, void *a, void *b, void *c) {                                                          \
+        auto *ctx = static_cast<DaphneContext *>(ctx_);                                                                 \
+        auto *x = static_cast<DenseMatrix<float> *>(a);                                                                 \
+        DenseMatrix<float> *r0 = nullptr, *r1 = nullptr, *r2 = nullptr;                                                 \
+        DenseMatrix<uint8_t> *r8 = nullptr;                                                                             \
+        const int threw = guarded([&] { CALL; });                                                                       \
+        for (auto *r : {r0, r1, r2})                                                                                    \
+            if (r != nullptr)                                                                                           \
+                DataObjectFactory::destroy(r);                                                                          \
+        if (r8 != nullptr)                                                                                              \
+            DataObjectFactory::destroy(r8);                                                                             \
+        (void)b, (void)c, (void)r1, (void)r2;                                                                           \
+        return threw;                                                                                                   \
+    }
+TH_SEQ(embedding, HIP::embeddingForward(r0, x, static_cast<DenseMatrix<int64_t> *>(b), 1.0f, ctx))
+TH_SEQ(rmsnorm,
+       HIP::rmsNormForward(r0, r1, r2, x, static_cast<DenseMatrix<float> *>(b), static_cast<DenseMatrix<float> *>(c), 1e-5f, ctx))
+TH_SEQ(recurrence, HIP::gatedRecurrenceForward(r0, r1, x, static_cast<DenseMatrix<float> *>(b), static_cast<DenseMatrix<float> *>(nullptr),
+                                               static_cast<DenseMatrix<int64_t> *>(c), ctx))
+TH_SEQ(q4, HIP::quantizeQ4(r8, r0, x, 31, ctx))
+#undef TH_SEQ
 
 // One fused body over `shares` row shares. in_roles: HIP::PipeInput per input, out_roles: HIP::PipeOutput per output.
 // outputs[o] receives a new matrix handle.
