@@ -91,7 +91,7 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, const T *table, size_t voc
     return dh_checked_end(ctx);
 }
 
-// Tables beyond what the sorted form below takes (more than 8 Mi rows): one workgroup per table row and slice of THREADS columns; the positions of its token are picked out of every THREADS
+// Tables beyond what the sorted form below takes (more than 4 Mi rows): one workgroup per table row and slice of THREADS columns; the positions of its token are picked out of every THREADS
 // token numbers in order, and their rows added.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size_t ld, long long vocab, size_t width, const T *d_out,
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size
 // sort_kernel puts the positions of all tokens in the order of owner and row (stable: positions stay in order) and notes where each
 // row's begin and end. An owner is a workgroup that has every `owners`-th row of the table, so that the frequent tokens, whose
 // numbers often lie together, are spread over all of them. It finds its positions by reading all tokens: 16 wavefronts go through a
-// share each (32768 tokens: 28 us, as much as by way of the partition, 65536: 35 against 27).
+// share each (32768 tokens: 21 us, by way of the partition 33).
 // Beyond SCAN_TOKENS that reading would cost too much: the tokens are first split into lists, one per owner, by a stable
 // partition (count, scan, scatter).
 // rows_kernel then writes every row, zeros where there is nothing to add: 64 lanes of 16 bytes (fewer where rows are shorter)
@@ -154,9 +154,10 @@ constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / DH_WAVE;
 constexpr unsigned HOT = 8, PART = 32;
 constexpr size_t SCAN_TOKENS = 32768;   // up to here every owner reads all tokens
 constexpr unsigned KEEP = 4096;                   // positions an owner keeps in LDS
+constexpr unsigned FOUND = 512;                   // positions a wavefront finds at once
 constexpr int OWNER_BITS = 8;                     // 1 << OWNER_BITS owners, more for large tables
 constexpr int MOST_OWNER_BITS = 12;
-constexpr size_t MOST_ROWS = 2048;                // most rows of an owner
+constexpr size_t MOST_ROWS = 1024;                // most rows of an owner
 constexpr size_t PART_THREADS = 256, PART_WAVES = PART_THREADS / DH_WAVE;
 
 struct HotPart { // positions [begin, end) of `sorted`; end = 0: none
@@ -232,6 +233,10 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
     unsigned *mine = cnt + wave * VR;
     __shared__ unsigned front;    // SCAN: positions of all rows before this owner's
     __shared__ unsigned keep[KEEP]; // SCAN: what is placed goes out together (each store by itself would hold up the loads behind it)
+    // SCAN: this owner's tokens as they are found, row << 16 | token of the wavefront's share, a list for every wavefront. One that
+    // does not fit (a token that half of all are) is found a second time.
+    __shared__ unsigned found[SCAN ? SORT_WAVES : 1][SCAN ? FOUND : 1];
+    unsigned have = 0;
     const unsigned owner = blockIdx.x, mask = (1u << a.owner_bits) - 1;
     const unsigned rows = a.vocab > owner ? (a.vocab - owner - 1) / (mask + 1) + 1 : 0;
     auto number = [&](unsigned r) { return owner + (r << a.owner_bits); };
@@ -272,9 +277,18 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
     __syncthreads();
     unsigned lower = 0;
     bool bad = false;
-    walk([&](unsigned r, unsigned, bool wrong, bool before) {
+    walk([&](unsigned r, unsigned position, bool wrong, bool before) {
         lower += before;
         bad |= wrong;
+        if constexpr (SCAN) {
+            const unsigned long long some = __ballot(r != ~0u);
+            if (some == 0)
+                return;
+            const unsigned at = have + __popcll(some & ((1ull << lane) - 1));
+            if (r != ~0u && at < FOUND)
+                found[wave][at] = (r << 16) | (position - static_cast<unsigned>(w0));
+            have += __popcll(some);
+        }
         if (r != ~0u)
             atomicAdd(&mine[r], 1u);
     });
@@ -357,22 +371,25 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
     }
     if (seg[VR] == 0)
         return;
-    walk([&](unsigned r, unsigned position, bool, bool) {
+    auto place = [&](unsigned r, unsigned position) {
         const bool in = r != ~0u;
-        if constexpr (SCAN) {
-            if (__ballot(in) == 0)
-                return;
-            const unsigned at = next_place_of_few(mine, in, in ? r : 0);
-            if (in && at < KEEP)
-                keep[at] = position;
-            else if (in)
-                a.sorted[all0 + at] = position;
-        } else {
-            const unsigned at = next_place(mine, in, in ? r : 0, a.row_bits);
-            if (in)
-                a.sorted[all0 + at] = position;
+        const unsigned at = SCAN ? next_place_of_few(mine, in, in ? r : 0) : next_place(mine, in, in ? r : 0, a.row_bits);
+        if (in && SCAN && at < KEEP)
+            keep[at] = position;
+        else if (in)
+            a.sorted[all0 + at] = position;
+    };
+    if (SCAN && have <= FOUND) {
+        for (unsigned i = 0; i < have; i += DH_WAVE) {
+            const unsigned f = found[wave][i + lane < have ? i + lane : have - 1];
+            place(i + lane < have ? f >> 16 : ~0u, static_cast<unsigned>(w0) + (f & 0xffffu));
         }
-    });
+    } else {
+        walk([&](unsigned r, unsigned position, bool, bool) {
+            if (!SCAN || __ballot(r != ~0u) != 0)
+                place(r, position);
+        });
+    }
     if constexpr (SCAN) {
         __syncthreads();
         for (unsigned i = tid; i < seg[VR] && i < KEEP; i += SORT_THREADS)
