@@ -91,8 +91,8 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, const T *table, size_t voc
     return dh_checked_end(ctx);
 }
 
-// Tables beyond what the sorted form below takes (more than 4 Mi rows): one workgroup per table row and slice of THREADS columns; the positions of its token are picked out of every THREADS
-// token numbers in order, and their rows added.
+// Tables beyond what the sorted form below takes (more than 4 Mi rows): one workgroup per table row and slice of THREADS columns; the
+// positions of its token are picked out of every THREADS token numbers in order, and their rows added.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size_t ld, long long vocab, size_t width, const T *d_out,
                                                                 size_t ld_out, const long long *ids, size_t ld_ids, size_t n, T scale,
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size
     }
     if (col < width && (any || !accumulate)) {
         T *p = d_table + static_cast<size_t>(v) * ld + col;
-        const double s = acc * static_cast<double>(scale);
+        const double s = any ? acc * static_cast<double>(scale) : 0.0;
         *p = static_cast<T>(accumulate ? s + static_cast<double>(*p) : s);
     }
 }
@@ -439,14 +439,15 @@ __device__ __forceinline__ void add_rows(double (&acc)[VEC], const T *d_out, siz
         round(std::integral_constant<int, 1>{}, k);
 }
 
+// scale: 0 for a row without positions, which is zero whatever the gradient's scale is.
 template <typename T, int VEC>
-__device__ __forceinline__ void write_row(const RowArgs<T> &a, size_t row, dh_seq::Piece at, const double (&acc)[VEC]) {
+__device__ __forceinline__ void write_row(const RowArgs<T> &a, size_t row, dh_seq::Piece at, const double (&acc)[VEC], double scale) {
     T *p = a.d_table + row * a.ld + at.at, v[VEC];
     if (a.accumulate)
         dh_seq::load<T, VEC>(p, v);
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
-        const double s = acc[e] * a.scale;
+        const double s = acc[e] * scale;
         v[e] = static_cast<T>(a.accumulate ? s + static_cast<double>(v[e]) : s);
     }
     dh_seq::store<T, VEC, true>(p, v, at.shift);
@@ -476,7 +477,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
                 add_rows<T, VEC>(acc, column, a.ld_out, p.begin, p.end, position);
             }
             if (p.whole)
-                write_row<T, VEC>(a, p.row, piece, acc);
+                write_row<T, VEC>(a, p.row, piece, acc, a.scale);
             else if (vec < a.width_vecs)
 #pragma unroll
                 for (int q = 0; q < VEC; q++)
@@ -506,7 +507,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
 #pragma unroll
                 for (int q = 0; q < VEC; q++)
                     acc[q] = some ? static_cast<double>(v[k][q]) : 0.0;
-                write_row<T, VEC>(a, row + k, piece, acc);
+                write_row<T, VEC>(a, row + k, piece, acc, some ? a.scale : 0.0);
             }
         } else {
 #pragma unroll
@@ -516,7 +517,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
                     continue;
                 double acc[VEC] = {};
                 add_rows<T, VEC>(acc, column, a.ld_out, b, e, position);
-                write_row<T, VEC>(a, row + k, piece, acc);
+                write_row<T, VEC>(a, row + k, piece, acc, b != e ? a.scale : 0.0);
             }
         }
     }
@@ -547,7 +548,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void join_k
 #pragma unroll
         for (int q = 0; q < VEC; q++)
             acc[q] += part[w][lane * VEC + q];
-    write_row<T, VEC>(a, h.row, dh_seq::piece<VEC>(vec, a.width), acc);
+    write_row<T, VEC>(a, h.row, dh_seq::piece<VEC>(vec, a.width), acc, a.scale);
 }
 
 // Stable partition of the tokens by owner: how many each block of tokens has for each owner, owner by owner.

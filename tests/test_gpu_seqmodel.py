@@ -153,6 +153,12 @@ def test_embedding_backward_views_and_no_tokens(ctx, dt):
         dv, _ = view(ctx, d_out, 2, 1)
         want, mag = embedding_gradient(ids, d_out, 90, 1.0)
         near(embeddingBackward(None, dv, iv, 90, 1.0, ctx).to_numpy(), want, (n + 2) * 2.0**-53 * mag + U(dt) * np.abs(want) * 1.001)
+    ids, d_out = np.array([[3], [3], [5]]), np.ones((3, 6), dt)  # rows of tokens that do not occur are zeros, whatever the scale
+    for scale in (-1.0, np.inf):
+        got = embeddingBackward(None, D(ctx, d_out), D(ctx, ids), 9, scale, ctx).to_numpy()
+        absent = np.delete(got, [3, 5], axis=0)
+        assert not absent.any() and not np.signbit(absent).any()
+        np.testing.assert_array_equal(got[[3, 5]], np.array([[2 * scale], [scale]]) * np.ones((1, 6)))
     none = embeddingBackward(D(ctx, np.ones((9, 21), dt)), DenseMatrix(ctx, 0, 21, dt), DenseMatrix(ctx, 0, 1, np.int64), 9, 1.0, ctx)
     assert not none.to_numpy().any()
     assert embeddingForward(None, D(ctx, np.ones((9, 21), dt)), DenseMatrix(ctx, 0, 1, np.int64), 1.0, ctx).rows == 0
@@ -618,6 +624,14 @@ def test_q4_views(ctx, rows, cols, outs, group):
             w, xw = whole.to_numpy(), xm.astype(F64) * f
             near(w[:, right:right + outs], xw @ (c * s).T, (cols / 8 + 20) * U(F32) * (np.abs(xw) @ np.abs(c * s).T))
             assert np.all(w[:, :right] == 7) and np.all(w[:, right + outs:] == 7)
+
+
+def test_q4_without_columns(ctx):
+    codes, scales = DenseMatrix(ctx, 5, 0, np.uint8), DenseMatrix(ctx, 5, 0, F32)
+    got = matVecQ4(D(ctx, np.full((3, 5), 7, F32)), DenseMatrix(ctx, 3, 0, F32), None, codes, scales, 32, ctx)
+    assert not got.to_numpy().any()
+    got = matVecQ4(D(ctx, np.full((3, 5), 7, F32)), DenseMatrix(ctx, 3, 0, np.int8), D(ctx, np.ones((3, 1), F32)), codes, scales, 32, ctx)
+    assert not got.to_numpy().any()
 
 
 def test_q4_values_that_are_not_finite_stay_in_their_rows(ctx):
