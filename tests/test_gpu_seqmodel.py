@@ -113,7 +113,7 @@ def embedding_gradient(ids, d_out, vocab, scale, before=None):
 
 
 EMBED_BWD = [(1, 1, 1), (1, 300, 64), (5, 17, 3), (64, 1000, 512), (300, 50, 129), (4096, 70, 33), (4097, 70, 33), (4099, 6000, 260),
-             (9000, 1, 8), (20000, 513, 36), (30000, 40000, 12), (12345, 300000, 5), (50, 3, 5000), (5000, 2000000, 2), (900, 2000001, 1), (40, 8400000, 1), (70000, 300, 4), (131073, 700, 3), (66000, 1500000, 1), (33000, 140000, 2), (600000, 5000, 1)]
+             (9000, 1, 8), (20000, 513, 36), (30000, 40000, 12), (12345, 300000, 5), (50, 3, 5000), (5000, 2000000, 2), (900, 2000001, 1), (40, 8400000, 1), (70000, 300, 4), (131073, 700, 3), (66000, 1500000, 1), (33000, 140000, 2), (66000, 9000, 3), (600000, 5000, 1)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
