@@ -70,7 +70,7 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, const T *table, size_t voc
     while (lpr < THREADS && lpr < wv)
         lpr <<= 1;
     const size_t gx = dh_ceil_div(n, THREADS / lpr);
-    const bool four = gx * dh_ceil_div(wv, lpr) >= 4096; // several vectors in flight a thread once the workgroups fill the device
+    const bool four = wv > lpr && gx * dh_ceil_div(wv, lpr) >= 4096; // several vectors in flight a thread once the workgroups fill the device
     const size_t gy = dh_ceil_div(wv, static_cast<size_t>(lpr) * (four ? 4 : 1));
     if (gx >= (size_t(1) << 31) || gy >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "embeddingForward - extents exceed one launch");
@@ -160,6 +160,8 @@ constexpr int MOST_OWNER_BITS = 12;
 constexpr size_t MOST_ROWS = 1024;                // most rows of an owner
 constexpr size_t PART_THREADS = 256, PART_WAVES = PART_THREADS / DH_WAVE;
 
+constexpr unsigned ONE = ~0u;
+
 struct HotPart { // positions [begin, end) of `sorted`; end = 0: none
     unsigned begin, end, row, whole; // whole: the row's only part
 };
@@ -216,7 +218,7 @@ struct SortArgs {
     const unsigned *starts; // partition: first place of owner b's list at starts[b * blocks], behind the last one the end
     size_t blocks;
     const unsigned long long *list; // row within the owner's << 32 | position
-    uint2 *spans;                   // [vocab]: the row's first position in `sorted` and the one behind its last
+    uint2 *spans;                   // [vocab]: where the row's positions begin and end in `sorted`, or its only position and ONE
     unsigned *sorted;
     HotRow *hot_rows;
     HotPart *hot_parts;
@@ -248,24 +250,34 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
     const size_t w0 = begin + wave * share < end ? begin + wave * share : end, w1 = w0 + share < end ? w0 + share : end;
     constexpr int EIGHT = 8;
     auto walk = [&](auto &&take) { // take(row or ~0, position, whether there is one, token)
-        for (size_t i0 = w0; i0 < w1; i0 += EIGHT * DH_WAVE) {
-            long long v[EIGHT];
+        const size_t ld = SCAN ? a.ld_ids : 1;
+        const unsigned long long *src = SCAN ? reinterpret_cast<const unsigned long long *>(a.ids) : a.list;
+        const unsigned long long *p = src + (w0 + lane) * ld;
+        const unsigned len = static_cast<unsigned>(w1 - w0);
+        for (unsigned i0 = 0; i0 < len; i0 += EIGHT * DH_WAVE, p += EIGHT * DH_WAVE * ld) {
+            unsigned long long v[EIGHT];
+            if (len - i0 >= EIGHT * DH_WAVE) {
 #pragma unroll
-            for (int u = 0; u < EIGHT; u++) { // behind the share: its last, not used (a guard would make each load wait for the one before)
-                const size_t i = i0 + u * DH_WAVE + lane, at = i < w1 ? i : w1 - 1;
-                v[u] = SCAN ? a.ids[at * a.ld_ids] : static_cast<long long>(a.list[at]);
+                for (int u = 0; u < EIGHT; u++)
+                    v[u] = p[u * DH_WAVE * ld];
+            } else {
+#pragma unroll
+                for (int u = 0; u < EIGHT; u++) { // behind the share: its last, not used (a guard would make each load wait for the one before)
+                    const unsigned i = i0 + u * DH_WAVE + lane;
+                    v[u] = src[(w0 + (i < len ? i : len - 1)) * ld];
+                }
             }
 #pragma unroll
             for (int u = 0; u < EIGHT; u++) {
-                const size_t i = i0 + u * DH_WAVE + lane;
-                const bool here = i < w1;
+                const unsigned i = i0 + u * DH_WAVE + lane;
+                const bool here = i < len;
                 if constexpr (SCAN) {
-                    const bool valid = here && v[u] >= 0 && v[u] < static_cast<long long>(a.vocab);
+                    const bool valid = here && v[u] < a.vocab; // a negative number is a large one
                     const unsigned id = static_cast<unsigned>(v[u]);
-                    take(valid && (id & mask) == owner ? id >> a.owner_bits : ~0u, static_cast<unsigned>(i), here && !valid,
+                    take(valid && (id & mask) == owner ? id >> a.owner_bits : ~0u, static_cast<unsigned>(w0) + i, here && !valid,
                          valid && (id & mask) < owner);
                 } else {
-                    take(here ? static_cast<unsigned>(static_cast<unsigned long long>(v[u]) >> 32) : ~0u, static_cast<unsigned>(v[u]), false, false);
+                    take(here ? static_cast<unsigned>(v[u] >> 32) : ~0u, static_cast<unsigned>(v[u]), false, false);
                 }
             }
         }
@@ -331,8 +343,6 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
     __syncthreads();
     for (unsigned r = tid; r < VR; r += SORT_THREADS) {
         unsigned at = seg[r];
-        if (r < rows)
-            a.spans[number(r)] = uint2{all0 + at, all0 + seg[r + 1]};
         for (int w = 0; w < SORT_WAVES; w++) {
             const unsigned c = cnt[w * VR + r];
             cnt[w * VR + r] = at;
@@ -369,14 +379,12 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
         for (unsigned k = row_slot + lane; k < row_slots; k += DH_WAVE)
             a.hot_rows[k] = HotRow{0, 0, 0, 0};
     }
-    if (seg[VR] == 0)
-        return;
     auto place = [&](unsigned r, unsigned position) {
         const bool in = r != ~0u;
         const unsigned at = SCAN ? next_place_of_few(mine, in, in ? r : 0) : next_place(mine, in, in ? r : 0, a.row_bits);
-        if (in && SCAN && at < KEEP)
+        if (in && at < KEEP)
             keep[at] = position;
-        else if (in)
+        if (in && (!SCAN || at >= KEEP))
             a.sorted[all0 + at] = position;
     };
     if (SCAN && have <= FOUND) {
@@ -390,10 +398,14 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
                 place(r, position);
         });
     }
+    __syncthreads();
     if constexpr (SCAN) {
-        __syncthreads();
         for (unsigned i = tid; i < seg[VR] && i < KEEP; i += SORT_THREADS)
             a.sorted[all0 + i] = keep[i];
+    }
+    for (unsigned r = tid; r < rows; r += SORT_THREADS) {
+        const unsigned b = seg[r], e = seg[r + 1];
+        a.spans[number(r)] = e == b + 1 && b < KEEP ? uint2{keep[b], ONE} : uint2{all0 + b, all0 + e};
     }
 }
 
@@ -411,7 +423,7 @@ template <typename T> struct RowArgs {
     const HotPart *hot_parts;
     size_t parts;
     double *partials;
-    unsigned lanes; // of a row: a power of two up to 64
+    unsigned lanes, slices; // of a row: a power of two up to 64, and how many times as many a row takes
 };
 
 // Adds rows [begin, end) of the positions to acc, in order, eight of them requested together.
@@ -422,7 +434,7 @@ __device__ __forceinline__ void add_rows(double (&acc)[VEC], const T *d_out, siz
         T v[N][VEC];
 #pragma unroll
         for (int u = 0; u < N; u++)
-            dh_seq::load_stream<T, VEC>(d_out + static_cast<size_t>(position(k + u < end ? k + u : end - 1)) * ld_out, v[u]);
+            dh_seq::load<T, VEC>(d_out + static_cast<size_t>(position(k + u < end ? k + u : end - 1)) * ld_out, v[u]);
 #pragma unroll
         for (int u = 0; u < N; u++)
             if (k + u < end)
@@ -458,12 +470,13 @@ __device__ __forceinline__ void write_row(const RowArgs<T> &a, size_t row, dh_se
 template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_kernel(RowArgs<T> a) {
     constexpr int AT_ONCE = 4;
     const unsigned lane = threadIdx.x % a.lanes, each = THREADS / a.lanes;
-    const size_t vec = static_cast<size_t>(blockIdx.y) * a.lanes + lane; // behind the last one: reads the last one, writes nothing
+    const size_t vec = static_cast<size_t>(blockIdx.x % a.slices) * a.lanes + lane; // behind the last one: reads the last one, writes nothing
     const size_t units = a.parts + (a.vocab + AT_ONCE - 1) / AT_ONCE;
     const dh_seq::Piece piece = dh_seq::piece<VEC>(vec, a.width);
     const T *column = a.d_out + piece.at;
     auto position = [&](size_t k) { return a.sorted[k]; };
-    for (size_t u = static_cast<size_t>(blockIdx.x) * each + threadIdx.x / a.lanes; u < units; u += static_cast<size_t>(gridDim.x) * each) {
+    const size_t stride = static_cast<size_t>(gridDim.x / a.slices) * each;
+    for (size_t u = static_cast<size_t>(blockIdx.x / a.slices) * each + threadIdx.x / a.lanes; u < units; u += stride) {
         if (u < a.parts) {
             const HotPart p = a.hot_parts[u];
             if (p.end == 0)
@@ -490,14 +503,14 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
 #pragma unroll
         for (int k = 0; k < AT_ONCE; k++) {
             at[k] = a.spans[row + k < a.vocab ? row + k : a.vocab - 1];
-            few &= at[k].y - at[k].x <= 1;
+            few &= at[k].y == ONE || at[k].y == at[k].x;
         }
         if (few) {
             T v[AT_ONCE][VEC];
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++)
                 if (at[k].y != at[k].x)
-                    dh_seq::load_stream<T, VEC>(column + static_cast<size_t>(a.sorted[at[k].x]) * a.ld_out, v[k]);
+                    dh_seq::load<T, VEC>(column + static_cast<size_t>(at[k].x) * a.ld_out, v[k]);
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++) {
                 const bool some = at[k].y != at[k].x;
@@ -512,11 +525,13 @@ template <typename T, int VEC> __global__ __launch_bounds__(THREADS) void rows_k
         } else {
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++) {
-                const unsigned b = at[k].x, e = at[k].y;
+                const bool one = at[k].y == ONE;
+                const unsigned b = one ? 0 : at[k].x, e = one ? 1 : at[k].y;
                 if (row + k >= a.vocab || (a.parts && e - b > HOT) || (b == e && a.accumulate))
                     continue;
                 double acc[VEC] = {};
-                add_rows<T, VEC>(acc, column, a.ld_out, b, e, position);
+                const unsigned *from = one ? &a.spans[row + k].x : a.sorted;
+                add_rows<T, VEC>(acc, column, a.ld_out, b, e, [&](size_t i) { return from[i]; });
                 write_row<T, VEC>(a, row + k, piece, acc, b != e ? a.scale : 0.0);
             }
         }
@@ -677,7 +692,7 @@ static inline BackwardPlan backward_plan(size_t n, size_t vocab, size_t width) {
     p.rows_each = dh_ceil_div(vocab, p.owners);
     while ((size_t(1) << p.row_bits) < p.rows_each)
         p.row_bits++;
-    p.how = p.rows_each > MOST_ROWS || n >= (size_t(1) << 32) ? BackwardPlan::PLAIN
+    p.how = p.rows_each > MOST_ROWS || n >= (size_t(1) << 32) - 1 ? BackwardPlan::PLAIN
             : n <= SCAN_TOKENS                                ? BackwardPlan::SCAN
                                                               : BackwardPlan::PARTITION;
     if (p.how == BackwardPlan::PLAIN)
@@ -716,6 +731,7 @@ static inline dh_status backward_sorted(dh_ctx *ctx, RowArgs<T> &r, SortArgs &a,
     while (r.lanes < DH_WAVE && r.lanes < r.width_vecs)
         r.lanes <<= 1;
     const size_t slices = dh_ceil_div(r.width_vecs, r.lanes);
+    r.slices = static_cast<unsigned>(slices);
     if (slices >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "embeddingBackward - extents exceed one launch");
     unsigned char *w = static_cast<unsigned char *>(work);
@@ -751,7 +767,7 @@ static inline dh_status backward_sorted(dh_ctx *ctx, RowArgs<T> &r, SortArgs &a,
     hipLaunchKernelGGL(sort, dim3(static_cast<unsigned>(p.owners)), dim3(SORT_THREADS), lds, ctx->stream, a);
     const size_t units = p.parts + dh_ceil_div(r.vocab, 4), grid = dh_ceil_div(units, THREADS / r.lanes);
     const size_t most = dh_ceil_div(static_cast<size_t>(ctx->num_cus) * 32, slices);
-    hipLaunchKernelGGL((rows_kernel<T, VEC>), dim3(static_cast<unsigned>(grid < most ? grid : most), static_cast<unsigned>(slices)),
+    hipLaunchKernelGGL((rows_kernel<T, VEC>), dim3(static_cast<unsigned>((grid < most ? grid : most) * slices)),
                        dim3(THREADS), 0, ctx->stream, r);
     if (p.hots)
         hipLaunchKernelGGL((join_kernel<T, VEC>), dim3(static_cast<unsigned>(p.hots), static_cast<unsigned>(dh_ceil_div(r.width_vecs, DH_WAVE))),

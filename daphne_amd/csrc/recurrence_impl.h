@@ -63,7 +63,17 @@ __device__ __forceinline__ void check_offsets(const Spans &sp, size_t num_seq, s
     }
 }
 
-// One thread per sequence and channel, one row after the other.
+// One thread per sequence and channel, one row after the other; the rows' values are requested SERIAL_AT_ONCE at a time, since
+// a thread that asks for one row only waits for memory at each (64 sequences of 64 rows, 4096 channels).
+constexpr int SERIAL_AT_ONCE = 8;
+// take(most, t): rows [t, t + most)
+template <class Take> __device__ __forceinline__ void by_rows(size_t rows, Take &&take) {
+    size_t done = 0;
+    for (; done + SERIAL_AT_ONCE <= rows; done += SERIAL_AT_ONCE)
+        take(std::integral_constant<int, SERIAL_AT_ONCE>{}, done);
+    for (; done < rows; done++)
+        take(std::integral_constant<int, 1>{}, done);
+}
 template <typename T>
 __global__ __launch_bounds__(THREADS) void forward_serial_kernel(T *res, size_t ld_res, T *last, size_t ld_last, const T *x, size_t ld_x,
                                                                  const T *z, size_t ld_z, const T *h0, size_t ld_h0, Spans sp,
@@ -75,13 +85,24 @@ __global__ __launch_bounds__(THREADS) void forward_serial_kernel(T *res, size_t 
         return;
     for (size_t s = blockIdx.y; s < num_seq; s += gridDim.y) {
         T h = h0 ? h0[s * ld_h0 + c] : T(0);
-        const size_t end = sp.at(s + 1);
-        for (size_t t = sp.at(s); t < end; t++) {
-            T f, w;
-            gates(z[t * ld_z + c], f, w);
-            h = f * h + w * x[t * ld_x + c];
-            res[t * ld_res + c] = h;
-        }
+        const size_t begin = sp.at(s), end = sp.at(s + 1);
+        by_rows(end > begin ? end - begin : 0, [&](auto most, size_t done) {
+            constexpr int N = decltype(most)::value;
+            T zv[N], xv[N];
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const size_t t = begin + done + u;
+                zv[u] = z[t * ld_z + c];
+                xv[u] = x[t * ld_x + c];
+            }
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                T f, w;
+                gates(zv[u], f, w);
+                h = f * h + w * xv[u];
+                res[(begin + done + u) * ld_res + c] = h;
+            }
+        });
         if (last)
             last[s * ld_last + c] = h;
     }
@@ -99,18 +120,30 @@ __global__ __launch_bounds__(THREADS) void backward_serial_kernel(T *d_x, size_t
         return;
     for (size_t s = blockIdx.y; s < num_seq; s += gridDim.y) {
         T carry = d_last ? d_last[s * ld_dl + c] : T(0); // f_{t+1} G_{t+1}
-        const size_t begin = sp.at(s);
-        for (size_t t = sp.at(s + 1); t > begin;) {
-            t--;
-            T f, w;
-            gates(z[t * ld_z + c], f, w);
-            const T g = d_out[t * ld_do + c] + carry;
-            const T before = t > begin ? h[(t - 1) * ld_h + c] : h0 ? h0[s * ld_h0 + c] : T(0);
-            const T xv = x[t * ld_x + c];
-            d_x[t * ld_dx + c] = w * g;
-            d_z[t * ld_dz + c] = g * (before - xv) * f * w;
-            carry = f * g;
-        }
+        const size_t begin = sp.at(s), end = sp.at(s + 1);
+        const T first = h0 ? h0[s * ld_h0 + c] : T(0);
+        by_rows(end > begin ? end - begin : 0, [&](auto most, size_t done) {
+            constexpr int N = decltype(most)::value;
+            T zv[N], xv[N], dv[N], hv[N];
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const size_t t = end - 1 - done - u;
+                zv[u] = z[t * ld_z + c];
+                xv[u] = x[t * ld_x + c];
+                dv[u] = d_out[t * ld_do + c];
+                hv[u] = h[(t > begin ? t - 1 : t) * ld_h + c]; // in front of the first row: the given state
+            }
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const size_t t = end - 1 - done - u;
+                T f, w;
+                gates(zv[u], f, w);
+                const T g = dv[u] + carry, before = t > begin ? hv[u] : first;
+                d_x[t * ld_dx + c] = w * g;
+                d_z[t * ld_dz + c] = g * (before - xv[u]) * f * w;
+                carry = f * g;
+            }
+        });
         if (d_h0)
             d_h0[s * ld_dh0 + c] = carry;
     }
