@@ -591,13 +591,16 @@ static inline dh_status check_sequences(const char *what, const long long *offse
     return DH_OK;
 }
 
-// Sequences short enough for a thread to walk: below this many rows each, all of one length.
-constexpr size_t SERIAL_ROWS = 8;
+// Sequences short enough for a thread to walk: up to this many rows each, all of one length. 64 sequences of 4096 channels, serial
+// and by chunks: 16 rows forward 9.4 and 20.8 us, 64 rows 43.6 and 52.3, backward 85 and 83; 128 rows backward 160 and 148. 8 sequences
+// of 512 channels, 64 rows: 7.4 and 9.7 us, backward 10.3 and 11.6; 128 rows backward 20.3 and 15.9.
+constexpr size_t SERIAL_ROWS = 64;
 
-// Shape of a pass: vectors (single values if there is not even one vector of channels), row chunks and channel blocks. Chunks are cut as tall as the registers allow,
-// and a quarter of that where so few workgroups would leave compute units idle.
+// Shape of a pass: vectors (single values if there is not even one vector of channels), row chunks and channel blocks. Chunks are
+// as tall as the registers allow, also where they are few: shorter ones make the chain longer (4096 rows of 256 channels:
+// 14.3 us, at a quarter of the height 21.7; 512 rows of 256 channels 11.7 and 10.1).
 struct Plan {
-    int vec, lanes, rows;
+    int vec, lanes;
     size_t blocks, chunks, padded;
 };
 template <typename T> Plan plan(size_t tokens, size_t channels, bool back) {
@@ -606,10 +609,8 @@ template <typename T> Plan plan(size_t tokens, size_t channels, bool back) {
     p.lanes = LANES;
     p.blocks = dh_ceil_div(channels, static_cast<size_t>(p.lanes) * p.vec);
     p.padded = p.blocks * p.lanes * p.vec;
-    const int tall = back ? ROWS_BACKWARD : ROWS_FORWARD;
-    const size_t groups = THREADS / p.lanes;
-    p.rows = p.blocks * dh_ceil_div(tokens, groups * tall) < 256 ? tall / 4 : tall;
-    p.chunks = dh_ceil_div(tokens, groups * p.rows);
+    const size_t tall = back ? ROWS_BACKWARD : ROWS_FORWARD, groups = THREADS / p.lanes;
+    p.chunks = dh_ceil_div(tokens, groups * tall);
     return p;
 }
 template <typename T> size_t plan_bytes(const Plan &p) {
@@ -652,14 +653,10 @@ dh_status scan(dh_ctx *ctx, const char *what, ScanArgs<T> &a, const Plan &p, voi
     const bool lines = at_lines(a.x, a.ld_x) && at_lines(a.z, a.ld_z) &&
                        (BACK ? at_lines(a.h, a.ld_h) && at_lines(a.d_out, a.ld_do) && at_lines(a.d_x, a.ld_dx) && at_lines(a.d_z, a.ld_dz)
                              : at_lines(a.res, a.ld_res));
-    if (p.vec > 1 && p.rows == R)
+    if (p.vec > 1)
         lines ? launch_scan<T, V, R, BACK, true>(ctx, a) : launch_scan<T, V, R, BACK, false>(ctx, a);
-    else if (p.vec > 1)
-        launch_scan<T, V, R / 4, BACK, false>(ctx, a);
-    else if (p.rows == R)
-        launch_scan<T, 1, R, BACK, false>(ctx, a);
     else
-        launch_scan<T, 1, R / 4, BACK, false>(ctx, a);
+        launch_scan<T, 1, R, BACK, false>(ctx, a);
     DH_CHECK_LAUNCH();
     return DH_OK;
 }
