@@ -217,7 +217,11 @@ constexpr int ROW_LIVE = 1, ROW_FIRST = 2, ROW_LAST = 4;
 template <typename T, int VEC, int LC, int R, bool BACK, bool LINES>
 __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
     constexpr int RG = THREADS / LC, ROWS = RG * R, CW = LC * VEC, NW = Words<T>::N, WAVES = THREADS / DH_WAVE;
-    constexpr int LB = RG < 16 ? RG : 16; // predecessors looked at in one round
+    // Predecessors looked at in the first round and in each later one, one a row group. What is read of them is traffic like any
+    // other: two, then eight, take 174 us where sixteen each time take 182 (backward, 32768 x 1024), and 330 for 360 (131072 x 512). In
+    // 64 bits few workgroups are in flight and rounds count for more: sixteen 178 us, two and eight 188 (32768 x 512).
+    constexpr int LB = sizeof(T) == 4 ? 8 : 16, FIRST = sizeof(T) == 4 ? 2 : 16;
+    static_assert(LB <= RG && FIRST <= LB);
     // ROW_*: which rows open the chain (take a given carry) and which close it (give their carry away), in scanning order
     constexpr int OPENS = BACK ? ROW_LAST : ROW_FIRST, CLOSES = BACK ? ROW_FIRST : ROW_LAST;
     __shared__ unsigned long long ticket_lds;
@@ -229,8 +233,10 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
     const unsigned tid = threadIdx.x, lc = tid % LC, g = tid / LC, wave = tid / DH_WAVE;
     unsigned long long ticket = blockIdx.x;
     if (a.ws) { // workgroups take chunks in the order in which they start, so that whoever is waited for is running
-        if (tid == 0)
-            ticket_lds = atomicAdd(a.ws, 1ull);
+        if (tid == 0) {
+            const unsigned long long t = atomicAdd(a.ws, 1ull), all = static_cast<unsigned long long>(a.blocks) * a.chunks;
+            ticket_lds = t < all ? t : t % all; // more: another call is in this workspace; whatever it does, indexes stay in range
+        }
         __syncthreads();
         ticket = ticket_lds;
     }
@@ -464,10 +470,11 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
             for (int e = 0; e < VEC; e++)
                 run[e] = T(1);
             bool done = false;
-            for (size_t back = 1;; back += LB) { // LB predecessors at a time, one a row group
+            unsigned width = FIRST;
+            for (size_t back = 1;; back += width, width = LB) {
                 T la[VEC], lb[VEC];
                 int got = 0; // 1: a composition, 2: a whole carry
-                if (g < LB && back + g <= chunk) {
+                if (g < width && back + g <= chunk) {
                     const unsigned long long *theirs = a.ws + 32 + (chunk - back - g) * 3 * NW * a.padded + c0;
                     // A predecessor runs (tickets) and publishes its composition without waiting for anybody. The bound is
                     // for a workspace that an overlapping call has overwritten: the call ends, and its results are NaN.
@@ -499,7 +506,7 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
                     }
                 }
                 __syncthreads(); // sA and sB have been read
-                if (g < LB) {
+                if (g < width) {
                     sOpen[g][lc] = got;
 #pragma unroll
                     for (int e = 0; e < VEC; e++) {
@@ -508,7 +515,7 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
                     }
                 }
                 __syncthreads();
-                for (unsigned q = 0; q < LB && !done; q++) {
+                for (unsigned q = 0; q < width && !done; q++) {
                     done = sOpen[q][lc] != 1; // a whole carry (the first chunk always has one)
 #pragma unroll
                     for (int e = 0; e < VEC; e++) {
