@@ -226,6 +226,12 @@ struct SortArgs {
     int *rec;
 };
 
+// A wavefront's LDS instructions execute in order; this keeps the compiler from reordering them.
+__device__ __forceinline__ void lds_in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // SCAN: owners read all tokens. Otherwise: their lists. Twice, to count and to place, eight steps of 64 requested together.
 template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(SortArgs a) {
     extern __shared__ unsigned sort_lds[];
@@ -243,44 +249,38 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
     const unsigned rows = a.vocab > owner ? (a.vocab - owner - 1) / (mask + 1) + 1 : 0;
     auto number = [&](unsigned r) { return owner + (r << a.owner_bits); };
     const size_t begin = SCAN ? 0 : a.starts[blockIdx.x * a.blocks], end = SCAN ? a.n : a.starts[(blockIdx.x + 1) * a.blocks];
-    // What a wavefront goes through, in order. Shares that are whole multiples of 4 KiB would have all wavefronts of all owners at the
-    // same few channels of the cache at a time (32768 tokens: 40 us).
-    size_t share = (end - begin + SORT_THREADS - 1) / SORT_THREADS * DH_WAVE;
-    share += share % 512 == 0 ? DH_WAVE : 0;
+    const size_t share = (end - begin + SORT_THREADS - 1) / SORT_THREADS * DH_WAVE; // what a wavefront goes through, in order
     const size_t w0 = begin + wave * share < end ? begin + wave * share : end, w1 = w0 + share < end ? w0 + share : end;
-    constexpr int EIGHT = 8;
-    auto walk = [&](auto &&take) { // take(row or ~0, position, whether there is one, token)
-        const size_t ld = SCAN ? a.ld_ids : 1;
-        const unsigned long long *src = SCAN ? reinterpret_cast<const unsigned long long *>(a.ids) : a.list;
-        const unsigned long long *p = src + (w0 + lane) * ld;
-        const unsigned len = static_cast<unsigned>(w1 - w0);
-        for (unsigned i0 = 0; i0 < len; i0 += EIGHT * DH_WAVE, p += EIGHT * DH_WAVE * ld) {
-            unsigned long long v[EIGHT];
-            if (len - i0 >= EIGHT * DH_WAVE) {
+    const size_t ld = SCAN ? a.ld_ids : 1;
+    const unsigned long long *src = (SCAN ? reinterpret_cast<const unsigned long long *>(a.ids) : a.list) + w0 * ld;
+    const unsigned len = static_cast<unsigned>(w1 - w0);
+    constexpr int AT_ONCE = 4; // twice as many are twice the instructions, which cost a short launch more: 2048 tokens 6.3 and 7.0 us
+    // AT_ONCE steps from i0: take(token or list entry, its place in the share, whether there is one). whole: all of them exist.
+    auto some_steps = [&](auto whole, unsigned i0, auto &&take) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        unsigned long long v[AT_ONCE];
+        const unsigned long long *p = src + (i0 + lane) * ld;
 #pragma unroll
-                for (int u = 0; u < EIGHT; u++)
-                    v[u] = p[u * DH_WAVE * ld];
-            } else {
-#pragma unroll
-                for (int u = 0; u < EIGHT; u++) { // behind the share: its last, not used (a guard would make each load wait for the one before)
-                    const unsigned i = i0 + u * DH_WAVE + lane;
-                    v[u] = src[(w0 + (i < len ? i : len - 1)) * ld];
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < EIGHT; u++) {
-                const unsigned i = i0 + u * DH_WAVE + lane;
-                const bool here = i < len;
-                if constexpr (SCAN) {
-                    const bool valid = here && v[u] < a.vocab; // a negative number is a large one
-                    const unsigned id = static_cast<unsigned>(v[u]);
-                    take(valid && (id & mask) == owner ? id >> a.owner_bits : ~0u, static_cast<unsigned>(w0) + i, here && !valid,
-                         valid && (id & mask) < owner);
-                } else {
-                    take(here ? static_cast<unsigned>(v[u] >> 32) : ~0u, static_cast<unsigned>(v[u]), false, false);
-                }
-            }
+        for (int u = 0; u < AT_ONCE; u++) { // behind the share: its last, not used (a guard would make each load wait for the one before)
+            const unsigned i = i0 + u * DH_WAVE + lane;
+            v[u] = WHOLE ? p[u * DH_WAVE * ld] : src[(i < len ? i : len - 1) * ld];
         }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            const unsigned i = i0 + u * DH_WAVE + lane;
+            take(v[u], i, WHOLE || i < len);
+        }
+    };
+    auto walk = [&](auto &&take) { // take(row or ~0, position)
+        for (unsigned i0 = 0; i0 < len; i0 += AT_ONCE * DH_WAVE)
+            some_steps(std::false_type{}, i0, [&](unsigned long long v, unsigned i, bool here) {
+                if constexpr (SCAN) {
+                    const unsigned id = static_cast<unsigned>(v);
+                    take(here && v < a.vocab && (id & mask) == owner ? id >> a.owner_bits : ~0u, static_cast<unsigned>(w0) + i);
+                } else {
+                    take(here ? static_cast<unsigned>(v >> 32) : ~0u, static_cast<unsigned>(v));
+                }
+            });
     };
     for (unsigned i = tid; i < VR * SORT_WAVES; i += SORT_THREADS)
         cnt[i] = 0;
@@ -289,21 +289,37 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
     __syncthreads();
     unsigned lower = 0;
     bool bad = false;
-    walk([&](unsigned r, unsigned position, bool wrong, bool before) {
-        lower += before;
-        bad |= wrong;
-        if constexpr (SCAN) {
-            const unsigned long long some = __ballot(r != ~0u);
-            if (some == 0)
-                return;
-            const unsigned at = have + __popcll(some & ((1ull << lane) - 1));
-            if (r != ~0u && at < FOUND)
-                found[wave][at] = (r << 16) | (position - static_cast<unsigned>(w0));
-            have += __popcll(some);
-        }
-        if (r != ~0u)
-            atomicAdd(&mine[r], 1u);
-    });
+    if constexpr (SCAN) {
+        auto find = [&](unsigned long long v, unsigned i, bool here) {
+            const bool valid = here && v < a.vocab; // a negative number is a large one
+            const unsigned id = static_cast<unsigned>(v);
+            const bool hit = valid && (id & mask) == owner;
+            lower += valid && (id & mask) < owner;
+            bad |= here && !valid;
+            const unsigned long long some = __ballot(hit);
+            if (some != 0) {
+                const unsigned at = have + __popcll(some & ((1ull << lane) - 1));
+                if (hit && at < FOUND)
+                    found[wave][at] = ((id >> a.owner_bits) << 16) | i;
+                have += __popcll(some);
+            }
+        };
+        unsigned i0 = 0;
+        for (; i0 + AT_ONCE * DH_WAVE <= len; i0 += AT_ONCE * DH_WAVE)
+            some_steps(std::true_type{}, i0, find);
+        if (i0 < len)
+            some_steps(std::false_type{}, i0, find);
+    }
+    if (SCAN && have <= FOUND) {
+        lds_in_order();
+        for (unsigned i = lane; i < have; i += DH_WAVE)
+            atomicAdd(&mine[found[wave][i] >> 16], 1u);
+    } else {
+        walk([&](unsigned r, unsigned) {
+            if (r != ~0u)
+                atomicAdd(&mine[r], 1u);
+        });
+    }
     if constexpr (SCAN) {
         dh_butterfly(DH_WAVE, [&](auto peer) { lower += peer(lower); });
         if (lane == 0)
@@ -393,7 +409,7 @@ template <bool SCAN> __global__ __launch_bounds__(SORT_THREADS) void sort_kernel
             place(i + lane < have ? f >> 16 : ~0u, static_cast<unsigned>(w0) + (f & 0xffffu));
         }
     } else {
-        walk([&](unsigned r, unsigned position, bool, bool) {
+        walk([&](unsigned r, unsigned position) {
             if (!SCAN || __ballot(r != ~0u) != 0)
                 place(r, position);
         });
