@@ -70,7 +70,9 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, const T *table, size_t voc
     while (lpr < THREADS && lpr < wv)
         lpr <<= 1;
     const size_t gx = dh_ceil_div(n, THREADS / lpr);
-    const bool four = wv > lpr && gx * dh_ceil_div(wv, lpr) >= 4096; // several vectors in flight a thread once the workgroups fill the device
+    // Rows of more vectors than a workgroup has threads: four in flight a thread (16384 x 2048 in 40 us, with one 47); shorter rows
+    // have none to give it (65536 x 256: 18 us, with four 22).
+    const bool four = wv > lpr;
     const size_t gy = dh_ceil_div(wv, static_cast<size_t>(lpr) * (four ? 4 : 1));
     if (gx >= (size_t(1) << 31) || gy >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "embeddingForward - extents exceed one launch");
@@ -151,7 +153,7 @@ __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size
 // [b / HOT, e / HOT), and never fewer than it has parts (a token with c > HOT positions has ceil(c / PART) <= c / HOT), and in
 // the same way the slots [b / PART, e / PART) for its tokens of several parts. It marks those that it does not use.
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / DH_WAVE;
-constexpr unsigned HOT = 8, PART = 32;
+constexpr unsigned HOT = 8, PART = 64;
 constexpr size_t SCAN_TOKENS = 65536;   // up to here every owner reads all tokens
 constexpr unsigned KEEP = 4096;                   // positions an owner keeps in LDS
 constexpr unsigned FOUND = 512;                   // positions a wavefront finds at once

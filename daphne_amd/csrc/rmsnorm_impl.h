@@ -242,29 +242,22 @@ template <int VEC, class Use> static inline void by_width(size_t vecs, Use &&use
     else if (vecs <= 256)
         use(Shape<64, 4>{});
     else if (vecs <= 512)
-        use(Shape<256, 2>{});
+        use(Shape<512, 1>{});
     else if (vecs <= 768)
         use(Shape<256, 3>{});
     else if (vecs <= 1024)
         use(Shape<256, 4>{});
     else if (vecs <= 2048)
         use(Shape<1024, 2>{});
+    else if (vecs <= 3 * 1024)
+        use(Shape<1024, 3>{});
     else if (vecs <= 4096)
         use(Shape<1024, 4>{});
     else
         use(Shape<1024, 0>{});
 }
 template <typename T, int VEC, bool Q8> static inline void forward_by_width(dh_ctx *ctx, const ForwardArgs<T> &a) {
-    // few rows: more threads on each, since nothing else hides what a thread waits for
-    const size_t vecs = dh_ceil_div(a.cols, VEC);
-    if (VEC > 1 && a.rows < static_cast<size_t>(ctx->num_cus) && vecs > 256 && vecs <= 2048) {
-        if (vecs <= 1024)
-            launch_forward<T, VEC, 1024, 1, Q8>(ctx, a);
-        else
-            launch_forward<T, VEC, 1024, 2, Q8>(ctx, a);
-        return;
-    }
-    by_width<VEC>(vecs, [&](auto shape) { launch_forward<T, VEC, decltype(shape)::TPR, decltype(shape)::KV, Q8>(ctx, a); });
+    by_width<VEC>(dh_ceil_div(a.cols, VEC), [&](auto shape) { launch_forward<T, VEC, decltype(shape)::TPR, decltype(shape)::KV, Q8>(ctx, a); });
 }
 
 template <typename T, bool Q8> dh_status forward(dh_ctx *ctx, const ForwardArgs<T> &a) {
