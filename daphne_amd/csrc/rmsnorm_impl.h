@@ -6,8 +6,9 @@
 //           out of the codes, which therefore do not depend on how the mean was summed
 //   backward: d_h = inv (gamma d_y - h inv^2 mean(gamma d_y h)) + d_sum,   d_gamma = sum over rows of d_y h inv
 //
-// All of it moves whole rows once and is bound by memory. A row is held in the registers of TPR threads (64, 256 or
-// 1024) between its reduction and its result; rows too wide for that are read a second time. Sums over a row are kept in
+// All of it moves whole rows once and is bound by memory: forward 16384 x 4096 with residual and sum 186 us (1.07 GB, 5.8 TB/s; a
+// copy of as much takes 205), backward 8192 x 2560 59 us (335 MB, 5.7 TB/s). A row is held in the registers of TPR threads
+// between its reduction and its result; rows too wide for that are read a second time. Sums over a row are kept in
 // 64 bits: the conversions hide behind the loads, and a row of any length keeps T's precision.
 #pragma once
 
@@ -227,34 +228,31 @@ template <typename T, int VEC, int TPR, int KV, bool Q8> static inline void laun
                        ctx->stream, a);
 }
 
-// The shape of a row of so many vectors: calls use(TPR, KV) as integral constants. As few threads a row as hold it with up to
-// four vectors each; KV = 0 beyond that.
+// The shape of a row of so many vectors: calls use(Shape), the first one that holds the row; KV = 0 holds none and takes any.
+// Measured in 32 bits, forward with 32 Mi values (residual and sum kept: 512 MiB moved) and backward with 16 Mi:
+//   128 vectors: 64 threads of 2 94 and 47 us, 256 of 1 99 and 78             256: 64 of 4 93 and 49, 256 of 1 92 and 50
+//   512: 512 of 1 90 and 46, 256 of 2 92 and 47, 1024 of 1 103 and 68         640: 256 of 3 93 and 48, 512 of 2 92 and 50
+//   1024: 256 of 4 94 and 47, 512 of 2 92 and 49, 1024 of 1 90 and 55         2048: 1024 of 2 94 and 53, 512 of 4 95 and 54
+//   4096: 1024 of 4 105 and 103, any length 112 and 100                       2750, 4096 rows backward: 1024 of 3 155, of 4 280
+// Backward, 1024 threads of 4 keep more than their registers hold; in 64 bits they still beat rows of any length, 120 and 177 us
+// (2048 x 8192).
 template <int A, int B> struct Shape {
     static constexpr int TPR = A, KV = B;
 };
+template <class Use, class S, class... Wider> static inline void first_fit(size_t vecs, Use &&use, S shape, Wider... wider) {
+    if constexpr (sizeof...(Wider) == 0)
+        use(shape);
+    else if (vecs <= static_cast<size_t>(S::TPR) * S::KV)
+        use(shape);
+    else
+        first_fit(vecs, use, wider...);
+}
 template <int VEC, class Use> static inline void by_width(size_t vecs, Use &&use) {
     if constexpr (VEC == 1) // rows shorter than a vector
         use(Shape<64, 1>{});
-    else if (vecs <= 64)
-        use(Shape<64, 1>{});
-    else if (vecs <= 128)
-        use(Shape<64, 2>{});
-    else if (vecs <= 256)
-        use(Shape<64, 4>{});
-    else if (vecs <= 512)
-        use(Shape<512, 1>{});
-    else if (vecs <= 768)
-        use(Shape<256, 3>{});
-    else if (vecs <= 1024)
-        use(Shape<256, 4>{});
-    else if (vecs <= 2048)
-        use(Shape<1024, 2>{});
-    else if (vecs <= 3 * 1024)
-        use(Shape<1024, 3>{});
-    else if (vecs <= 4096)
-        use(Shape<1024, 4>{});
     else
-        use(Shape<1024, 0>{});
+        first_fit(vecs, use, Shape<64, 1>{}, Shape<64, 2>{}, Shape<64, 4>{}, Shape<512, 1>{}, Shape<256, 3>{}, Shape<256, 4>{}, Shape<1024, 2>{},
+                  Shape<1024, 3>{}, Shape<1024, 4>{}, Shape<1024, 0>{});
 }
 template <typename T, int VEC, bool Q8> static inline void forward_by_width(dh_ctx *ctx, const ForwardArgs<T> &a) {
     by_width<VEC>(dh_ceil_div(a.cols, VEC), [&](auto shape) { launch_forward<T, VEC, decltype(shape)::TPR, decltype(shape)::KV, Q8>(ctx, a); });
@@ -303,7 +301,9 @@ template <typename T> struct BackwardArgs {
 };
 
 // Rows and d_gamma together: a workgroup goes through every gridDim.x-th row (four rows at a time where a wavefront holds one)
-// and keeps the sums of d_y h inv of its columns in registers, which it leaves in partials[blockIdx.x].
+// and keeps the sums of d_y h inv of its columns in registers, which it leaves in partials[blockIdx.x]. With the rows read a second
+// time for d_gamma, which is what remains for the widest ones, 8192 x 2560 takes 95 us instead of 59. What a row reads is
+// requested past the caches: 8192 x 4096 93 us, by way of them 104; batches that fit into them lose (2048 x 2560: 22.5 and 19.9).
 template <typename T, int VEC, int TPR, int KV>
 __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kernel(BackwardArgs<T> a, T *partials) {
     constexpr int WG = TPR > THREADS ? TPR : THREADS, RPW = WG / TPR;
