@@ -892,3 +892,72 @@ def test_two_contexts_on_streams_of_their_own(ctx):
             c.sync()
             c.destroy()
 
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(5, 1500), (3, 2048), (600, 520), (2, 9999), (3, 12288), (2, 12289), (4, 5000)])
+def test_rms_norm_widths_between(ctx, dt, rows, cols):
+    test_rms_norm_forward(ctx, dt, rows, cols)
+    test_rms_norm_backward(ctx, dt, rows, cols)
+    test_rms_norm_forward_views_and_in_place(ctx, dt, rows, cols)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("seqs,length,channels", [(64, 64, 40), (2, 65, 33), (3, 23, 270), (70, 8, 5), (1, 63, 1), (9, 16, 256)])
+def test_gated_recurrence_short_sequences(ctx, dt, seqs, length, channels):
+    check_recurrence(ctx, dt, [length] * seqs, channels, even=True)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n,vocab,width", [(3000, 100000, 1024), (3000, 100000, 65), (66000, 100000, 7), (65536, 70, 9), (65537, 70, 9), (9000, 20000, 1100)])
+def test_embedding_backward_of_rare_tokens(ctx, dt, n, vocab, width):
+    """Most tokens occur once or not at all; one fills its owner's lists."""
+    rng = np.random.default_rng(n + width)
+    ids, d_out = rng.integers(0, vocab, (n, 1)), rng.standard_normal((n, width)).astype(dt)
+    ids[rng.random(n) < 0.1] = 256 % vocab
+    want, mag = embedding_gradient(ids, d_out, vocab, 1.0)
+    tol = (n + 2) * 2.0**-53 * mag + U(dt) * np.abs(want) * 1.001  # as above
+    near(embeddingBackward(None, D(ctx, d_out), D(ctx, ids), vocab, 1.0, ctx).to_numpy(), want, tol, "gradient")
+
+
+def test_two_captured_graphs_of_one_workspace_in_turn(ctx):
+    """Calls that do not overlap may share a workspace, whatever the one before left in it."""
+    torch = pytest.importorskip("torch")
+    c = HIPContext(0)
+    try:
+        stream = torch.cuda.Stream()
+        rng = np.random.default_rng(45)
+        c.set_stream(stream.cuda_stream)
+        sizes = [(3000, 48, 90), (7000, 20, 400)]
+        need = max(max(embeddingBackwardWorkspaceBytes(n, v, w, F32), rmsNormBackwardWorkspaceBytes(n, w, F32), gatedRecurrenceWorkspaceBytes(n, 1, w, F32))
+                   for n, w, v in sizes)
+        ws = DenseMatrix(c, 1, need, np.uint8)
+        sets = []
+        for n, w, v in sizes:
+            x, ids, inv = D(c, rng.standard_normal((n, w)).astype(F32)), D(c, token_ids(rng, n, v)), D(c, rng.random((n, 1)).astype(F32))
+            outs = [DenseMatrix(c, n, w, F32), DenseMatrix(c, 1, w, F32), DenseMatrix(c, n, w, F32), DenseMatrix(c, 1, w, F32), DenseMatrix(c, v, w, F32)]
+
+            def run(o, ws, x=x, ids=ids, inv=inv, v=v):
+                gatedRecurrenceForward(o[0], o[1], x, x, None, None, 1, c, workspace=ws)
+                rmsNormBackward(o[2], o[3], x, inv, None, o[0], None, c, workspace=ws)
+                embeddingBackward(o[4], o[2], ids, v, 0.5, c, workspace=ws)
+
+            sets.append((run, outs, torch.cuda.CUDAGraph()))
+        c.sync()
+        with c.deferred_checks():
+            for run, outs, graph in sets:
+                with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+                    run(outs, ws)
+        for k in range(4):
+            for run, outs, graph in sets if k % 2 else sets[::-1]:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            for run, outs, graph in sets:
+                plain = [DenseMatrix(c, m.rows, m.cols, F32) for m in outs]
+                run(plain, None)
+                for a, b in zip(outs, plain):
+                    np.testing.assert_array_equal(a.to_numpy(), b.to_numpy())
+        c.check_deferred()
+        sets.clear()
+    finally:
+        c.sync()
+        c.destroy()
