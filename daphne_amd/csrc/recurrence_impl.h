@@ -15,7 +15,7 @@
 // result), which makes it bound by memory: a workgroup composes its chunk, publishes the composition, looks back over its
 // predecessors' until it meets a carry that is already whole, publishes its own, and writes its rows. 32768 rows forward,
 // 2048 channels: 158 us (806 MB, 5.1 TB/s); backward, 1024 channels: 174 us (806 MB, 4.6 TB/s); a copy of as much: 155 us.
-// 64 bits: 100001 x 96 in 73 us (230 MB, 3.2 TB/s), 58 without looking back: two wavefronts a SIMD hide less of it.
+// 64 bits: 100001 x 96 in 64 us (230 MB, 3.6 TB/s): two wavefronts a SIMD hide less of the looking back and of the exponentials.
 #pragma once
 
 #include "seq_common.h"
@@ -221,8 +221,8 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
     constexpr int RG = THREADS / LC, ROWS = RG * R, CW = LC * VEC, NW = Words<T>::N, WAVES = THREADS / DH_WAVE;
     // Predecessors looked at in the first round and in each later one, one a row group. What is read of them is traffic like any
     // other: two, then eight, take 174 us where sixteen each time take 182 (backward, 32768 x 1024), and 330 for 360 (131072 x 512). In
-    // 64 bits few workgroups are in flight and rounds count for more: sixteen 178 us, two and eight 188 (32768 x 512).
-    constexpr int LB = sizeof(T) == 4 ? 8 : 16, FIRST = sizeof(T) == 4 ? 2 : 16;
+    // 64 bits fewer workgroups are in flight and eight are no worse: 63.9 us, four at first 64.5, sixteen 65.3 (100001 x 96).
+    constexpr int LB = 8, FIRST = sizeof(T) == 4 ? 2 : 8;
     static_assert(LB <= RG && FIRST <= LB);
     // ROW_*: which rows open the chain (take a given carry) and which close it (give their carry away), in scanning order
     constexpr int OPENS = BACK ? ROW_LAST : ROW_FIRST, CLOSES = BACK ? ROW_FIRST : ROW_LAST;
@@ -586,10 +586,13 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
 //   flight, so tall and narrow is cheap: 16 lanes 191 and 219 us. 4 lanes take less than a memory line of a row: 273 and 250.
 //   8 rows a thread forward (4 backward, which holds twice as many arrays): 167 registers, 3 wavefronts a SIMD. 16 (8) rows leave
 //   one: 195 and 193 us; 4 rows forward 238 us.
+//   In 64 bits 12 and 7 rows, which leave two wavefronts: 64 us forward (100001 x 96) and 159 backward (32768 x 512); 8 and 4 rows 73
+//   and 178, 6 and 3, for three wavefronts, 77 and 182, 14 rows, for one, 77.
 // Without any look-back (sequences as long as a chunk) the same rows take 147 and 157 us, a plain copy of as many bytes 155.
 // Rows that do not begin at memory lines (2047 and 1023 channels) have every line in two chunks: 237 and 250 us by way of the
 // caches, 315 and 308 past them.
-constexpr int ROWS_FORWARD = 8, ROWS_BACKWARD = 4, LANES = 8;
+constexpr int LANES = 8;
+template <typename T> constexpr int rows_of(bool back) { return sizeof(T) == 4 ? (back ? 4 : 8) : (back ? 7 : 12); }
 
 // What every entry point checks of its sequences.
 static inline dh_status check_sequences(const char *what, const long long *offsets, size_t ld_offsets, size_t num_seq, size_t tokens) {
@@ -619,7 +622,7 @@ template <typename T> Plan plan(size_t tokens, size_t channels, bool back) {
     p.lanes = LANES;
     p.blocks = dh_ceil_div(channels, static_cast<size_t>(p.lanes) * p.vec);
     p.padded = p.blocks * p.lanes * p.vec;
-    const size_t tall = back ? ROWS_BACKWARD : ROWS_FORWARD, groups = THREADS / p.lanes;
+    const size_t tall = rows_of<T>(back), groups = THREADS / p.lanes;
     p.chunks = dh_ceil_div(tokens, groups * tall);
     return p;
 }
@@ -659,7 +662,7 @@ dh_status scan(dh_ctx *ctx, const char *what, ScanArgs<T> &a, const Plan &p, voi
         hipLaunchKernelGGL(clear_kernel, dim3(static_cast<unsigned>(grid < 2048 ? grid : 2048)), dim3(THREADS), 0, ctx->stream,
                            static_cast<ulonglong2 *>(work), n);
     }
-    constexpr int V = dh_vec<T>::N, R = BACK ? ROWS_BACKWARD : ROWS_FORWARD;
+    constexpr int V = dh_vec<T>::N, R = rows_of<T>(BACK);
     const bool lines = at_lines(a.x, a.ld_x) && at_lines(a.z, a.ld_z) &&
                        (BACK ? at_lines(a.h, a.ld_h) && at_lines(a.d_out, a.ld_do) && at_lines(a.d_x, a.ld_dx) && at_lines(a.d_z, a.ld_dz)
                              : at_lines(a.res, a.ld_res));
