@@ -154,35 +154,59 @@ __global__ __launch_bounds__(THREADS) void backward_serial_kernel(T *d_x, size_t
 // ---------------------------------------------------------------------------------------
 // one pass over chunks of rows
 // ---------------------------------------------------------------------------------------
-// A published value: each 32 bits of it in a word of their own beside the mark that they are there, so that a reader needs
-// no fence between a flag and the value. Zero: not there yet.
-template <typename T> struct Words {
-    static constexpr int N = sizeof(T) / 4;
-};
-template <typename T> __device__ __forceinline__ void publish(unsigned long long *p, size_t stride, T v) {
-    if constexpr (sizeof(T) == 4) {
-        __hip_atomic_store(p, (static_cast<unsigned long long>(__builtin_bit_cast(unsigned, v)) << 32) | 1ull, __ATOMIC_RELAXED,
+// What a chunk publishes for a channel: its map (A, B), later the whole carry behind it. Every word says itself whether it is there
+// (zero: not yet), so that a reader needs no fence between a flag and a value.
+//   32 bits: one word, A above B. A is never negative, so its sign bit marks a map; 1 in its place marks a whole carry, which takes
+//   the map's place. With words of their own for A, B and the carry, backward 32768 x 1024 takes 174 us.
+//   64 bits: A, B and the carry two words each, 32 bits of the value above the mark.
+template <typename T> struct Published;
+template <> struct Published<float> {
+    static constexpr int WORDS = 1;
+    static __device__ __forceinline__ void store(unsigned long long *p, unsigned hi, float lo) {
+        __hip_atomic_store(p, (static_cast<unsigned long long>(hi) << 32) | __builtin_bit_cast(unsigned, lo), __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
-    } else {
+    }
+    static __device__ __forceinline__ void map(unsigned long long *p, size_t, float A, float B) {
+        store(p, __builtin_bit_cast(unsigned, A) | 0x80000000u, B);
+    }
+    static __device__ __forceinline__ void whole(unsigned long long *p, size_t, float carry) { store(p, 1, carry); }
+    // 0: not there, 1: a map, 2: a whole carry, in B
+    static __device__ __forceinline__ int read(const unsigned long long *p, size_t, float &A, float &B) {
+        const unsigned long long v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const unsigned hi = static_cast<unsigned>(v >> 32);
+        A = __builtin_bit_cast(float, hi & 0x7fffffffu);
+        B = __builtin_bit_cast(float, static_cast<unsigned>(v));
+        return hi >> 31 ? 1 : hi != 0 ? 2 : 0;
+    }
+};
+template <> struct Published<double> {
+    static constexpr int WORDS = 6;
+    static __device__ __forceinline__ void store(unsigned long long *p, size_t stride, double v) {
         const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
         __hip_atomic_store(p, (b << 32) | 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(p + stride, (b & 0xffffffff00000000ull) | 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-}
-template <typename T> __device__ __forceinline__ bool published(const unsigned long long *p, size_t stride, T &v) {
-    const unsigned long long a = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if constexpr (sizeof(T) == 4) {
-        v = __builtin_bit_cast(T, static_cast<unsigned>(a >> 32));
-        return a != 0;
-    } else {
+    static __device__ __forceinline__ bool load(const unsigned long long *p, size_t stride, double &v) {
+        const unsigned long long a = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const unsigned long long b = __hip_atomic_load(p + stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        v = __builtin_bit_cast(T, (a >> 32) | (b & 0xffffffff00000000ull));
+        v = __builtin_bit_cast(double, (a >> 32) | (b & 0xffffffff00000000ull));
         return a != 0 && b != 0;
     }
-}
+    static __device__ __forceinline__ void map(unsigned long long *p, size_t stride, double A, double B) {
+        store(p, stride, A);
+        store(p + 2 * stride, stride, B);
+    }
+    static __device__ __forceinline__ void whole(unsigned long long *p, size_t stride, double carry) { store(p + 4 * stride, stride, carry); }
+    static __device__ __forceinline__ int read(const unsigned long long *p, size_t stride, double &A, double &B) {
+        if (load(p + 4 * stride, stride, B))
+            return 2;
+        const bool a = load(p, stride, A), b = load(p + 2 * stride, stride, B);
+        return a && b;
+    }
+};
 
-// The workspace: a ticket counter (256 bytes), then for every chunk the three published values A, B and the whole carry,
-// each a row of `padded` channels (times the words of a value). Cleared by clear_kernel before each pass.
+// The workspace: a ticket counter (256 bytes), then for every chunk what it publishes, WORDS rows of `padded` channels. Cleared by
+// clear_kernel before each pass.
 static __global__ __launch_bounds__(THREADS) void clear_kernel(ulonglong2 *p, size_t n) {
     for (size_t i = static_cast<size_t>(blockIdx.x) * THREADS + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * THREADS)
         p[i] = ulonglong2{0, 0};
@@ -218,7 +242,7 @@ constexpr int ROW_LIVE = 1, ROW_FIRST = 2, ROW_LAST = 4;
 // touched by two workgroups and none needs to stay in a cache.
 template <typename T, int VEC, int LC, int R, bool BACK, bool LINES>
 __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
-    constexpr int RG = THREADS / LC, ROWS = RG * R, CW = LC * VEC, NW = Words<T>::N, WAVES = THREADS / DH_WAVE;
+    constexpr int RG = THREADS / LC, ROWS = RG * R, CW = LC * VEC, NW = Published<T>::WORDS, WAVES = THREADS / DH_WAVE;
     // Predecessors looked at in the first round and in each later one, one a row group. What is read of them is traffic like any
     // other: two, then eight, take 174 us where sixteen each time take 182 (backward, 32768 x 1024), and 330 for 360 (131072 x 512). In
     // 64 bits fewer workgroups are in flight and eight are no worse: 63.9 us, four at first 64.5, sixteen 65.3 (100001 x 96).
@@ -445,8 +469,7 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
     T carry[VEC] = {}; // what enters the chunk; a chunk that no carry enters takes 0, and no row uses it
     if (a.ws) {
         const bool alone = chunk == 0 || (flags[0] & OPENS); // the same in all threads
-        unsigned long long *mine = a.ws + 32 + chunk * 3 * NW * a.padded + c0;
-        const size_t field = static_cast<size_t>(NW) * a.padded;
+        unsigned long long *mine = a.ws + 32 + chunk * NW * a.padded + c0;
         const bool publisher = g == RG - 1 && chunk + 1 < a.chunks;
         const bool copen = popen || open;
         T cA[VEC], cB[VEC];
@@ -458,12 +481,10 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
         if (publisher) {
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                if (copen || alone) {
-                    publish(mine + 2 * field + e, a.padded, cB[e]);
-                } else {
-                    publish(mine + e, a.padded, cA[e]);
-                    publish(mine + field + e, a.padded, cB[e]);
-                }
+                if (copen || alone)
+                    Published<T>::whole(mine + e, a.padded, cB[e]);
+                else
+                    Published<T>::map(mine + e, a.padded, cA[e], cB[e]);
             }
         }
         if (!alone) {
@@ -477,27 +498,19 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
                 T la[VEC], lb[VEC];
                 int got = 0; // 1: a composition, 2: a whole carry
                 if (g < width && back + g <= chunk) {
-                    const unsigned long long *theirs = a.ws + 32 + (chunk - back - g) * 3 * NW * a.padded + c0;
+                    const unsigned long long *theirs = a.ws + 32 + (chunk - back - g) * NW * a.padded + c0;
                     // A predecessor runs (tickets) and publishes its composition without waiting for anybody. The bound is
                     // for a workspace that an overlapping call has overwritten: the call ends, and its results are NaN.
                     for (unsigned tries = 0; got == 0 && tries < (1u << 20); tries++) {
-                        bool all = true;
-#pragma unroll
-                        for (int e = 0; e < VEC; e++)
-                            all &= published(theirs + 2 * field + e, a.padded, lb[e]);
-                        if (all) {
-                            got = 2;
-                            break;
-                        }
-                        all = true;
+                        bool map = true, whole = true;
 #pragma unroll
                         for (int e = 0; e < VEC; e++) {
-                            all &= published(theirs + e, a.padded, la[e]);
-                            all &= published(theirs + field + e, a.padded, lb[e]);
+                            const int is = Published<T>::read(theirs + e, a.padded, la[e], lb[e]);
+                            map &= is == 1;
+                            whole &= is == 2;
                         }
-                        if (all)
-                            got = 1;
-                        else
+                        got = whole ? 2 : map; // of some channels a map, of others the carry that is taking its place: once more
+                        if (got == 0)
                             __builtin_amdgcn_s_sleep(1);
                     }
                     if (got == 0) {
@@ -531,7 +544,7 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
             if (publisher && !copen)
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
-                    publish(mine + 2 * field + e, a.padded, cA[e] * carry[e] + cB[e]);
+                    Published<T>::whole(mine + e, a.padded, cA[e] * carry[e] + cB[e]);
         }
     }
     if (!on)
@@ -627,7 +640,7 @@ template <typename T> Plan plan(size_t tokens, size_t channels, bool back) {
     return p;
 }
 template <typename T> size_t plan_bytes(const Plan &p) {
-    return p.chunks > 1 ? 256 + p.chunks * 3 * Words<T>::N * p.padded * sizeof(unsigned long long) : 0;
+    return p.chunks > 1 ? 256 + p.chunks * Published<T>::WORDS * p.padded * sizeof(unsigned long long) : 0;
 }
 
 // Enough for both directions.
