@@ -14,7 +14,7 @@
 // scan_kernel does it in one pass over the data (a chunk's inputs stay in registers from its composition to its
 // result), which makes it bound by memory: a workgroup composes its chunk, publishes the composition, looks back over its
 // predecessors' until it meets a carry that is already whole, publishes its own, and writes its rows. 32768 rows forward,
-// 2048 channels: 158 us (806 MB, 5.1 TB/s); backward, 1024 channels: 174 us (806 MB, 4.6 TB/s); a copy of as much: 155 us.
+// 2048 channels: 154 us (806 MB, 5.2 TB/s); backward, 1024 channels: 169 us (806 MB, 4.8 TB/s); a copy of as much: 155 us.
 // 64 bits: 100001 x 96 in 64 us (230 MB, 3.6 TB/s): two wavefronts a SIMD hide less of the looking back and of the exponentials.
 #pragma once
 
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(THREADS) void backward_serial_kernel(T *d_x, size_t
 // (zero: not yet), so that a reader needs no fence between a flag and a value.
 //   32 bits: one word, A above B. A is never negative, so its sign bit marks a map; 1 in its place marks a whole carry, which takes
 //   the map's place. With words of their own for A, B and the carry, backward 32768 x 1024 takes 174 us.
-//   64 bits: A, B and the carry two words each, 32 bits of the value above the mark.
+//   64 bits: A with the same mark in a word, B and the carry two words each, 32 bits of the value above the mark.
 template <typename T> struct Published;
 template <> struct Published<float> {
     static constexpr int WORDS = 1;
@@ -180,7 +180,7 @@ template <> struct Published<float> {
     }
 };
 template <> struct Published<double> {
-    static constexpr int WORDS = 6;
+    static constexpr int WORDS = 5;
     static __device__ __forceinline__ void store(unsigned long long *p, size_t stride, double v) {
         const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
         __hip_atomic_store(p, (b << 32) | 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -193,15 +193,17 @@ template <> struct Published<double> {
         return a != 0 && b != 0;
     }
     static __device__ __forceinline__ void map(unsigned long long *p, size_t stride, double A, double B) {
-        store(p, stride, A);
-        store(p + 2 * stride, stride, B);
+        __hip_atomic_store(p, __builtin_bit_cast(unsigned long long, A) | (1ull << 63), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        store(p + stride, stride, B);
     }
-    static __device__ __forceinline__ void whole(unsigned long long *p, size_t stride, double carry) { store(p + 4 * stride, stride, carry); }
+    static __device__ __forceinline__ void whole(unsigned long long *p, size_t stride, double carry) { store(p + 3 * stride, stride, carry); }
     static __device__ __forceinline__ int read(const unsigned long long *p, size_t stride, double &A, double &B) {
-        if (load(p + 4 * stride, stride, B))
-            return 2;
-        const bool a = load(p, stride, A), b = load(p + 2 * stride, stride, B);
-        return a && b;
+        const unsigned long long a = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        double w;
+        const bool b = load(p + stride, stride, B), c = load(p + 3 * stride, stride, w);
+        A = __builtin_bit_cast(double, a & 0x7fffffffffffffffull);
+        B = c ? w : B;
+        return c ? 2 : a != 0 && b;
     }
 };
 
@@ -244,9 +246,9 @@ template <typename T, int VEC, int LC, int R, bool BACK, bool LINES>
 __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
     constexpr int RG = THREADS / LC, ROWS = RG * R, CW = LC * VEC, NW = Published<T>::WORDS, WAVES = THREADS / DH_WAVE;
     // Predecessors looked at in the first round and in each later one, one a row group. What is read of them is traffic like any
-    // other: two, then eight, take 174 us where sixteen each time take 182 (backward, 32768 x 1024), and 330 for 360 (131072 x 512). In
-    // 64 bits fewer workgroups are in flight and eight are no worse: 63.9 us, four at first 64.5, sixteen 65.3 (100001 x 96).
-    constexpr int LB = 8, FIRST = sizeof(T) == 4 ? 2 : 8;
+    // other: two, then eight, take 169 us where four, then eight, take 170 (backward, 32768 x 1024), and 323 for 332 (131072 x 512); in
+    // 64 bits, with fewer workgroups in flight, four at first 63.8 and eight 64.5 us (100001 x 96).
+    constexpr int LB = 8, FIRST = sizeof(T) == 4 ? 2 : 4;
     static_assert(LB <= RG && FIRST <= LB);
     // ROW_*: which rows open the chain (take a given carry) and which close it (give their carry away), in scanning order
     constexpr int OPENS = BACK ? ROW_LAST : ROW_FIRST, CLOSES = BACK ? ROW_FIRST : ROW_LAST;
@@ -594,7 +596,7 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
 
 // Shape of a chunk, chosen by measurement (32768 rows; forward 2048 channels in 8 sequences, backward 1024 in 5):
 //   8 lanes of 16-byte vectors a row, so that a chunk is 128 bytes wide and 256 (backward 128) rows tall: 158 and 181 us (with
-//   sixteen predecessors in every round, as all that follows; 174 without). What a
+//   sixteen predecessors in every round and words of their own for A, B and the carry, as all that follows). What a
 //   chunk reads back of its predecessors is as wide as the chunk and as long as there are chunks of its channels in
 //   flight, so tall and narrow is cheap: 16 lanes 191 and 219 us. 4 lanes take less than a memory line of a row: 273 and 250.
 //   8 rows a thread forward (4 backward, which holds twice as many arrays): 167 registers, 3 wavefronts a SIMD. 16 (8) rows leave
