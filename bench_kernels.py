@@ -72,7 +72,7 @@ def main() -> int:
         print(json.dumps({"kernel": kernel, "dtype": dt, "shape": shape, "us": round(us, 1), "achieved": round(ach, 1),
                           "unit": unit, "peak": peak, "frac": round(ach / peak, 3)}), flush=True)
 
-    groups = ("ew", "agg", "pipeline", "reorg", "tall", "gemm", "dnn", "train", "solve")
+    groups = ("ew", "agg", "pipeline", "reorg", "tall", "gemm", "dnn", "train", "seq", "solve")
 
     def want(group):
         # --only takes a group name (runs that group) or a substring of a kernel name (runs all, prints the matches)
@@ -281,6 +281,37 @@ def main() -> int:
             emit("conv2DBackwardFilter 32->64 ch, 14x14, 5x5 pad 2 (image resident in LDS, slabs per workgroup)", dt, f"batch {Nc}",
                  timed(lambda: K.conv2DBackwardFilter(dwc, xc, dyc, 1, 1, 2, 2, Nc, 32, 14, 14, 64, 32, 5, 5, ctx)), flops=fl)
             for m in (x, dy, gam, zer, dpool, dxp, xc, wc, dyc, dxc, dwc, *res_bn):
+                m.destroy()
+        # --- sequence models ---------------------------------------------------------------------------------------
+        if want("seq"):
+            def rnd(r, c):
+                return DM.from_torch(ctx, torch.randn(r, c, device="cuda", dtype=tdt, generator=gen))
+
+            n, vocab, w = 16384, 65536, 2048 if dt == "f32" else 1024
+            table, out, grad = rnd(vocab, w), DM(ctx, n, w, ndt), DM(ctx, vocab, w, ndt)
+            ids = DM.from_torch(ctx, (vocab ** torch.rand(n, 1, device="cuda", generator=gen)).long().clamp(max=vocab - 1))
+            distinct = len(np.unique(ids.to_numpy()))
+            with ctx.deferred_checks():
+                emit("embeddingForward", dt, f"{n} of {vocab} x {w}", timed(lambda: K.embeddingForward(out, table, ids, 1.0, ctx)), (n + distinct) * w * sz)
+                emit("embeddingBackward", dt, f"{n} of {vocab} x {w}", timed(lambda: K.embeddingBackward(grad, out, ids, vocab, 1.0, ctx)),
+                     (n + vocab) * w * sz)
+            x, z, h, y = rnd(n, w), rnd(n, w), DM(ctx, n, w, ndt), DM(ctx, n, w, ndt)
+            inv, dg, gam = DM(ctx, n, 1, ndt), DM(ctx, 1, w, ndt), rnd(1, w)
+            emit("rmsNormForward (residual, sum kept)", dt, f"{n}x{w}", timed(lambda: K.rmsNormForward(y, h, inv, x, z, gam, 1e-5, ctx)), 4 * n * w * sz)
+            emit("rmsNormBackward", dt, f"{n}x{w}", timed(lambda: K.rmsNormBackward(y, dg, h, inv, gam, x, z, ctx)), 4 * n * w * sz)
+            emit("gatedRecurrenceForward, 4 sequences", dt, f"{n}x{w}",
+                 timed(lambda: K.gatedRecurrenceForward(h, None, x, z, None, None, 4, ctx)), 3 * n * w * sz)
+            emit("gatedRecurrenceBackward, 4 sequences", dt, f"{n}x{w}",
+                 timed(lambda: K.gatedRecurrenceBackward(y, out, None, x, z, h, None, x, None, None, 4, ctx)), 6 * n * w * sz)
+            if dt == "f32":
+                k, o = 8192, 16384
+                wt = rnd(o, k)
+                codes, scales = K.quantizeQ4(None, None, wt, 128, ctx)
+                for r in (1, 16):
+                    xr, yr = rnd(r, k), DM(ctx, r, o, ndt)
+                    emit("matVecQ4, groups of 128", dt, f"{r} x {k} by {o}", timed(lambda: K.matVecQ4(yr, xr, None, codes, scales, 128, ctx)),
+                         o * k // 2 + o * k // 128 * 4 + r * (k + o) * 4)
+            for m in (table, out, grad, ids, x, z, h, y, inv, dg, gam):
                 m.destroy()
         # --- solve -------------------------------------------------------------------------------------------
         if want("solve"):
