@@ -71,26 +71,27 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, const T *table, size_t voc
     unsigned lpr = 1;
     while (lpr < THREADS && lpr < wv)
         lpr <<= 1;
-    const size_t gx = dh_ceil_div(n, THREADS / lpr);
     // Rows of more vectors than a workgroup has threads: four in flight a thread (16384 x 2048 in 40 us, with one 47); shorter rows
     // have none to give it (65536 x 256: 18 us, with four 22).
     const bool four = wv > lpr;
     const size_t gy = dh_ceil_div(wv, static_cast<size_t>(lpr) * (four ? 4 : 1));
-    if (gx >= (size_t(1) << 31) || gy >= 65536)
+    if (gy >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "embeddingForward - extents exceed one launch");
-    const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
+    const size_t each = dh_seq::MOST_GROUPS * (THREADS / lpr);
+    for (size_t i0 = 0; i0 < n; i0 += each) {
+        const size_t m = n - i0 < each ? n - i0 : each;
+        const dim3 grid(static_cast<unsigned>(dh_ceil_div(m, THREADS / lpr)), static_cast<unsigned>(gy));
 #define DH_EMBED_FORWARD(VEC, UN)                                                                                                          \
-    hipLaunchKernelGGL((forward_kernel<T, VEC, UN>), grid, dim3(THREADS), 0, ctx->stream, res, ld_res, table, ld_table,                   \
-                       static_cast<long long>(vocab), width, ids, ld_ids, n, scale, lpr, rec)
-    if (vec && four)
-        DH_EMBED_FORWARD(V, 4);
-    else if (vec)
-        DH_EMBED_FORWARD(V, 1);
-    else if (four)
-        DH_EMBED_FORWARD(1, 4);
-    else
-        DH_EMBED_FORWARD(1, 1);
+    hipLaunchKernelGGL((forward_kernel<T, VEC, UN>), grid, dim3(THREADS), 0, ctx->stream, res + i0 * ld_res, ld_res, table, ld_table,     \
+                       static_cast<long long>(vocab), width, ids + i0 * ld_ids, ld_ids, m, scale, lpr, rec)
+        if (vec && four)
+            DH_EMBED_FORWARD(V, 4);
+        else if (vec)
+            DH_EMBED_FORWARD(V, 1);
+        else
+            DH_EMBED_FORWARD(1, 1); // fewer values than a vector has
 #undef DH_EMBED_FORWARD
+    }
     DH_CHECK_LAUNCH();
     return dh_checked_end(ctx);
 }
@@ -103,39 +104,40 @@ __global__ __launch_bounds__(THREADS) void backward_scan_kernel(T *d_table, size
                                                                 int accumulate, int *rec) {
     __shared__ unsigned hits[THREADS];
     __shared__ unsigned count[THREADS / DH_WAVE];
-    const long long v = static_cast<long long>(blockIdx.x);
     const size_t col = static_cast<size_t>(blockIdx.y) * THREADS + threadIdx.x;
     const unsigned wave = threadIdx.x / DH_WAVE, lane = threadIdx.x % DH_WAVE;
-    double acc = 0.0;
-    bool any = false;
-    for (size_t base = 0; base < n; base += THREADS) {
-        const size_t i = base + threadIdx.x;
-        const long long id = i < n ? ids[i * ld_ids] : -1;
-        if (blockIdx.x == 0 && blockIdx.y == 0 && i < n && (id < 0 || id >= vocab))
-            dh_raise(rec, DH_DEFERRED_TOKEN_ID, 0, id, vocab);
-        const bool hit = i < n && id == v;
-        const unsigned long long mask = __ballot(hit);
-        if (lane == 0)
-            count[wave] = __popcll(mask);
-        __syncthreads();
-        unsigned at = __popcll(mask & ((1ull << lane) - 1)), total = 0;
-        for (unsigned w = 0; w < THREADS / DH_WAVE; w++) {
-            at += w < wave ? count[w] : 0;
-            total += count[w];
+    for (long long v = blockIdx.x; v < (vocab ? vocab : 1); v += gridDim.x) {
+        double acc = 0.0;
+        bool any = false;
+        for (size_t base = 0; base < n; base += THREADS) {
+            const size_t i = base + threadIdx.x;
+            const long long id = i < n ? ids[i * ld_ids] : -1;
+            if (v == 0 && blockIdx.y == 0 && i < n && (id < 0 || id >= vocab))
+                dh_raise(rec, DH_DEFERRED_TOKEN_ID, 0, id, vocab);
+            const bool hit = i < n && id == v;
+            const unsigned long long mask = __ballot(hit);
+            if (lane == 0)
+                count[wave] = __popcll(mask);
+            __syncthreads();
+            unsigned at = __popcll(mask & ((1ull << lane) - 1)), total = 0;
+            for (unsigned w = 0; w < THREADS / DH_WAVE; w++) {
+                at += w < wave ? count[w] : 0;
+                total += count[w];
+            }
+            if (hit)
+                hits[at] = threadIdx.x;
+            __syncthreads();
+            any |= total != 0;
+            if (col < width)
+                for (unsigned k = 0; k < total; k++)
+                    acc += static_cast<double>(d_out[(base + hits[k]) * ld_out + col]);
+            __syncthreads();
         }
-        if (hit)
-            hits[at] = threadIdx.x;
-        __syncthreads();
-        any |= total != 0;
-        if (col < width)
-            for (unsigned k = 0; k < total; k++)
-                acc += static_cast<double>(d_out[(base + hits[k]) * ld_out + col]);
-        __syncthreads();
-    }
-    if (col < width && (any || !accumulate)) {
-        T *p = d_table + static_cast<size_t>(v) * ld + col;
-        const double s = any ? acc * static_cast<double>(scale) : 0.0;
-        *p = static_cast<T>(accumulate ? s + static_cast<double>(*p) : s);
+        if (col < width && (any || !accumulate)) {
+            T *p = d_table + static_cast<size_t>(v) * ld + col;
+            const double s = any ? acc * static_cast<double>(scale) : 0.0;
+            *p = static_cast<T>(accumulate ? s + static_cast<double>(*p) : s);
+        }
     }
 }
 
@@ -829,8 +831,8 @@ dh_status backward(dh_ctx *ctx, T *d_table, size_t vocab, size_t width, size_t l
         DH_CHECK_LAUNCH();
         return dh_checked_end(ctx);
     }
-    const size_t gy = dh_ceil_div(width, THREADS), gx = vocab ? vocab : 1;
-    if (gx >= (size_t(1) << 31) || gy >= 65536)
+    const size_t gy = dh_ceil_div(width, THREADS), gx = vocab == 0 ? 1 : vocab < dh_seq::MOST_GROUPS ? vocab : dh_seq::MOST_GROUPS;
+    if (gy >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "embeddingBackward - extents exceed one launch");
     hipLaunchKernelGGL((backward_scan_kernel<T>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), dim3(THREADS), 0, ctx->stream,
                        d_table, ld, static_cast<long long>(vocab), vocab ? width : 0, d_out, ld_out, ids, ld_ids, n, scale, accumulate, rec);

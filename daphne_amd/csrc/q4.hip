@@ -9,7 +9,7 @@
 // One row, 4096 x 8192: 8.2 us with its launch (18 MB; at the rate of a copy 3.5); 16384 x 16384 44 us (143 MB, 3.2 TB/s).
 // 16 rows of floats, 8192 x 16384, 35 us: there the splitting and decoding bind; 16 rows of 8 bits, with the norm that makes them,
 // 28 us.
-#include "common.h"
+#include "seq_common.h"
 
 #include <type_traits>
 
@@ -371,7 +371,7 @@ dh_status matvec(dh_ctx *ctx, float *res, size_t ld_res, const X *x, size_t rows
     if (rows > 0 && outs > 0 &&
         (res == nullptr || (cols > 0 && (x == nullptr || codes == nullptr || scales == nullptr)) || (sizeof(X) == 1 && x_scale == nullptr)))
         return dh_fail(DH_ERR_RUNTIME, "%s - a matrix is null", what);
-    if (cols >= (size_t(1) << 25) || outs >= (size_t(1) << 31) || dh_ceil_div(rows, 16) >= 65536)
+    if (cols >= (size_t(1) << 25) || outs >= (size_t(1) << 27) || dh_ceil_div(rows, 16) >= 65536)
         return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
     DH_REQUIRE_CTX(ctx);
     if (rows == 0 || outs == 0)
@@ -396,31 +396,31 @@ dh_status matvec(dh_ctx *ctx, float *res, size_t ld_res, const X *x, size_t rows
 static __global__ __launch_bounds__(THREADS) void quantize_kernel(unsigned char *codes, size_t ld_codes, float *scales, size_t ld_scales,
                                                                   const float *w, size_t rows, size_t cols, size_t ld, size_t group,
                                                                   size_t groups) {
-    const size_t job = static_cast<size_t>(blockIdx.x) * (THREADS / DH_WAVE) + threadIdx.x / DH_WAVE;
-    if (job >= rows * groups)
-        return;
-    const size_t r = job / groups, g = job % groups, c0 = g * group, c1 = c0 + group < cols ? c0 + group : cols;
-    const unsigned lane = threadIdx.x % DH_WAVE;
-    const float *row = w + r * ld;
-    float most = 0.f;
-    for (size_t c = c0 + lane; c < c1; c += DH_WAVE) {
-        const float v = fabsf(row[c]);
-        most = most != most ? most : (v != v || v > most ? v : most);
-    }
-    dh_butterfly(DH_WAVE, [&](auto peer) {
-        const float o = peer(most);
-        most = most != most ? most : (o != o || o > most ? o : most);
-    });
-    const bool finite = most <= 3.402823466e38f;
-    const float scale = finite ? most / 7.0f : dh_nan<float>();
-    if (lane == 0)
-        scales[r * ld_scales + g] = scale;
-    // in 64 bits: the quotient of two floats is never rounded onto a border between two codes
-    const double to_code = finite && most > 0.f ? 7.0 / static_cast<double>(most) : 0.0;
-    for (size_t b = c0 / 2 + lane; 2 * b < c1; b += DH_WAVE) {
-        const int lo = finite ? static_cast<int>(rint(static_cast<double>(row[2 * b]) * to_code)) : 0;
-        const int hi = finite && 2 * b + 1 < cols ? static_cast<int>(rint(static_cast<double>(row[2 * b + 1]) * to_code)) : 0;
-        codes[r * ld_codes + b] = static_cast<unsigned char>((lo & 15) | ((hi & 15) << 4));
+    for (size_t job = static_cast<size_t>(blockIdx.x) * (THREADS / DH_WAVE) + threadIdx.x / DH_WAVE; job < rows * groups;
+         job += static_cast<size_t>(gridDim.x) * (THREADS / DH_WAVE)) {
+        const size_t r = job / groups, g = job % groups, c0 = g * group, c1 = c0 + group < cols ? c0 + group : cols;
+        const unsigned lane = threadIdx.x % DH_WAVE;
+        const float *row = w + r * ld;
+        float most = 0.f;
+        for (size_t c = c0 + lane; c < c1; c += DH_WAVE) {
+            const float v = fabsf(row[c]);
+            most = most != most ? most : (v != v || v > most ? v : most);
+        }
+        dh_butterfly(DH_WAVE, [&](auto peer) {
+            const float o = peer(most);
+            most = most != most ? most : (o != o || o > most ? o : most);
+        });
+        const bool finite = most <= 3.402823466e38f;
+        const float scale = finite ? most / 7.0f : dh_nan<float>();
+        if (lane == 0)
+            scales[r * ld_scales + g] = scale;
+        // in 64 bits: the quotient of two floats is never rounded onto a border between two codes
+        const double to_code = finite && most > 0.f ? 7.0 / static_cast<double>(most) : 0.0;
+        for (size_t b = c0 / 2 + lane; 2 * b < c1; b += DH_WAVE) {
+            const int lo = finite ? static_cast<int>(rint(static_cast<double>(row[2 * b]) * to_code)) : 0;
+            const int hi = finite && 2 * b + 1 < cols ? static_cast<int>(rint(static_cast<double>(row[2 * b + 1]) * to_code)) : 0;
+            codes[r * ld_codes + b] = static_cast<unsigned char>((lo & 15) | ((hi & 15) << 4));
+        }
     }
 }
 
@@ -448,9 +448,8 @@ extern "C" dh_status dh_quantize_q4_f32(dh_ctx *ctx, uint8_t *codes, size_t ld_c
     DH_REQUIRE_CTX(ctx);
     if (rows == 0 || cols == 0)
         return DH_OK;
-    const size_t groups = dh_ceil_div(cols, group), gx = dh_ceil_div(rows * groups, dh_q4::THREADS / DH_WAVE);
-    if (gx >= (size_t(1) << 31))
-        return dh_fail(DH_ERR_RUNTIME, "quantizeQ4 - extents exceed one launch");
+    const size_t groups = dh_ceil_div(cols, group), all = dh_ceil_div(rows * groups, dh_q4::THREADS / DH_WAVE);
+    const size_t gx = all < dh_seq::MOST_GROUPS ? all : dh_seq::MOST_GROUPS;
     hipLaunchKernelGGL(dh_q4::quantize_kernel, dim3(static_cast<unsigned>(gx)), dim3(dh_q4::THREADS), 0, ctx->stream, codes, ld_codes, scales,
                        ld_scales, w, rows, cols, ld, group, groups);
     DH_CHECK_LAUNCH();

@@ -666,7 +666,7 @@ dh_status scan(dh_ctx *ctx, const char *what, ScanArgs<T> &a, const Plan &p, voi
     const size_t need = plan_bytes<T>(p);
     if (dh_status st = dh_call_workspace(ctx, what, ws, ws_bytes, need, &work); st != DH_OK)
         return st;
-    if (p.blocks * p.chunks >= (size_t(1) << 31) || a.num_seq >= (size_t(1) << 32))
+    if (p.blocks * p.chunks >= (size_t(1) << 32) / THREADS || a.num_seq >= (size_t(1) << 32))
         return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
     a.blocks = p.blocks;
     a.chunks = p.chunks;
@@ -710,7 +710,7 @@ dh_status forward(dh_ctx *ctx, T *res, size_t ld_res, T *last, size_t ld_last, c
     const Spans sp{offsets, ld_offsets, tokens / num_seq, tokens};
     if (tokens == 0 || (offsets == nullptr && sp.even <= SERIAL_ROWS)) {
         const size_t gx = dh_ceil_div(channels, THREADS), gy = num_seq < 65535 ? num_seq : 65535;
-        if (gx >= (size_t(1) << 31))
+        if (gx >= (size_t(1) << 32) / THREADS)
             return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
         hipLaunchKernelGGL((forward_serial_kernel<T>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), dim3(THREADS), 0,
                            ctx->stream, res, ld_res, last, ld_last, x, ld_x, z, ld_z, h0, ld_h0, sp, num_seq, channels, rec);
@@ -749,7 +749,7 @@ dh_status backward(dh_ctx *ctx, T *d_x, size_t ld_dx, T *d_z, size_t ld_dz, T *d
     const Spans sp{offsets, ld_offsets, tokens / num_seq, tokens};
     if (tokens == 0 || (offsets == nullptr && sp.even <= SERIAL_ROWS)) {
         const size_t gx = dh_ceil_div(channels, THREADS), gy = num_seq < 65535 ? num_seq : 65535;
-        if (gx >= (size_t(1) << 31))
+        if (gx >= (size_t(1) << 32) / THREADS)
             return dh_fail(DH_ERR_RUNTIME, "%s - extents exceed one launch", what);
         hipLaunchKernelGGL((backward_serial_kernel<T>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), dim3(THREADS), 0,
                            ctx->stream, d_x, ld_dx, d_z, ld_dz, d_h0, ld_dh0, x, ld_x, z, ld_z, h, ld_h, h0, ld_h0, d_out, ld_do, d_last,

@@ -224,8 +224,24 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void forward_kerne
 
 template <typename T, int VEC, int TPR, int KV, bool Q8> static inline void launch_forward(dh_ctx *ctx, const ForwardArgs<T> &a) {
     constexpr int WG = TPR > THREADS ? TPR : THREADS;
-    hipLaunchKernelGGL((forward_kernel<T, VEC, TPR, KV, Q8>), dim3(static_cast<unsigned>(dh_ceil_div(a.rows, WG / TPR))), dim3(WG), 0,
-                       ctx->stream, a);
+    constexpr size_t EACH = dh_seq::MOST_GROUPS * (WG / TPR);
+    for (size_t r = 0; r < a.rows; r += EACH) {
+        ForwardArgs<T> b = a;
+        b.rows = a.rows - r < EACH ? a.rows - r : EACH;
+        b.x += r * a.ld_x;
+        if constexpr (Q8)
+            b.codes += r * a.ld_res, b.scale += r;
+        else
+            b.res += r * a.ld_res;
+        if (a.sum)
+            b.sum += r * a.ld_sum;
+        if (a.inv_rms)
+            b.inv_rms += r;
+        if (a.residual)
+            b.residual += r * a.ld_r;
+        hipLaunchKernelGGL((forward_kernel<T, VEC, TPR, KV, Q8>), dim3(static_cast<unsigned>(dh_ceil_div(b.rows, WG / TPR))), dim3(WG), 0,
+                           ctx->stream, b);
+    }
 }
 
 // The shape of a row of so many vectors: calls use(Shape), the first one that holds the row; KV = 0 holds none and takes any.
@@ -403,48 +419,50 @@ __global__ __launch_bounds__((TPR > THREADS ? TPR : THREADS)) void backward_kern
 template <typename T> __global__ __launch_bounds__(1024) void backward_rows_kernel(BackwardArgs<T> a) {
     constexpr int VEC = dh_vec<T>::N;
     __shared__ double slots[1024 / DH_WAVE];
-    const size_t row = blockIdx.x, vecs = (a.cols + VEC - 1) / VEC;
-    const T *h = a.h + row * a.ld_h, *dy = a.dy + row * a.ld_dy, *ds = a.dsum ? a.dsum + row * a.ld_ds : nullptr;
-    T *dx = a.dx + row * a.ld_dx;
-    const T inv = a.inv_rms[row];
-    T hv[VEC], yv[VEC], gv[VEC], sv[VEC];
-    auto read = [&](size_t at) {
-        dh_seq::load<T, VEC>(h + at, hv);
-        dh_seq::load<T, VEC>(dy + at, yv);
-        if (a.gamma)
-            dh_seq::load<T, VEC>(a.gamma + at, gv);
-        else
+    const size_t vecs = (a.cols + VEC - 1) / VEC;
+    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *h = a.h + row * a.ld_h, *dy = a.dy + row * a.ld_dy, *ds = a.dsum ? a.dsum + row * a.ld_ds : nullptr;
+        T *dx = a.dx + row * a.ld_dx;
+        const T inv = a.inv_rms[row];
+        T hv[VEC], yv[VEC], gv[VEC], sv[VEC];
+        auto read = [&](size_t at) {
+            dh_seq::load<T, VEC>(h + at, hv);
+            dh_seq::load<T, VEC>(dy + at, yv);
+            if (a.gamma)
+                dh_seq::load<T, VEC>(a.gamma + at, gv);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    gv[e] = T(1);
+        };
+        double dot = 0.0;
+#pragma unroll 4
+        for (size_t j = threadIdx.x; j < vecs; j += 1024) {
+            const dh_seq::Piece at = dh_seq::piece<VEC>(j, a.cols);
+            read(at.at);
 #pragma unroll
             for (int e = 0; e < VEC; e++)
-                gv[e] = T(1);
-    };
-    double dot = 0.0;
-#pragma unroll 4
-    for (size_t j = threadIdx.x; j < vecs; j += 1024) {
-        const dh_seq::Piece at = dh_seq::piece<VEC>(j, a.cols);
-        read(at.at);
-#pragma unroll
-        for (int e = 0; e < VEC; e++)
-            dot += static_cast<size_t>(e) >= at.shift ? static_cast<double>(yv[e]) * static_cast<double>(hv[e]) * static_cast<double>(gv[e]) : 0.0;
-    }
-    dot = over_row<1024>(dot, slots, Add());
-    const T m = static_cast<T>(dot / static_cast<double>(a.cols) * static_cast<double>(inv) * static_cast<double>(inv));
-    // A moved last vector shares values with the one before it, which may be written by then where dx takes an input's place:
-    // only values of its own are stored, and those nobody else writes.
-#pragma unroll 4
-    for (size_t j = threadIdx.x; j < vecs; j += 1024) {
-        const dh_seq::Piece at = dh_seq::piece<VEC>(j, a.cols);
-        read(at.at);
-        if (ds)
-            dh_seq::load<T, VEC>(ds + at.at, sv);
-        T v[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            v[e] = inv * (yv[e] * gv[e] - hv[e] * m);
-            if (ds)
-                v[e] += sv[e];
+                dot += static_cast<size_t>(e) >= at.shift ? static_cast<double>(yv[e]) * static_cast<double>(hv[e]) * static_cast<double>(gv[e]) : 0.0;
         }
-        dh_seq::store<T, VEC>(dx + at.at, v, at.shift);
+        dot = over_row<1024>(dot, slots, Add());
+        const T m = static_cast<T>(dot / static_cast<double>(a.cols) * static_cast<double>(inv) * static_cast<double>(inv));
+        // A moved last vector shares values with the one before it, which may be written by then where dx takes an input's place:
+        // only values of its own are stored, and those nobody else writes.
+#pragma unroll 4
+        for (size_t j = threadIdx.x; j < vecs; j += 1024) {
+            const dh_seq::Piece at = dh_seq::piece<VEC>(j, a.cols);
+            read(at.at);
+            if (ds)
+                dh_seq::load<T, VEC>(ds + at.at, sv);
+            T v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                v[e] = inv * (yv[e] * gv[e] - hv[e] * m);
+                if (ds)
+                    v[e] += sv[e];
+            }
+            dh_seq::store<T, VEC>(dx + at.at, v, at.shift);
+        }
     }
 }
 
@@ -513,7 +531,7 @@ template <typename T> dh_status backward(dh_ctx *ctx, const BackwardArgs<T> &a, 
                 if (partials) // before d_x, which may take the place of d_y
                     hipLaunchKernelGGL((gamma_kernel<T>), dim3(static_cast<unsigned>(dh_ceil_div(a.cols, THREADS)), static_cast<unsigned>(groups)),
                                        dim3(THREADS), 0, ctx->stream, a, partials);
-                hipLaunchKernelGGL((backward_rows_kernel<T>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, ctx->stream, a);
+                hipLaunchKernelGGL((backward_rows_kernel<T>), dim3(static_cast<unsigned>(a.rows < dh_seq::MOST_GROUPS ? a.rows : dh_seq::MOST_GROUPS)), dim3(1024), 0, ctx->stream, a);
             } else {
                 constexpr int WG = TPR > THREADS ? TPR : THREADS;
                 const size_t fit = dh_ceil_div(a.rows, WG / TPR);

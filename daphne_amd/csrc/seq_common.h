@@ -39,6 +39,10 @@ template <typename T, int VEC> __device__ __forceinline__ void load_stream(const
     }
 }
 
+// Most workgroups of one launch along x, far below where a grid's threads no longer count in 32 bits. What needs more takes several
+// launches, or several turns of a workgroup.
+constexpr size_t MOST_GROUPS = size_t(1) << 20;
+
 // Vector j of n values: where it begins, and how many of its values belong to the vector before it.
 struct Piece {
     size_t at;

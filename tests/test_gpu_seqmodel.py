@@ -961,3 +961,32 @@ def test_two_captured_graphs_of_one_workspace_in_turn(ctx):
     finally:
         c.sync()
         c.destroy()
+
+
+def test_more_rows_than_one_launch_takes(ctx):
+    torch = pytest.importorskip("torch")
+    rows = (1 << 22) + 3
+    rng = np.random.default_rng(51)
+    x, r, g = rng.standard_normal((rows, 2)).astype(F32), rng.standard_normal((rows, 2)).astype(F32), np.array([[0.5, 2]], F32)
+    res, total, inv = rmsNormForward(None, DenseMatrix(ctx, rows, 2, F32), DenseMatrix(ctx, rows, 1, F32), D(ctx, x), D(ctx, r), D(ctx, g), 1e-5, ctx)
+    h, w_inv, y = norm_forward(x, r, g, 1e-5, F32)
+    rel = 2 * U(F32)  # the mean's and the root's own roundings, and inv's to 32 bits
+    np.testing.assert_array_equal(total.to_numpy(), h)
+    near(inv.to_numpy(), w_inv, rel * w_inv, "inv")
+    near(res.to_numpy(), y, (rel + 3 * U(F32)) * np.abs(y) * 1.001, "norm")
+    codes, scale = rmsNormForwardQ8(None, None, None, None, D(ctx, x), None, None, 1e-5, ctx)[:2]
+    assert np.all(np.abs(codes.to_numpy().astype(np.int32)).max(axis=1) == 127)
+    near(scale.to_numpy() * 127, np.abs(norm_forward(x, None, None, 1e-5, F32)[2]).max(axis=1, keepdims=True), 8 * U(F32) * 10)
+    c, s = quantizeQ4(None, None, D(ctx, x), 32, ctx)
+    big = np.abs(x).argmax(axis=1)
+    np.testing.assert_array_equal(s.to_numpy(), np.abs(x).max(axis=1, keepdims=True) / F32(7))
+    four = (c.to_numpy()[:, 0] >> (4 * big)) & 15
+    np.testing.assert_array_equal(four, np.where(x[np.arange(rows), big] > 0, 7, 9))
+    n = (1 << 20) + 5
+    table, ids = torch.randn(100, 1024, device="cuda"), torch.randint(0, 100, (n, 1), device="cuda")
+    out = torch.zeros(n, 1024, device="cuda")
+    torch.cuda.synchronize()
+    embeddingForward(DenseMatrix.from_torch(ctx, out), DenseMatrix.from_torch(ctx, table), DenseMatrix.from_torch(ctx, ids), 1.0, ctx)
+    ctx.sync()
+    for part in (slice(0, 3), slice((1 << 20) - 4, n)):
+        assert torch.equal(out[part], table[ids[part, 0]])
