@@ -7,8 +7,8 @@
 // the products go to the matrix cores, which leaves the ALUs to the decoding. Codes are two to a byte, row by row, the even
 // column in the low half.
 // One row, 4096 x 8192: 8.2 us with its launch (18 MB; at the rate of a copy 3.5); 16384 x 16384 44 us (143 MB, 3.2 TB/s).
-// 16 rows of floats, 8192 x 16384, 35 us: there the splitting and decoding bind; 16 rows of 8 bits, with the norm that makes them,
-// 28 us.
+// 16 rows of floats, 8192 x 16384, 34 us (with x requested when it is needed 35; 4 rows 23.0 and 26.4): there the splitting and
+// decoding bind; 16 rows of 8 bits, with the norm that makes them, 28 us.
 #include "seq_common.h"
 
 #include <type_traits>
@@ -101,7 +101,7 @@ struct Bytes {
 };
 
 // WHOLE: groups are whole steps, so that a step has one scale. MT: rows of x that are staged (floats), a power of two: all 16, of
-// which one exists, take 46 us for 21.5 (8192 x 16384), and 35 for 30 with eight.
+// which one exists, took 46 us for 21.5 (8192 x 16384), and 35 for 30 with eight.
 template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WAVES *DH_WAVE) void matvec_kernel(Args<X> a) {
     constexpr bool FLOATS = sizeof(X) == 4;
     constexpr int CHUNKS = STEP / 32;
@@ -251,21 +251,27 @@ template <typename X, int T, bool WHOLE, int MT> __global__ __launch_bounds__(WA
             else if constexpr (MT == 1)
                 xf[u] = *reinterpret_cast<const f32x2_any *>(x + (s * STEP + 2 * lane < cols ? s * STEP + 2 * lane : 0));
         }
+        f32x2_any v[MT]; // several rows of x: the next step's are on their way while one is multiplied
+        auto request_x = [&](unsigned s) {
+            const unsigned k2 = (s < full ? s : full - 1) * STEP + 2 * lane;
+#pragma unroll
+            for (int r = 0; r < MT; r++)
+                v[r] = *reinterpret_cast<const f32x2_any *>(x + (static_cast<unsigned>(r) < M ? r : M - 1) * a.ld_x + (k2 < cols ? k2 : 0));
+        };
+        if constexpr (FLOATS && MT > 1)
+            request_x(sb);
         keep_scales(g0);
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             if (sb + u >= full)
                 break;
             if constexpr (FLOATS) {
-                f32x2_any v[MT];
-                const unsigned k2 = (sb + u) * STEP + 2 * lane;
-#pragma unroll
-                for (int r = 0; r < MT; r++)
-                    if constexpr (MT == 1)
-                        v[r] = xf[u];
-                    else
-                        v[r] = *reinterpret_cast<const f32x2_any *>(x + (static_cast<unsigned>(r) < M ? r : M - 1) * a.ld_x + (k2 < cols ? k2 : 0));
+                if constexpr (MT == 1)
+                    v[0] = xf[u];
                 stage(v);
+                if constexpr (MT > 1)
+                    if (u + 1 < AHEAD)
+                        request_x(sb + u + 1);
             }
             multiply(c[u], xq[u], sb + u, g0);
         }
@@ -381,8 +387,8 @@ dh_status matvec(dh_ctx *ctx, float *res, size_t ld_res, const X *x, size_t rows
                     dh_ceil_div(size_t(1) << 40, per_group)};
     // As many tiles a wavefront as leave every compute unit a workgroup: 8192 x 16384, one row by 1, 2 and 4 tiles 23.3, 21.4 and 22.5 us,
     // 4096 x 8192, which 4 tiles leave half the units, 8.2, 8.2 and 12.3. Four: where rows of floats are many, whose splitting
-    // then serves twice the outputs: 8192 x 16384, 16 rows 69, 46 and 35 us, 4 rows 30.0, 26.5 and 28.0; 16 rows of 8 bits, with
-    // the norm, 34.2, 28.2 and 30.4.
+    // then serves twice the outputs: 8192 x 16384, 16 rows 71, 42 and 34 us, 8 rows 38, 35 and 29, 4 rows 28.9, 23.2 and 24.0; 16
+    // rows of 8 bits, with the norm, 34.2, 28.2 and 30.4.
     const size_t row_tiles = dh_ceil_div(rows, 16), cus = static_cast<size_t>(ctx->num_cus);
     const bool whole = group % STEP == 0;
     if (sizeof(X) == 4 && rows > 4 && dh_ceil_div(outs, 64) * row_tiles >= cus)
