@@ -14,8 +14,8 @@
 // scan_kernel does it in one pass over the data (a chunk's inputs stay in registers from its composition to its
 // result), which makes it bound by memory: a workgroup composes its chunk, publishes the composition, looks back over its
 // predecessors' until it meets a carry that is already whole, publishes its own, and writes its rows. 32768 rows forward,
-// 2048 channels: 154 us (806 MB, 5.2 TB/s); backward, 1024 channels: 169 us (806 MB, 4.8 TB/s); a copy of as much: 155 us.
-// 64 bits: 100001 x 96 in 64 us (230 MB, 3.6 TB/s): two wavefronts a SIMD hide less of the looking back and of the exponentials.
+// 2048 channels: 153 us (806 MB, 5.3 TB/s); backward, 1024 channels: 168 us (806 MB, 4.8 TB/s); a copy of as much: 155 us.
+// 64 bits: 100001 x 96 in 63 us (230 MB, 3.7 TB/s): two wavefronts a SIMD hide less of the looking back and of the exponentials.
 #pragma once
 
 #include "seq_common.h"
@@ -252,23 +252,24 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
     static_assert(LB <= RG && FIRST <= LB);
     // ROW_*: which rows open the chain (take a given carry) and which close it (give their carry away), in scanning order
     constexpr int OPENS = BACK ? ROW_LAST : ROW_FIRST, CLOSES = BACK ? ROW_FIRST : ROW_LAST;
-    __shared__ unsigned long long ticket_lds;
+    __shared__ unsigned place_lds[2];
     __shared__ int flags[ROWS];
     __shared__ unsigned seq_of[ROWS];
     constexpr int SLOTS = LB > WAVES ? LB : WAVES;
     __shared__ T sA[SLOTS][CW], sB[SLOTS][CW]; // compositions of the wavefronts, then of the predecessors
     __shared__ int sOpen[SLOTS][LC];
     const unsigned tid = threadIdx.x, lc = tid % LC, g = tid / LC, wave = tid / DH_WAVE;
-    unsigned long long ticket = blockIdx.x;
+    size_t chunk = 0, block = blockIdx.x;
     if (a.ws) { // workgroups take chunks in the order in which they start, so that whoever is waited for is running
         if (tid == 0) {
-            const unsigned long long t = atomicAdd(a.ws, 1ull), all = static_cast<unsigned long long>(a.blocks) * a.chunks;
-            ticket_lds = t < all ? t : t % all; // more: another call is in this workspace; whatever it does, indexes stay in range
+            const unsigned blocks = static_cast<unsigned>(a.blocks), all = gridDim.x;
+            unsigned t = atomicAdd(reinterpret_cast<unsigned *>(a.ws), 1u);
+            t = t < all ? t : t % all; // more: another call is in this workspace; whatever it does, indexes stay in range
+            place_lds[0] = t / blocks, place_lds[1] = t % blocks;
         }
         __syncthreads();
-        ticket = ticket_lds;
+        chunk = place_lds[0], block = place_lds[1];
     }
-    const size_t chunk = ticket / a.blocks, block = ticket % a.blocks;
     const size_t c0 = block * CW + lc * VEC; // as the workspace counts channels; vectors behind the last one read it and write nothing
     const dh_seq::Piece piece = dh_seq::piece<VEC>(block * LC + lc, a.channels);
     const size_t cc = piece.at, shift = piece.shift;
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
         plain &= fl == ROW_LIVE;
     }
     if (a.sp.offsets) {
-        check_offsets(a.sp, a.num_seq, ticket * THREADS + tid, static_cast<size_t>(a.blocks * a.chunks) * THREADS, a.rec);
+        check_offsets(a.sp, a.num_seq, static_cast<size_t>(blockIdx.x) * THREADS + tid, static_cast<size_t>(a.blocks * a.chunks) * THREADS, a.rec);
         if (on) // sequences without rows hand their state on
             for (size_t s = chunk * RG + g; s < a.num_seq; s += a.chunks * RG)
                 if (a.sp.at(s) >= a.sp.at(s + 1)) {
@@ -604,8 +605,9 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(ScanArgs<T> a) {
 //   In 64 bits 12 and 7 rows, which leave two wavefronts: 64 us forward (100001 x 96) and 159 backward (32768 x 512); 8 and 4 rows 73
 //   and 178, 6 and 3, for three wavefronts, 77 and 182, 14 rows, for one, 77.
 // Without any look-back (sequences as long as a chunk) the same rows take 147 and 157 us, a plain copy of as many bytes 155.
-// Rows that do not begin at memory lines (2047 and 1023 channels) have every line in two chunks: 237 and 250 us by way of the
-// caches, 315 and 308 past them.
+// Rows that do not begin at memory lines (2047 and 1023 channels) have every line in two chunks: 232 and 237 us by way of the
+// caches (past them 315 and 308 for 237 and 250). Giving each XCD neighbouring channels, so that the two meet in one L2, gains where
+// there are many (3333: 103 us for 108) and loses where there are few (1023: 132 for 124).
 constexpr int LANES = 8;
 template <typename T> constexpr int rows_of(bool back) { return sizeof(T) == 4 ? (back ? 4 : 8) : (back ? 7 : 12); }
 
